@@ -293,15 +293,16 @@ def _sampling(s):
     before = (sums - mass).double()
     inside = (before < top_p.double() * sums[:, -1:].double()) | (top_p >= 1)
     inside[:, 0] = True
+    inside &= weight.gather(1, order) >= min_p
     mass = torch.where(inside, mass, 0)
-    kept = torch.zeros_like(fixed).scatter_(1, order, mass)
-    kept = torch.where(weight >= min_p, kept, 0)
-    sums = kept.cumsum(-1)
+    # the token at the random share of what is kept, from the most likely token on
+    sums = mass.cumsum(-1)
     total = sums[:, -1:]
     target = (s["uniforms"][:, None].double() * total.double()).long()
     target = torch.minimum(target, total - 1)
-    token = (sums > target).long().argmax(-1, keepdim=True)
-    prob = (kept.gather(1, token).double() / total.double()).float()
+    at = (sums > target).long().argmax(-1, keepdim=True)
+    token = order.gather(1, at)
+    prob = (mass.gather(1, at).double() / total.double()).float()
     none = total == 0
     return {"tokens": torch.where(none, -1, token)[:, 0], "probs": torch.where(none, 0.0, prob)[:, 0]}
 
@@ -391,9 +392,9 @@ def _exact_sampling(case, s):
             ahead = torch.cat([q.new_zeros(1), q.cumsum(0)[:-1]])
             q = torch.where(ahead < float(s["top_p"][i]), q, 0.0)
         q = torch.where(p[index] >= float(s["min_p"][i]) * p.max(), q, 0.0)
-        p = torch.zeros_like(p).scatter(0, index, q / q.sum())
-        token = int(torch.searchsorted(p.cumsum(0), float(s["uniforms"][i]), right=True))
-        probs.append(p[min(token, len(x) - 1)])
+        q = q / q.sum()
+        token = int(torch.searchsorted(q.cumsum(0), float(s["uniforms"][i]), right=True))
+        probs.append(q[min(token, len(x) - 1)])
     return {"tokens": None, "probs": torch.stack(probs)}
 
 
