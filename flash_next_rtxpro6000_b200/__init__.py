@@ -13,6 +13,11 @@ the hand-written CUDA library ``_fnx.so``):
   and its softmax top-k routing table (fused into one launch by ``router_topk``);
 * ``draft_topk1_postprocess``, ``draft_head_topk1`` -- the greedy draft step with the
   hot-vocabulary token map (the latter fused into the draft head's argmax);
+* ``rotary_table``, ``rotary_append`` -- rotary positions and the append of keys and values to
+  a paged cache, in one launch;
+* ``tree_layout``, ``tree_attention`` -- attention of drafted token trees over a paged cache
+  (one node a request: decode);
+* ``sample_tokens`` -- temperature, top-k, top-p and min-p sampling from given random numbers;
 * ``nvfp4_dense`` -- the NVFP4 dense lm_head: load-time packing with an on-disk cache
   and the linear method serving it through the NVFP4 GEMV;
 * ``sharded`` -- vocab-sharded lm_head and expert-sharded MoE over torch.distributed;
@@ -60,5 +65,8 @@ from .draft_moe_gemv import (  # noqa: F401
 from .errors import DeviceWaitError, check_device_errors  # noqa: F401
 from .router import covered, route_softmax_fast, router_gemv, router_topk  # noqa: F401
 from .draft_topk1 import draft_head_topk1, draft_topk1_postprocess  # noqa: F401
+from .rotary import RotaryScaling, rotary_append, rotary_table  # noqa: F401
+from .sampling import sample_tokens  # noqa: F401
+from .tree_attention import tree_attention, tree_layout  # noqa: F401
 
 __version__ = "0.1.0"

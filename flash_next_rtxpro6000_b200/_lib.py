@@ -15,6 +15,7 @@ from .build import LIB_PATH
 FNX_OK, FNX_EINVAL, FNX_ECUDA, FNX_EUNSUPPORTED = 0, 1, 2, 3
 W_INT8, W_FP8_E4M3, W_BF16, W_NVFP4 = 0, 1, 2, 3
 SCALE_NONE, SCALE_F32_SCALAR, SCALE_F32_ROW, SCALE_BF16_SCALAR, SCALE_BF16_ROW = 0, 1, 2, 3, 4
+T_BF16, T_F16, T_F32 = 0, 1, 2
 MAX_M = 16
 STATIC_PARTIAL_FLOATS, STATIC_COUNTERS = 256 * 1024, 2048  # fnx_w8a16_gemv_static_ws limits
 PEER_BUFFER_BYTES, IPC_HANDLE_BYTES, MAX_PEERS = 4096, 64, 8
@@ -31,6 +32,11 @@ DEVICE_ERRORS = {
     9: "ROUTES: a routing table the kernel cannot hold",
     10: "WAIT_EXPERT: a down projection waited for its expert's activations",
     11: "RING: a launch whose ring stages the waits cannot order",
+    12: "POSITION: a position outside the rotary table",
+    13: "SLOT: a cache slot outside the cache",
+    14: "LENGTHS: lengths that contradict each other or the bounds given",
+    15: "PAGE: a page number outside the cache",
+    16: "TREE: a parent that is not an earlier node",
 }
 
 EXPORTED = (
@@ -62,6 +68,11 @@ EXPORTED = (
     "fnx_moe_gemv",
     "fnx_argmax_decode",
     "fnx_static_ws_error",
+    "fnx_rotary_append",
+    "fnx_tree_layout",
+    "fnx_tree_attention_workspace_floats",
+    "fnx_tree_attention",
+    "fnx_sample",
     "fnx_last_error",
     "fnx_version",
 )
@@ -193,6 +204,18 @@ def _declare(lib):
     lib.fnx_argmax_decode.argtypes = [_P, _P, c_int, _P]
     lib.fnx_peer_set_wait_limit.argtypes = [_P, c_int64]
     lib.fnx_static_ws_error.argtypes = [c_int, _P, POINTER(c_int)]
+    lib.fnx_rotary_append.argtypes = [
+        _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, _P,
+        c_int64, c_int64, _P, _I64P, _P, _I64P, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_int, _P, c_int, _P]
+    lib.fnx_tree_layout.argtypes = [_P, _P, _P, _P, c_int64, c_int, c_int64, c_int, c_int, c_int, _P, _P, _P,
+                                    _P, c_int, _P]
+    lib.fnx_tree_attention_workspace_floats.argtypes = [_I64P]
+    lib.fnx_tree_attention.argtypes = [
+        _P, c_int64, c_int64, _P, _I64P, _P, _I64P, c_int64, c_int, _P, c_int64, c_int, _P, _P, _P, _P,
+        c_int64, c_int64, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_float, c_int, _P, _P,
+        c_int, _P]
+    lib.fnx_sample.argtypes = [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P]
     lib.fnx_last_error.restype = c_char_p
     lib.fnx_version.restype = c_char_p
     for name in EXPORTED:

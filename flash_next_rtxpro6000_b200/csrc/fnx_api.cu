@@ -13,6 +13,7 @@
 #include "../../include/fnx_gemv.h"
 #include "fnx_common.cuh"
 #include "fnx_kernels.h"
+#include "tree_attn.cuh"
 
 #include <mutex>
 #include <set>
@@ -1253,5 +1254,229 @@ int fnx_argmax_decode(const unsigned long long* keys, int64_t* out, int M,
 const char* fnx_last_error(void) { return g_err.c_str(); }
 
 const char* fnx_version(void) { return "fnx-b200 0.1.0 (sm_100a)"; }
+
+namespace {
+
+bool type16(int dtype) { return dtype == FNX_T_BF16 || dtype == FNX_T_F16; }
+
+// The page / place / head strides of a cache; false if null.
+bool cache_strides(const int64_t* st, int64_t (&out)[3]) {
+  if (!st) return false;
+  for (int i = 0; i < 3; ++i) out[i] = st[i];
+  return true;
+}
+
+bool vec8(int64_t stride) { return stride % 8 == 0; }
+
+}  // namespace
+
+int fnx_rotary_append(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                      int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out,
+                      int64_t o_st, int64_t o_sh, const int64_t* pos, const int64_t* slots,
+                      const float* table, int64_t table_ld, int64_t positions, void* k_cache,
+                      const int64_t* k_strides, void* v_cache, const int64_t* v_strides,
+                      int64_t num_pages, int page_size, int tokens, int q_heads, int kv_heads,
+                      int dim, int rotated, int interleaved, int dtype, int* error_flag, int pdl,
+                      fnx_stream_t stream) {
+  g_err.clear();
+  if (!type16(dtype)) return fail(FNX_EUNSUPPORTED, "rotary: bf16 or fp16 only (dtype %d)", dtype);
+  if (tokens < 0 || q_heads < 0 || kv_heads < 0 || q_heads + kv_heads < 1 || dim < 1)
+    return fail(FNX_EINVAL, "rotary: bad shape tokens=%d q_heads=%d kv_heads=%d dim=%d", tokens,
+                q_heads, kv_heads, dim);
+  if (rotated < 0 || rotated > dim || rotated % 2)
+    return fail(FNX_EINVAL, "rotary: rotated=%d must be even and at most dim=%d", rotated, dim);
+  if (page_size < 1 || num_pages < 0 || positions < 1 || table_ld < rotated)
+    return fail(FNX_EINVAL, "rotary: bad table or cache shape");
+  if (tokens == 0) return FNX_OK;
+  if ((q_heads && (!q || !q_out)) || (kv_heads && (!k || !v || !k_cache || !v_cache)) || !pos ||
+      !slots || !table)
+    return fail(FNX_EINVAL, "rotary: null pointer");
+  fnx::RotaryArgs a = {};
+  if (!cache_strides(k_strides, a.kc_st) || !cache_strides(v_strides, a.vc_st))
+    return fail(FNX_EINVAL, "rotary: null cache strides");
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_out = q_out;
+  a.q_st = q_st;
+  a.q_sh = q_sh;
+  a.k_st = k_st;
+  a.k_sh = k_sh;
+  a.v_st = v_st;
+  a.v_sh = v_sh;
+  a.o_st = o_st;
+  a.o_sh = o_sh;
+  a.positions = pos;
+  a.slots = slots;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.P = positions;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.n_slots = num_pages * page_size;
+  a.page_size = page_size;
+  a.T = tokens;
+  a.Hq = q_heads;
+  a.Hk = kv_heads;
+  a.D = dim;
+  a.R = rotated;
+  a.interleaved = interleaved ? 1 : 0;
+  a.f16 = dtype == FNX_T_F16;
+  a.err = error_flag;
+  a.pdl = pdl;
+  bool ok = dim % 16 == 0 && dim <= 4096 && rotated % 16 == 0 && aligned(table, 16) &&
+            table_ld % 4 == 0 && aligned(q, 16) && aligned(k, 16) && aligned(v, 16) &&
+            aligned(q_out, 16) && aligned(k_cache, 16) && aligned(v_cache, 16);
+  for (int64_t st : {q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh}) ok = ok && vec8(st);
+  for (int i = 0; i < 3; ++i) ok = ok && vec8(a.kc_st[i]) && vec8(a.vc_st[i]);
+  a.vectors = ok;
+  if (fnx::launch_rotary(a, static_cast<cudaStream_t>(stream))) return cuda_fail("rotary launch");
+  return FNX_OK;
+}
+
+int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
+                    const int32_t* context_lens, const int32_t* page_table, int64_t table_ld,
+                    int table_width, int64_t num_pages, int page_size, int batch, int nodes,
+                    uint64_t* mask, int64_t* positions, int64_t* slots, int* error_flag, int pdl,
+                    fnx_stream_t stream) {
+  g_err.clear();
+  if (batch < 0 || nodes < 0 || (slots && (page_size < 1 || table_width < 0 || num_pages < 0)))
+    return fail(FNX_EINVAL, "tree layout: bad shape batch=%d nodes=%d page_size=%d", batch, nodes,
+                page_size);
+  if (nodes == 0) return FNX_OK;
+  if (batch < 1 || !parents || !node_offsets || ((positions || slots) && !context_lens) ||
+      (slots && !page_table))
+    return fail(FNX_EINVAL, "tree layout: null pointer");
+  fnx::TreeArgs a = {};
+  a.parents = parents;
+  a.node_offsets = node_offsets;
+  a.context_lens = context_lens;
+  a.page_table = page_table;
+  a.table_ld = table_ld;
+  a.num_pages = num_pages;
+  a.table_width = table_width;
+  a.page_size = page_size;
+  a.B = batch;
+  a.N = nodes;
+  a.mask = reinterpret_cast<unsigned long long*>(mask);
+  a.positions = positions;
+  a.slots = slots;
+  a.err = error_flag;
+  a.pdl = pdl;
+  if (fnx::launch_tree_layout(a, static_cast<cudaStream_t>(stream)))
+    return cuda_fail("tree layout launch");
+  return FNX_OK;
+}
+
+int fnx_tree_attention_workspace_floats(int64_t* floats) {
+  g_err.clear();
+  if (!floats) return fail(FNX_EINVAL, "tree attention: null pointer");
+  *floats = fnx::attn_workspace_floats();
+  return FNX_OK;
+}
+
+int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,
+                       const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
+                       int64_t num_pages, int page_size, const int32_t* page_table,
+                       int64_t table_ld, int table_width, const int32_t* context_lens,
+                       const int32_t* node_offsets, const uint64_t* tree_mask, void* out,
+                       int64_t o_sn, int64_t o_sh, float* lse, int batch, int nodes, int q_heads,
+                       int kv_heads, int dim, int max_nodes, int64_t max_context, float scale,
+                       int dtype, float* partials, int* error_flag, int pdl,
+                       fnx_stream_t stream) {
+  g_err.clear();
+  if (!type16(dtype))
+    return fail(FNX_EUNSUPPORTED, "tree attention: bf16 or fp16 only (dtype %d)", dtype);
+  if (dim != 64 && dim != 128 && dim != 256)
+    return fail(FNX_EUNSUPPORTED, "tree attention: head size %d (64, 128 or 256)", dim);
+  if (batch < 0 || nodes < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads)
+    return fail(FNX_EINVAL, "tree attention: bad shape batch=%d nodes=%d q_heads=%d kv_heads=%d",
+                batch, nodes, q_heads, kv_heads);
+  if (max_nodes < 1 || max_context < 0 || page_size < 1 || table_width < 0 || num_pages < 0)
+    return fail(FNX_EINVAL, "tree attention: bad max_nodes, max_context or cache shape");
+  if (max_nodes > 64)
+    return fail(FNX_EUNSUPPORTED, "tree attention: %d nodes a request (at most 64)", max_nodes);
+  if (max_context > (1ll << 31) - 1 - 256)
+    return fail(FNX_EUNSUPPORTED, "tree attention: contexts of 2^31 tokens");
+  if (q_heads > 65535) return fail(FNX_EUNSUPPORTED, "tree attention: %d heads", q_heads);
+  if (nodes == 0) return FNX_OK;
+  if (batch < 1 || !q || !k_cache || !v_cache || !page_table || !context_lens || !node_offsets ||
+      !out || !partials)
+    return fail(FNX_EINVAL, "tree attention: null pointer");
+  fnx::AttnArgs a = {};
+  if (!cache_strides(k_strides, a.kc_st) || !cache_strides(v_strides, a.vc_st))
+    return fail(FNX_EINVAL, "tree attention: null cache strides");
+  bool ok = aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16) &&
+            aligned(partials, 16) && vec8(q_sn) && vec8(q_sh) && vec8(o_sn) && vec8(o_sh);
+  for (int i = 0; i < 3; ++i) ok = ok && vec8(a.kc_st[i]) && vec8(a.vc_st[i]);
+  if (!ok)
+    return fail(FNX_EINVAL, "tree attention: rows and strides must be 16-byte aligned");
+  a.q = q;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.out = out;
+  a.lse = lse;
+  a.q_sn = q_sn;
+  a.q_sh = q_sh;
+  a.o_sn = o_sn;
+  a.o_sh = o_sh;
+  a.tree_mask = reinterpret_cast<const unsigned long long*>(tree_mask);
+  a.table_ld = table_ld;
+  a.num_pages = num_pages;
+  a.table_width = table_width;
+  a.page_size = page_size;
+  a.N = nodes;
+  a.Hq = q_heads;
+  a.Hk = kv_heads;
+  a.group = q_heads / kv_heads;
+  a.D = dim;
+  a.max_nodes = max_nodes;
+  a.max_context = (int)max_context;
+  a.scale = scale;
+  a.f16 = dtype == FNX_T_F16;
+  a.partials = partials;
+  a.err = error_flag;
+  a.pdl = pdl;
+  for (int b0 = 0; b0 < batch; b0 += fnx::kAttnMaxBatch) {  // requests of one launch
+    a.B = std::min(batch - b0, fnx::kAttnMaxBatch);
+    a.page_table = page_table + (int64_t)b0 * table_ld;
+    a.context_lens = context_lens + b0;
+    a.node_offsets = node_offsets + b0;
+    if (fnx::launch_tree_attn(a, static_cast<cudaStream_t>(stream)))
+      return cuda_fail("tree attention launch");
+  }
+  return FNX_OK;
+}
+
+int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const float* uniforms,
+               const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, int64_t* tokens, float* probs, int pdl, fnx_stream_t stream) {
+  g_err.clear();
+  if (dtype != FNX_T_BF16 && dtype != FNX_T_F16 && dtype != FNX_T_F32)
+    return fail(FNX_EUNSUPPORTED, "sampling: bf16, fp16 or fp32 logits (dtype %d)", dtype);
+  if (M < 0 || V < 1 || ldl < V)
+    return fail(FNX_EINVAL, "sampling: bad logits shape M=%d V=%d ldl=%lld", M, V, (long long)ldl);
+  if (V > 1 << 22) return fail(FNX_EUNSUPPORTED, "sampling: V=%d (at most 2^22)", V);
+  if (M > 1 << 24) return fail(FNX_EUNSUPPORTED, "sampling: M=%d (at most 2^24)", M);
+  if (M == 0) return FNX_OK;
+  if (!logits || !uniforms || !tokens || !probs)
+    return fail(FNX_EINVAL, "sampling: null pointer");
+  fnx::SampleArgs a = {};
+  a.logits = logits;
+  a.ldl = ldl;
+  a.type = dtype;
+  a.M = M;
+  a.V = V;
+  a.uniforms = uniforms;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.tokens = tokens;
+  a.probs = probs;
+  a.pdl = pdl;
+  if (fnx::launch_sample(a, static_cast<cudaStream_t>(stream))) return cuda_fail("sampling launch");
+  return FNX_OK;
+}
 
 }  // extern "C"

@@ -594,4 +594,69 @@ int launch_with_pdl(const void* func, const Args& args, int grid, int threads, s
   return cudaLaunchKernelExC(&cfg, func, params) == cudaSuccess ? 0 : 2;
 }
 
+// Verify-step operators (rotary.cu, tree_attn.cu, sample.cu).
+struct RotaryArgs {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;  // strides over tokens and heads
+  const int64_t *positions, *slots;
+  const float* table;
+  int64_t table_ld, P;
+  void *k_cache, *v_cache;
+  int64_t kc_st[3], vc_st[3];  // strides over pages, places and heads
+  int64_t n_slots;
+  int page_size, T, Hq, Hk, D, R;
+  int interleaved, f16;
+  int vectors;  // sizes and alignment allow 16-byte accesses
+  int* err;
+  int pdl;
+};
+int launch_rotary(const RotaryArgs& a, cudaStream_t stream);
+
+struct TreeArgs {
+  const int *parents, *node_offsets, *context_lens, *page_table;
+  int64_t table_ld, num_pages;
+  int table_width, page_size, B, N;
+  unsigned long long* mask;
+  int64_t *positions, *slots;
+  int* err;
+  int pdl;
+};
+int launch_tree_layout(const TreeArgs& a, cudaStream_t stream);
+
+struct AttnArgs {
+  const void *q, *k_cache, *v_cache;
+  void* out;
+  float* lse;
+  int64_t q_sn, q_sh, o_sn, o_sh;
+  int64_t kc_st[3], vc_st[3];  // strides over pages, places and heads
+  const int *page_table, *context_lens, *node_offsets;
+  const unsigned long long* tree_mask;
+  int64_t table_ld, num_pages;
+  int table_width, page_size;
+  int B, N, Hq, Hk, group, D, max_nodes, max_context;
+  float scale;
+  int f16;
+  float* partials;
+  int* err;
+  int pdl;
+};
+int64_t attn_workspace_floats();
+int launch_tree_attn(const AttnArgs& a, cudaStream_t stream);
+
+enum LogitsType : int { LOGITS_BF16 = 0, LOGITS_F16 = 1, LOGITS_F32 = 2 };
+struct SampleArgs {
+  const void* logits;
+  int64_t ldl;
+  int type, M, V;
+  const float *uniforms, *temperature, *top_p, *min_p;
+  const int* top_k;
+  int64_t* tokens;
+  float* probs;
+  int per;      // logits per CTA of a row's cluster
+  int in_smem;  // they fit into its shared memory
+  int pdl;
+};
+int launch_sample(SampleArgs a, cudaStream_t stream);
+
 }  // namespace fnx

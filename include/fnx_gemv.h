@@ -90,6 +90,11 @@ typedef void* fnx_stream_t;
 #define FNX_DEVERR_ROUTES 9        /* a routing table the kernel cannot hold        */
 #define FNX_DEVERR_WAIT_EXPERT 10  /* a down projection waited for its expert's act */
 #define FNX_DEVERR_RING 11         /* a launch whose ring stages the waits cannot order */
+#define FNX_DEVERR_POSITION 12     /* a position outside the rotary table             */
+#define FNX_DEVERR_SLOT 13         /* a cache slot outside the cache (and not -1)     */
+#define FNX_DEVERR_LENGTHS 14      /* lengths that contradict each other or the bounds */
+#define FNX_DEVERR_PAGE 15         /* a page number outside the cache                 */
+#define FNX_DEVERR_TREE 16         /* a parent that is not an earlier node            */
 
 /* Split-K and argmax scratch of the dense GEMVs.  Counters and keys must be zero when
  * first used; every launch leaves them zero again (self-resetting, graph-replay safe).
@@ -436,6 +441,97 @@ int fnx_w8a16_gemv_static_ws(const void* x, int64_t ldx, const void* w, int64_t 
  * the work on `stream` has finished (this call synchronises the stream); clear != 0 sets
  * it back to zero.  *code receives an FNX_DEVERR_* value, or 0. */
 int fnx_static_ws_error(int clear, fnx_stream_t stream, int* code);
+
+/* Activation types of the verify-step operators below. */
+#define FNX_T_BF16 0
+#define FNX_T_F16 1
+#define FNX_T_F32 2 /* logits only */
+
+/*
+ * Rotary positions on queries and keys, with keys and values stored in a paged cache.
+ * The first `rotated` of `dim` elements of every query and key head are rotated in pairs:
+ * (i, i + rotated / 2), or (2i, 2i + 1) when interleaved; the others and the values pass
+ * through.  Products in fp32, rounded once.
+ *  q [tokens, q_heads, dim], k, v [tokens, kv_heads, dim] with strides (elements) over
+ *  tokens and heads; q_out likewise (it may be q itself).  table: fp32 rows of `positions`
+ *  positions (row stride table_ld), rotated / 2 cosines then rotated / 2 sines.
+ *  pos int64 [tokens]; slots int64 [tokens]: token t's place in the cache (page * page_size
+ *  + place in the page), -1 = not stored.  k_cache / v_cache [num_pages, page_size,
+ *  kv_heads, dim] with *_strides = element strides of pages, places and heads.
+ * Two tokens with the same slot race.  A position outside the table takes the nearest row and
+ * records FNX_DEVERR_POSITION; a slot outside the cache is not stored and records
+ * FNX_DEVERR_SLOT (error_flag may be NULL).
+ */
+int fnx_rotary_append(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                      int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out,
+                      int64_t o_st, int64_t o_sh, const int64_t* pos, const int64_t* slots,
+                      const float* table, int64_t table_ld, int64_t positions, void* k_cache,
+                      const int64_t* k_strides, void* v_cache, const int64_t* v_strides,
+                      int64_t num_pages, int page_size, int tokens, int q_heads, int kv_heads,
+                      int dim, int rotated, int interleaved, int dtype, int* error_flag, int pdl,
+                      fnx_stream_t stream);
+
+/*
+ * What a verify step over drafted trees needs, from the trees: for every node the bit mask of
+ * the nodes of its request that it sees (itself and its ancestors), its position (context
+ * length + depth) and the cache slot of its key and value (context length + index, through
+ * the page table).  parents int32 [nodes]: the parent's index within the request, below the
+ * node's own, or -1.  node_offsets int32 [batch + 1], context_lens int32 [batch], page_table
+ * int32 [batch, table_width] (row stride table_ld).  mask (uint64 bits), positions and slots
+ * int64 [nodes]; each may be NULL (page_table too, when slots is).  At most 64 nodes a
+ * request.  A parent that is not an earlier node records FNX_DEVERR_TREE and counts as -1;
+ * lengths beyond the table record FNX_DEVERR_LENGTHS, pages outside [0, num_pages)
+ * FNX_DEVERR_PAGE, with slot -1.
+ */
+int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
+                    const int32_t* context_lens, const int32_t* page_table, int64_t table_ld,
+                    int table_width, int64_t num_pages, int page_size, int batch, int nodes,
+                    uint64_t* mask, int64_t* positions, int64_t* slots, int* error_flag, int pdl,
+                    fnx_stream_t stream);
+
+/*
+ * Attention of drafted trees over a paged cache.  Node i of request b (nodes node_offsets[b]
+ * .. node_offsets[b + 1] - 1, at most max_nodes <= 64) attends the context_lens[b] keys of its
+ * context and, at places context_lens[b] + j of the cache, the drafted tokens j whose bit is
+ * set in tree_mask[i] (NULL: a chain, j <= i).  Query head h reads kv head h / (q_heads /
+ * kv_heads).  out = softmax(scale q k) v in the type of q, lse (may be NULL, fp32 [nodes,
+ * q_heads] contiguous) the natural logarithm of the sum; a row that sees nothing gives 0 and
+ * -inf.  What a row does not see does not reach it, NaN and infinities included, and page
+ * table entries past a request's last page are not read.
+ *  q, out [nodes, q_heads, dim] with strides (elements) over nodes and heads; caches as in
+ *  fnx_rotary_append, the type of q (FNX_T_BF16 or FNX_T_F16); dim 64, 128 or 256; rows and
+ *  strides 16-byte aligned.  max_context: a bound on context_lens.  partials: scratch of
+ *  fnx_tree_attention_workspace_floats fp32, not shared by calls that may overlap.
+ * Lengths outside the bounds record FNX_DEVERR_LENGTHS and leave the request's rows unwritten;
+ * page numbers outside [0, num_pages) record FNX_DEVERR_PAGE and their keys count as zeros.
+ */
+int fnx_tree_attention_workspace_floats(int64_t* floats);
+int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,
+                       const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
+                       int64_t num_pages, int page_size, const int32_t* page_table,
+                       int64_t table_ld, int table_width, const int32_t* context_lens,
+                       const int32_t* node_offsets, const uint64_t* tree_mask, void* out,
+                       int64_t o_sn, int64_t o_sh, float* lse, int batch, int nodes, int q_heads,
+                       int kv_heads, int dim, int max_nodes, int64_t max_context, float scale,
+                       int dtype, float* partials, int* error_flag, int pdl,
+                       fnx_stream_t stream);
+
+/*
+ * Sampling: tokens[m] drawn from row m of logits (fp32, bf16 or fp16, row stride ldl) by
+ * uniforms[m] in [0, 1), and its probability among the tokens kept.  In the order of falling
+ * logits (lower token first on ties) top-k keeps top_k tokens, top-p the shortest prefix whose
+ * probability reaches top_p of those, min-p the tokens with at least min_p of the largest
+ * probability; the token is the one at which the running probability passes uniforms[m] of
+ * what is kept.  Weights are whole numbers (2^40 exp((x - max) / temperature), truncated),
+ * so results do not depend on the split of the work.
+ * temperature <= 0 (or NaN): the first token.  top_k < 1, top_p >= 1 or NaN, min_p <= 0 or
+ * NaN: off; a NULL array: off (temperature 1).  top_p <= 0: the first token; min_p counts as
+ * at most 1; uniforms outside [0, 1) draw the first or the last token kept.  NaN logits
+ * count as -inf; a row without a larger one gives token -1 and probability 0.
+ */
+int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const float* uniforms,
+               const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, int64_t* tokens, float* probs, int pdl, fnx_stream_t stream);
 
 /* Description of the last error of the calling thread ("" if none). */
 const char* fnx_last_error(void);
