@@ -10,7 +10,7 @@ import ctypes
 import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_void_p
 
-from .build import LIB_PATH
+from .build import LIB_PATH, OPS_PATH
 
 FNX_OK, FNX_EINVAL, FNX_ECUDA, FNX_EUNSUPPORTED = 0, 1, 2, 3
 W_INT8, W_FP8_E4M3, W_BF16, W_NVFP4 = 0, 1, 2, 3
@@ -138,8 +138,9 @@ class FnxMoeWorkspaceSizes(ctypes.Structure):
     ]
 
 
-_lock = threading.Lock()
+_lock = threading.RLock()
 _lib = None
+_ops = None
 
 _P = c_void_p
 _I64P = POINTER(c_int64)
@@ -244,6 +245,37 @@ def lib():
             _declare(handle)
             _lib = handle
     return _lib
+
+
+def ops():
+    """The native binding of the verify-step operators (built with the library)."""
+    global _ops
+    if _ops is not None:
+        return _ops
+    with _lock:
+        if _ops is None:
+            lib()
+            if not OPS_PATH.exists():
+                try:
+                    from .build import build_binding
+
+                    build_binding()
+                except Exception as e:  # pragma: no cover - depends on the toolchain
+                    raise ImportError(
+                        f"{OPS_PATH.name} is missing and could not be built ({e}); run "
+                        "`python -m flash_next_rtxpro6000_b200.build`"
+                    ) from e
+            import importlib.machinery
+            import importlib.util
+
+            import torch  # noqa: F401  its libraries have to be loaded first
+
+            loader = importlib.machinery.ExtensionFileLoader("_fnx_ops", str(OPS_PATH))
+            spec = importlib.util.spec_from_loader("_fnx_ops", loader)
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+            _ops = module
+    return _ops
 
 
 def last_error() -> str:

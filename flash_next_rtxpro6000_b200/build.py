@@ -1,10 +1,12 @@
-"""Build the sm_100a shared library ``_fnx.so`` in-tree with nvcc.
+"""Build the sm_100a shared library ``_fnx.so`` in-tree with nvcc, and the native Python
+binding of the verify-step operators ``_fnx_ops.so`` (csrc/binding.cpp) with g++ and torch's headers.
 
     python -m flash_next_rtxpro6000_b200.build [--force]
 
 Each ``csrc/*.cu`` file is compiled to an object in parallel, then linked into one
 shared library with the CUDA runtime linked statically (the library then depends only on
-the driver, not on a particular libcudart).
+the driver, not on a particular libcudart).  The binding links that library (found beside it)
+and torch.
 """
 
 from __future__ import annotations
@@ -21,12 +23,14 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB_PATH = PKG / "_fnx.so"
+OPS_PATH = PKG / "_fnx_ops.so"
 OBJ_DIR = PKG / "_build"
 
 SOURCES = ["fnx_api.cu", "dense_gemv.cu", "dense_gemv_slice.cu", "dense_gemv_norm.cu", "dense_tc.cu",
            "moe_gemv.cu",
            "moe_fused.cu", "moe_lean.cu", "nvfp4_codec.cu", "router.cu", "topk1.cu",
            "rotary.cu", "tree_attn.cu", "sample.cu"]
+BINDING = "binding.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
          "-I" + str(INCLUDE)]
@@ -40,14 +44,14 @@ def nvcc() -> str:
 
 
 def _inputs():
-    return [CSRC / s for s in SOURCES] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + \
+    return [CSRC / s for s in SOURCES + [BINDING]] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + \
         sorted(INCLUDE.glob("*.h"))
 
 
 def up_to_date() -> bool:
-    if not LIB_PATH.exists():
+    if not LIB_PATH.exists() or not OPS_PATH.exists():
         return False
-    t = LIB_PATH.stat().st_mtime
+    t = min(LIB_PATH.stat().st_mtime, OPS_PATH.stat().st_mtime)
     return all(p.stat().st_mtime <= t for p in _inputs())
 
 
@@ -77,7 +81,30 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
+    build_binding()
     return LIB_PATH
+
+
+def build_binding() -> Path:
+    """Compile csrc/binding.cpp against the interpreter's torch, linked to ``_fnx.so``."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = OPS_PATH.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", str(CSRC / BINDING),
+           "-o", str(tmp), f"-L{PKG}", "-l:_fnx.so", f"-L{root}/lib", "-lc10", "-lc10_cuda", "-ltorch",
+           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, OPS_PATH)
+    return OPS_PATH
 
 
 def main():

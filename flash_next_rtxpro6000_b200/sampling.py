@@ -13,11 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import check, ptr
-from .rotary import _index
-from .w8a16_gemv import PDL, _stream
-
-_LOGITS = {torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16, torch.float32: _lib.T_F32}
+from .w8a16_gemv import PDL
 
 
 def sample_tokens(
@@ -39,24 +35,5 @@ def sample_tokens(
     Temperature 0 draws the first token; top_k < 1, top_p >= 1 and min_p <= 0 keep everything.  NaN
     logits count as -inf; a row of nothing else gives token -1 and probability 0.  Weights are whole
     numbers, so results are the same bit for bit from call to call."""
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError(f"logits must be row-contiguous [rows, vocab], got {tuple(logits.shape)}")
-    if logits.dtype not in _LOGITS:
-        raise NotImplementedError(f"sample_tokens: fp32, bf16 or fp16 logits, got {logits.dtype}")
-    if not logits.is_cuda:
-        raise ValueError("sample_tokens needs CUDA tensors")
-    M, V = logits.shape
-    dev = logits.device
-    _index(uniforms, "uniforms", M, torch.float32, dev)
-    for t, name, dtype in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
-                           (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
-        if t is not None:
-            _index(t, name, M, dtype, dev)
-    tokens = torch.empty(M, dtype=torch.int64, device=dev)
-    probs = torch.empty(M, dtype=torch.float32, device=dev)
-    rc = _lib.lib().fnx_sample(
-        ptr(logits), max(logits.stride(0), V), _LOGITS[logits.dtype], M, V, ptr(uniforms), ptr(temperature),
-        ptr(top_k), ptr(top_p), ptr(min_p), ptr(tokens), ptr(probs), int(PDL if pdl is None else pdl),
-        _stream(logits))
-    check(rc, "sample_tokens")
-    return tokens, probs
+    return _lib.ops().sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p,
+                                    PDL if pdl is None else pdl)

@@ -14,6 +14,7 @@ greedy top-1 of the bf16-rounded logits (lowest row on ties) into the same launc
 
 from __future__ import annotations
 
+import ctypes
 import logging
 import os
 from dataclasses import dataclass
@@ -33,6 +34,7 @@ _N_SLOTS = 2
 _SLOT = 0
 _WS: dict = {}
 _ONES: dict = {}
+_ADDRESSES: dict = {}
 
 
 def _env_flag(name: str, default: str = "0") -> bool:
@@ -119,12 +121,32 @@ def _workspace(device) -> Workspace:
     return _workspace_slot(device, _SLOT)
 
 
+def _addresses(index: int, slot: int) -> Tuple[int, int]:
+    ws = _workspace_slot(torch.device("cuda", index), slot)
+    n = ctypes.c_int64()
+    _lib.check(_lib.lib().fnx_tree_attention_workspace_floats(ctypes.byref(n)), "scratch")
+    ws.attention = torch.empty(n.value, dtype=torch.float32, device=ws.device)
+    got = _ADDRESSES[(index, slot)] = (ptr(ws.error_flag), ptr(ws.attention))
+    return got
+
+
+def _scratch(t: torch.Tensor) -> Tuple[int, int]:
+    """(error flag, attention scratch) addresses of the current slot on t's device, for the native
+    binding of the verify-step operators; (0, 0) for a tensor on the host, which it refuses."""
+    got = _ADDRESSES.get((t.get_device(), _SLOT))
+    if got is None:
+        return _addresses(t.get_device(), _SLOT) if t.is_cuda else (0, 0)
+    return got
+
+
 def prealloc(device) -> None:
     """Materialise every slot's scratch before any CUDA graph is captured
     (w8a16_gemv.py:383-395)."""
+    d = _norm_device(device)
     for slot in range(_N_SLOTS):
         _workspace_slot(device, slot)
-    d = _norm_device(device)
+        if d.type == "cuda" and (d.index, slot) not in _ADDRESSES:
+            _addresses(d.index, slot)
     if d not in _ONES:
         _ONES[d] = torch.ones(1, dtype=torch.float32, device=d)
     _lib.lib()
