@@ -1456,7 +1456,7 @@ int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const f
     return fail(FNX_EUNSUPPORTED, "sampling: bf16, fp16 or fp32 logits (dtype %d)", dtype);
   if (M < 0 || V < 1 || ldl < V)
     return fail(FNX_EINVAL, "sampling: bad logits shape M=%d V=%d ldl=%lld", M, V, (long long)ldl);
-  if (V > 1 << 22) return fail(FNX_EUNSUPPORTED, "sampling: V=%d (at most 2^22)", V);
+  if (V > 1 << 21) return fail(FNX_EUNSUPPORTED, "sampling: V=%d (at most 2^21)", V);
   if (M > 1 << 24) return fail(FNX_EUNSUPPORTED, "sampling: M=%d (at most 2^24)", M);
   if (M == 0) return FNX_OK;
   if (!logits || !uniforms || !tokens || !probs)

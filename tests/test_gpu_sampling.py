@@ -250,3 +250,14 @@ def test_no_rows_and_refusals():
     for change, error in bad:
         with pytest.raises(error):
             fx.sample_tokens(**(dict(logits=x, uniforms=u) | change))
+
+
+@pytest.mark.parametrize("V", [1000, 50021])
+def test_many_rows(V):
+    """More rows than run at once."""
+    g = torch.Generator().manual_seed(14)
+    M = 150
+    x = torch.randn(M, V, generator=g) * 3
+    x[:, torch.randint(0, V, (40,), generator=g)] += torch.rand(40, generator=g) * 10
+    _check(x.to(dev()), *_params(M, g, dev()))
+    _check(x.half().to(dev()), *_params(M, g, dev()))
