@@ -29,7 +29,7 @@ OBJ_DIR = PKG / "_build"
 SOURCES = ["fnx_api.cu", "dense_gemv.cu", "dense_gemv_slice.cu", "dense_gemv_norm.cu", "dense_tc.cu",
            "moe_gemv.cu",
            "moe_fused.cu", "moe_lean.cu", "nvfp4_codec.cu", "router.cu", "topk1.cu",
-           "rotary.cu", "tree_attn.cu", "sample.cu"]
+           "rotary.cu", "tree_attn.cu", "tree_attn_tc.cu", "sample.cu"]
 BINDING = "binding.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",

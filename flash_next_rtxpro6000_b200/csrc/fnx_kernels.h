@@ -643,6 +643,8 @@ struct AttnArgs {
 };
 int64_t attn_workspace_floats();
 int launch_tree_attn(const AttnArgs& a, cudaStream_t stream);
+// The tensor-memory form; its grid and rows per item's slot are for the launch that joins the partials.
+int launch_tree_attn_tc(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows);
 
 enum LogitsType : int { LOGITS_BF16 = 0, LOGITS_F16 = 1, LOGITS_F32 = 2 };
 struct SampleArgs {

@@ -486,7 +486,8 @@ template <typename T, int D>
 int launch_d(const AttnArgs& a, cudaStream_t stream) {
   int grid = 0, rows = 0, rc;
   const int most = a.max_nodes * a.group;
-  if (most <= 16) rc = launch_form<T, D, 1, 4>(a, stream, grid, rows);
+  if (most > 32) rc = launch_tree_attn_tc(a, stream, grid, rows);
+  else if (most <= 16) rc = launch_form<T, D, 1, 4>(a, stream, grid, rows);
   else if (most <= 32) rc = launch_form<T, D, 2, 4>(a, stream, grid, rows);
   else rc = launch_form<T, D, 4, 2>(a, stream, grid, rows);
   if (rc) return rc;
@@ -514,7 +515,9 @@ int launch_t(const AttnArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-int64_t attn_workspace_floats() { return 2ll * num_sms() * attn_slot_floats(64, 256); }
+int64_t attn_workspace_floats() {
+  // the widest slots: 256 rows of 128, 128 rows of 256
+  return 2ll * num_sms() * attn_slot_floats(256, 128); }
 
 int launch_tree_attn(const AttnArgs& a, cudaStream_t stream) {
   return a.f16 ? launch_t<__half>(a, stream) : launch_t<__nv_bfloat16>(a, stream);

@@ -16,7 +16,7 @@
 namespace fnx {
 
 constexpr int kKeyTile = 64;
-constexpr int kAttnMaxBatch = 512;  // requests of one launch
+constexpr int kAttnMaxBatch = 128;  // requests of one launch
 
 struct AttnReq {
   int ctx, nodes, n0;  // context length, drafted nodes, first row in q

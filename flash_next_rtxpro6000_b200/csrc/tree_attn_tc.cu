@@ -1,0 +1,606 @@
+// Tree attention on the 5th-generation tensor cores (tcgen05), for the requests whose nodes and query
+// heads fill a good part of a 128-row operand.  The operator, the split of the work and the partial
+// results are those of tree_attn.cu; here the two products run asynchronously with their operands and
+// sums in shared and tensor memory, so loading, products and softmax of different key tiles overlap:
+//
+//   S = Q K^T   A = Q (128 rows x D, shared memory), B = a tile of 64 keys (shared memory)
+//   O += P V    A = P (128 x 64, tensor memory, written over S), B = the tile's values as they lie
+//               in the cache (N contiguous), D = O (128 x D fp32, tensor memory)
+//
+// RT row tiles of 128 share every key tile that is loaded (RT = 2: up to 256 rows, D <= 128).
+// Keys and values travel through one ring of 64-row chunks, in 64-element blocks of 128-byte rows with
+// the 128-byte swizzle: the same layout serves K-major keys and N-major values.
+//
+// Roles: 4 RT softmax warps (a thread has a row: its scores come from tensor memory in one piece, so
+// the row's maximum and sum need no shuffles), 4 loading warps (cp.async, any page size), 1 warp that
+// issues the products.  O is rescaled only when a row's maximum has risen by more than 2^8: until then
+// weights may be larger than one, which costs nothing in floating point.
+// Every wait is bounded and records an error code; roles then fall through to the end.
+#include "tree_attn.cuh"
+
+namespace fnx {
+
+namespace {
+
+constexpr int kTile = kKeyTile;
+constexpr int kBlockBytes = kTile * 128;  // 64 rows of a 64-element block
+constexpr float kRise = 8.0f;
+
+template <int D, int RT>
+struct TcAttn {
+  static constexpr int kBlocks = D / 64;
+  static constexpr int kChunk = kBlocks * kBlockBytes;  // keys or values of a tile
+  static constexpr int kQTile = kBlocks * 128 * 128;    // a row tile of queries
+  static constexpr int kChunks = D == 256 ? 5 : D == 128 ? (RT == 2 ? 9 : 11) : 16;
+  static constexpr int kLag = D == 256 ? 3 : D == 128 ? 6 : 10;  // chunks in flight behind the last one
+  static_assert(kLag <= kChunks - 2, "a chunk's product may need the next chunk");
+  static constexpr int kThreads = (4 * RT + 5) * 32;
+  static constexpr int kCols = RT * D + RT * 2 * kTile <= 256 ? 256 : 512;
+  static_assert(RT * D + RT * 2 * kTile <= 512, "tensor memory");
+  struct Smem {
+    uint8_t q[RT][kQTile];
+    uint8_t ring[kChunks][kChunk];
+    long long before[kAttnMaxBatch + 1];
+    unsigned long long full[kChunks], empty[kChunks];
+    unsigned long long sfull[RT][2], pfull[RT][2], odone[RT], qfull[RT];
+    unsigned long long drain;
+    unsigned long long joined[2];  // softmax warps of one row tile, of all
+    unsigned long long odd;  // drafted tokens of the segment whose values are not all finite
+    uint32_t tmem;
+  };
+};
+
+__device__ __forceinline__ uint64_t* bar(unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); }
+
+// Shared-memory descriptors with the 128-byte swizzle (layout type 2 at bits 61-63, version 1 at bits
+// 46-47), addresses and distances in 16-byte units.  K-major: 8-row groups SBO apart.  MN-major: 8
+// k-rows of 128 bytes each are a group, groups SBO apart, 64-element blocks LBO apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Instruction descriptor of kind::f16 with fp32 sums: operand types (0 fp16, 1 bf16) at bits 7 and 10,
+// B N-major at bit 16, N / 8 at bit 17, M / 16 at bit 24.
+__host__ __device__ constexpr uint32_t attn_idesc(int type, int n_major, int N) {
+  return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)n_major << 16) |
+         ((uint32_t)(N >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void commit_to(unsigned long long& b) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(&b)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ bool all_wait(unsigned long long& b, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar(b), parity));
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 p = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T> struct TcType;
+template <> struct TcType<__nv_bfloat16> { static constexpr int kCode = 1; static constexpr uint32_t kExp = 0x7F80u; };
+template <> struct TcType<__half> { static constexpr int kCode = 0; static constexpr uint32_t kExp = 0x7C00u; };
+template <typename T>
+__device__ __forceinline__ bool odd_pair(uint32_t w) {
+  constexpr uint32_t e = TcType<T>::kExp;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// The CTA's segments, one after the other: the same for every role.
+struct Segments {
+  const AttnArgs& a;
+  const long long* before;
+  long long w, end;
+  int rows, b;
+  AttnReq rq;
+  int head, row0, live, t0, t1;
+  bool first, last;  // whether the segment has the item's first and last tile
+
+  __device__ __forceinline__ Segments(const AttnArgs& args, const long long* bf, int rows_, long long total, long long G)
+      : a(args), before(bf), rows(rows_) {
+    w = attn_first(blockIdx.x, total, G);
+    end = attn_first(blockIdx.x + 1, total, G);
+    b = attn_find(before, a.B, w);
+  }
+  __device__ __forceinline__ bool next() {
+    if (w >= end) return false;
+    while (before[b + 1] <= w) ++b;
+    rq = attn_request(a, b, false);
+    const AttnShape sh = attn_shape(a, rq, rows);
+    const int item = (int)((w - before[b]) / sh.key_tiles);
+    head = item / sh.row_tiles;
+    row0 = (item % sh.row_tiles) * rows;
+    live = min(rows, rq.nodes * a.group - row0);
+    const long long i0 = before[b] + (long long)item * sh.key_tiles, i1 = i0 + sh.key_tiles;
+    const long long w1 = end < i1 ? end : i1;
+    t0 = (int)(w - i0);
+    t1 = (int)(w1 - i0);
+    first = w == i0;
+    last = w1 == i1;
+    w = w1;
+    return true;
+  }
+};
+
+}  // namespace
+
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
+  using Cfg = TcAttn<D, RT>;
+  constexpr int NC = Cfg::kChunks, kBlocks = Cfg::kBlocks, kRows = 128 * RT;
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  typename Cfg::Smem& s = *reinterpret_cast<typename Cfg::Smem*>(base);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  attn_prefix(a, kRows, s.before, reinterpret_cast<long long*>(s.q), blockIdx.x == 0);
+  const long long total = s.before[a.B];
+  const long long G = total < (long long)gridDim.x ? total : (long long)gridDim.x;
+  if (blockIdx.x >= G) {
+    pdl_trigger();
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NC; ++i) mbar_init(bar(s.full[i]), 4), mbar_init(bar(s.empty[i]), 1);
+    for (int r = 0; r < RT; ++r) {
+      for (int i = 0; i < 2; ++i) mbar_init(bar(s.sfull[r][i]), 1), mbar_init(bar(s.pfull[r][i]), 4);
+      mbar_init(bar(s.odone[r]), 1);
+      mbar_init(bar(s.qfull[r]), 4);
+    }
+    mbar_init(bar(s.drain), 1);
+    mbar_init(bar(s.joined[0]), 4);
+    mbar_init(bar(s.joined[1]), 4 * RT);
+    s.odd = 0ull;
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 4 * RT + 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)),
+                 "r"(Cfg::kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tm = s.tmem;
+  Segments sg(a, s.before, kRows, total, G);
+
+  if (warp >= 4 * RT && warp < 4 * RT + 4) {
+    // ------------------------------------------------------------------ loading warps
+    constexpr int kLanesRow = D / 8 < 32 ? D / 8 : 32;  // lanes of a row: 16 bytes each
+    constexpr int kRowsPer = 32 / kLanesRow;            // rows of one instruction
+    const int pw = warp - 4 * RT;                       // rows 16 pw .. + 15 of every chunk
+    const int col = lane % kLanesRow;                   // 16-byte unit of the row
+    const T* kc = reinterpret_cast<const T*>(a.k_cache);
+    const T* vc = reinterpret_cast<const T*>(a.v_cache);
+    int i = 0;
+    bool ok = true;
+    auto landed = [&](int chunk) {  // the thread's copies of the chunk are done
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(s.full[chunk % NC]));
+    };
+    while (ok && sg.next()) {
+      const int len = sg.rq.ctx + sg.rq.nodes;
+      int64_t ko, vo, kn, vn;
+      attn_place(a, sg.b, sg.t0 * kTile + pw * 16 + (lane & 15), len, sg.head, kn, vn);
+      for (int t = sg.t0; ok && t < sg.t1; ++t) {
+        ko = kn, vo = vn;
+        if (t + 1 < sg.t1) attn_place(a, sg.b, (t + 1) * kTile + pw * 16 + (lane & 15), len, sg.head, kn, vn);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!all_wait(s.empty[i % NC], ((i / NC) & 1) ^ 1)) {
+            if (lane == 0) record_error(a.err, ERR_WAIT_EMPTY);
+            ok = false;
+            break;
+          }
+          const uint32_t to = smem_u32(s.ring[i % NC]) + (col >> 3) * kBlockBytes;
+          const T* from = (kv ? vc : kc) + col * 8;
+          const int64_t place = kv ? vo : ko;
+#pragma unroll
+          for (int j = 0; j < 16 / kRowsPer; ++j) {
+            const int rr = j * kRowsPer + lane / kLanesRow;  // row within the warp's 16
+            const int64_t at = __shfl_sync(0xffffffffu, place, rr);
+            const int r = pw * 16 + rr;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             to + r * 128 + (((col & 7) ^ (r & 7)) << 4)),
+                         "l"(from + (at < 0 ? 0 : at)), "r"(at < 0 ? 0 : 16)
+                         : "memory");
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          ++i;
+          if (i > Cfg::kLag) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kLag) : "memory");
+            landed(i - 1 - Cfg::kLag);
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    for (int j = i > Cfg::kLag ? i - Cfg::kLag : 0; j < i; ++j) landed(j);
+  } else if (warp == 4 * RT + 4) {
+    // ------------------------------------------------------------------ products
+    constexpr uint32_t kIdS = attn_idesc(TcType<T>::kCode, 0, kTile), kIdO = attn_idesc(TcType<T>::kCode, 1, D);
+    int i = 0, n[RT], segs[RT];  // chunk of the next keys; tiles and segments of each row tile
+#pragma unroll
+    for (int r = 0; r < RT; ++r) n[r] = segs[r] = 0;
+    int code = 0;
+    auto scores = [&](int r, int chunk) {
+      const uint32_t d = tm + RT * D + (r * 2 + (n[r] & 1)) * kTile;
+      const uint32_t q = smem_u32(s.q[r]), k = smem_u32(s.ring[chunk % NC]);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x)
+        mma_ss(d, desc_sw128(q + (x >> 2) * (128 * 128) + (x & 3) * 32, 16, 1024),
+               desc_sw128(k + (x >> 2) * kBlockBytes + (x & 3) * 32, 16, 1024), kIdS, x > 0);
+      commit_to(s.sfull[r][n[r] & 1]);
+    };
+    auto values = [&](int r, int m, int chunk, bool add) {  // tile m of row tile r
+      const uint32_t p = tm + RT * D + (r * 2 + (m & 1)) * kTile;
+      const uint32_t v = smem_u32(s.ring[chunk % NC]);
+#pragma unroll
+      for (int x = 0; x < kTile / 16; ++x)
+        mma_ts(tm + r * D, p + 8 * x, desc_sw128(v + x * 2048, kBlockBytes, 1024), kIdO, add || x > 0);
+      commit_to(s.odone[r]);
+    };
+    while (code == 0 && sg.next()) {
+      const int rts = RT == 1 ? 1 : (sg.live + 127) / 128;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        if (r >= rts) break;
+        if (!all_wait(s.qfull[r], segs[r] & 1)) code = ERR_WAIT_X;
+        ++segs[r];
+      }
+      for (int t = sg.t0; code == 0 && t <= sg.t1; ++t) {
+        if (t < sg.t1) {
+          if (!all_wait(s.full[i % NC], (i / NC) & 1)) { code = ERR_WAIT_FULL; break; }
+          fence_after();
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            if (r >= rts) break;
+            // the buffer's previous tile (its weights) has been used; a segment's first tile comes after the
+            // softmax warps have seen all products of the segment before
+            if (t > sg.t0 && n[r] >= 2 && !all_wait(s.odone[r], n[r] & 1)) { code = ERR_WAIT_RFREE; break; }
+            fence_after();
+            scores(r, i);
+          }
+          commit_to(s.empty[i % NC]);
+        }
+        if (t > sg.t0 && code == 0) {
+          const int vchunk = i - 1;
+          if (!all_wait(s.full[vchunk % NC], (vchunk / NC) & 1)) { code = ERR_WAIT_FULL; break; }
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            if (r >= rts) break;
+            const int m = n[r] - 1;
+            if (!all_wait(s.pfull[r][m & 1], (m >> 1) & 1)) { code = ERR_WAIT_RED; break; }
+            fence_after();
+            values(r, m, vchunk, t - 1 > sg.t0);
+          }
+          commit_to(s.empty[vchunk % NC]);
+        }
+        if (t < sg.t1) {
+          i += 2;
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            if (r < rts) ++n[r];
+        }
+      }
+    }
+    if (code && lane == 0) record_error(a.err, code);
+    commit_to(s.drain);  // nothing runs any more when the tensor memory is freed
+    if (!all_wait(s.drain, 0) && lane == 0) record_error(a.err, ERR_DRAIN);
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const int rt = warp >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane;  // of the row tile, and its lane in tensor memory
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const float c2 = a.scale * 1.4426950408889634f;
+    int n = 0, tiles = 0;  // tiles of this row tile, and of the CTA
+    int joins[2] = {0, 0};
+    auto join = [&](int all) {  // a barrier of the live row tiles' warps, with a bounded wait
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(s.joined[all]));
+      return all_wait(s.joined[all], joins[all]++ & 1);
+    };
+    bool ok = true;
+    while (ok && sg.next()) {
+      const int first_tile = tiles;
+      tiles += sg.t1 - sg.t0;
+      if (rt * 128 >= sg.live) continue;
+      const int all_live = RT == 2 && sg.live > 128 ? 1 : 0, threads = all_live ? 256 : 128;
+      unsigned long long odd = 0ull;
+      const int r = rt * 128 + row;
+      const bool mine = r < sg.live;
+      const bool busy = rt * 128 + quad * 32 < sg.live;  // the warp has a live row
+      const int node = mine ? (sg.row0 + r) / a.group : 0;
+      const int hq = sg.head * a.group + (sg.row0 + r) % a.group;
+      const int64_t qn = sg.rq.n0 + node;
+      const unsigned long long mask = mine ? attn_mask(a, sg.rq, node) : 0ull;
+      {
+        const T* q = reinterpret_cast<const T*>(a.q) + qn * a.q_sn + (int64_t)hq * a.q_sh;
+        uint8_t* to = s.q[rt] + row * 128;
+#pragma unroll 8
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 x = mine ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(to + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = x;
+        }
+        if (tid == 0) s.odd = 0ull;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(s.qfull[rt]));
+      }
+      float ref = -INFINITY, sum = 0.f;
+      const int len = sg.rq.ctx + sg.rq.nodes;
+      for (int t = sg.t0; t < sg.t1; ++t, ++n) {
+        const int pos0 = t * kTile;
+        const bool tail = pos0 + kTile > sg.rq.ctx;
+        if (tail) {
+          // A drafted token hidden from a row has weight 0 there, but 0 times an infinite or NaN value is
+          // NaN: such tokens' values are cleared here and added at the end for the rows that see them.
+          const int chunk = 2 * (first_tile + t - sg.t0) + 1;
+          if (!all_wait(s.full[chunk % NC], (chunk / NC) & 1)) {
+            if (lane == 0) record_error(a.err, ERR_WAIT_FULL);
+            ok = false;
+            break;
+          }
+          ok = join(all_live);
+          uint8_t* v = s.ring[chunk % NC];
+          for (int u = rt * 128 + row; u < kTile * kBlocks * 8; u += threads) {
+            const int j = (u >> 3) % kTile;  // unit u: block, row, place
+            if (pos0 + j < sg.rq.ctx || pos0 + j >= len) continue;
+            const uint4 x = lds128(v + u * 16);
+            if (odd_pair<T>(x.x) || odd_pair<T>(x.y) || odd_pair<T>(x.z) || odd_pair<T>(x.w))
+              atomicOr(&s.odd, 1ull << (pos0 + j - sg.rq.ctx));
+          }
+          ok = ok && join(all_live);
+          odd = s.odd;
+          if (odd) {
+            for (int u = rt * 128 + row; u < kTile * kBlocks * 8; u += threads) {
+              const int d = pos0 + (u >> 3) % kTile - sg.rq.ctx;
+              if (d >= 0 && d < sg.rq.nodes && (odd >> d & 1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+          }
+          ok = ok && join(all_live);
+          if (!ok) {
+            if (lane == 0) record_error(a.err, ERR_WAIT_RED);
+            break;
+          }
+        }
+        if (!all_wait(s.sfull[rt][n & 1], (n >> 1) & 1)) {
+          if (lane == 0) record_error(a.err, ERR_WAIT_RED);
+          ok = false;
+          break;
+        }
+        fence_after();
+        const uint32_t sp = tm + lanes + RT * D + (rt * 2 + (n & 1)) * kTile;
+        if (busy) {
+          float x[kTile];
+          ld32(sp, reinterpret_cast<uint32_t*>(x));
+          ld32(sp + 32, reinterpret_cast<uint32_t*>(x) + 32);
+          wait_ld();
+          if (tail) {
+#pragma unroll
+            for (int j = 0; j < kTile; ++j) {
+              const int d = pos0 + j - sg.rq.ctx;
+              x[j] = d >= 0 && (d >= sg.rq.nodes || !(mask >> (d & 63) & 1)) ? -INFINITY : x[j] * c2;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kTile; ++j) x[j] *= c2;
+          }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < kTile; j += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m4[e] = fmaxf(m4[e], x[j + e]);
+          }
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          const bool rise = mx > ref + kRise || (ref == -INFINITY && mx > ref);
+          if (t == sg.t0) {
+            ref = mx;
+          } else if (__any_sync(0xffffffffu, rise)) {
+            if (!all_wait(s.odone[rt], (n - 1) & 1)) {
+              if (lane == 0) record_error(a.err, ERR_WAIT_RED);
+              ok = false;
+              break;
+            }
+            fence_after();
+            const float to = rise ? mx : ref;
+            const float f = to == ref ? 1.f : exp2_fast(ref - to);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              ld32(tm + lanes + rt * D + c, reinterpret_cast<uint32_t*>(o));
+              wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= f;
+              st32(tm + lanes + rt * D + c, reinterpret_cast<const uint32_t*>(o));
+            }
+            sum *= f;
+            ref = to;
+          }
+          const float zero = ref == -INFINITY ? 0.f : ref;
+          float s4[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t p[kTile / 2];
+#pragma unroll
+          for (int j = 0; j < kTile; j += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[j + e] = exp2_fast(x[j + e] - zero);
+              s4[e] += x[j + e];
+            }
+            p[j / 2] = pack2<T>(x[j], x[j + 1]);
+            p[j / 2 + 1] = pack2<T>(x[j + 2], x[j + 3]);
+          }
+          sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          st32(sp, p);
+          wait_st();
+          fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(s.pfull[rt][n & 1]));
+      }
+      if (!ok) break;
+      if (!all_wait(s.odone[rt], (n - 1) & 1)) {
+        if (lane == 0) record_error(a.err, ERR_WAIT_RED);
+        break;
+      }
+      fence_after();
+      if (busy) {
+        const uint32_t oa = tm + lanes + rt * D;
+        while (odd) {  // rare: values that are not finite, for the rows that see them
+          const int d = __ffsll((long long)odd) - 1;
+          odd &= odd - 1;
+          int64_t ko, vo;
+          attn_place(a, sg.b, sg.rq.ctx + d, len, sg.head, ko, vo);
+          float wgt = 0.f;
+          if (mine && (mask >> d & 1) && ko >= 0) {
+            const T* q = reinterpret_cast<const T*>(a.q) + qn * a.q_sn + (int64_t)hq * a.q_sh;
+            const T* k = reinterpret_cast<const T*>(a.k_cache) + ko;
+            float dot = 0.f;
+            for (int e = 0; e < D; ++e) dot += to_f32(q[e]) * to_f32(k[e]);
+            wgt = exp2_fast(dot * c2 - (ref == -INFINITY ? 0.f : ref));
+          }
+          const bool add = mine && (mask >> d & 1) && vo >= 0;
+          const T* v = reinterpret_cast<const T*>(a.v_cache) + (vo >= 0 ? vo : 0);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            __syncwarp();
+            ld32(oa + c, reinterpret_cast<uint32_t*>(o));
+            wait_ld();
+            if (add) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] += wgt * to_f32(v[c + e]);
+            }
+            __syncwarp();
+            st32(oa + c, reinterpret_cast<const uint32_t*>(o));
+          }
+          wait_st();
+        }
+        const bool all = sg.first && sg.last;
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        T* out = reinterpret_cast<T*>(a.out) + qn * a.o_sn + (int64_t)hq * a.o_sh;
+        float* slot = a.partials + (2ll * blockIdx.x + (sg.first ? 1 : 0)) * attn_slot_floats(kRows, D);
+#pragma unroll 2
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          __syncwarp();
+          ld32(oa + c, reinterpret_cast<uint32_t*>(o));
+          wait_ld();
+          if (mine && all) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 y;
+              y.x = pack2<T>(o[e] * inv, o[e + 1] * inv);
+              y.y = pack2<T>(o[e + 2] * inv, o[e + 3] * inv);
+              y.z = pack2<T>(o[e + 4] * inv, o[e + 5] * inv);
+              y.w = pack2<T>(o[e + 6] * inv, o[e + 7] * inv);
+              *reinterpret_cast<uint4*>(out + c + e) = y;
+            }
+          } else if (mine) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(slot + (int64_t)r * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (mine && all && a.lse)
+          a.lse[qn * a.Hq + hq] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+        if (mine && !all)
+          *reinterpret_cast<float2*>(slot + (int64_t)kRows * D + 2 * r) = make_float2(ref, sum);
+      }
+      __syncwarp();
+      fence_before();
+    }
+  }
+  pdl_trigger();
+  fence_before();
+  __syncthreads();
+  if (warp == 4 * RT + 4) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(Cfg::kCols) : "memory");
+  }
+}
+
+namespace {
+
+template <typename T, int D, int RT>
+int launch_tc(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
+  const void* k = (const void*)tree_attn_tc_kernel<T, D, RT>;
+  if (!prepare_kernel(k)) return 2;
+  grid = num_sms();
+  rows = 128 * RT;
+  return launch_with_pdl(k, a, grid, TcAttn<D, RT>::kThreads, sizeof(typename TcAttn<D, RT>::Smem) + 1024, a.pdl, stream);
+}
+
+template <typename T>
+int launch_tc_t(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
+  const bool wide = a.max_nodes * a.group > 128;
+  if (a.D == 64) return wide ? launch_tc<T, 64, 2>(a, stream, grid, rows) : launch_tc<T, 64, 1>(a, stream, grid, rows);
+  if (a.D == 128)
+    return wide ? launch_tc<T, 128, 2>(a, stream, grid, rows) : launch_tc<T, 128, 1>(a, stream, grid, rows);
+  return launch_tc<T, 256, 1>(a, stream, grid, rows);
+}
+
+}  // namespace
+
+int launch_tree_attn_tc(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
+  return a.f16 ? launch_tc_t<__half>(a, stream, grid, rows) : launch_tc_t<__nv_bfloat16>(a, stream, grid, rows);
+}
+
+}  // namespace fnx
