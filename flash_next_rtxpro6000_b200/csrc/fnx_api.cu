@@ -1399,6 +1399,8 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
   if (max_context > (1ll << 31) - 1 - 256)
     return fail(FNX_EUNSUPPORTED, "tree attention: contexts of 2^31 tokens");
   if (q_heads > 65535) return fail(FNX_EUNSUPPORTED, "tree attention: %d heads", q_heads);
+  if (!(scale > 0.f) || scale > 3.0e38f)
+    return fail(FNX_EINVAL, "tree attention: scale %g must be positive and finite", (double)scale);
   if (nodes == 0) return FNX_OK;
   if (batch < 1 || !q || !k_cache || !v_cache || !page_table || !context_lens || !node_offsets ||
       !out || !partials)

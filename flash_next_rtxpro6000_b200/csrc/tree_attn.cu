@@ -103,10 +103,8 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn_kernel(const __grid
   attn_prefix(a, kRows, s.before, s.scratch, blockIdx.x == 0);
   const long long total = s.before[a.B];
   const long long G = total < (long long)gridDim.x ? total : (long long)gridDim.x;
-  if (blockIdx.x >= G) {
-    pdl_trigger();
-    return;
-  }
+  pdl_trigger();  // the launch that joins the partials may get ready
+  if (blockIdx.x >= G) return;
   long long w = attn_first(blockIdx.x, total, G);
   const long long end = attn_first(blockIdx.x + 1, total, G);
   int b = attn_find(s.before, a.B, w);
@@ -395,23 +393,23 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn_kernel(const __grid
     }
     w = w1;
   }
-  pdl_trigger();
 }
 
-// Adds up the partial results of the items that several CTAs held: one block per (node, query head);
-// D / 4 threads take four elements each, and the thread groups take the item's slots in turn.
+// Adds up the partial results of the items that several CTAs held: one block per (node, query head).
+// First the slots' maxima and sums, which give each slot its factor; then the sums, D / 4 threads by
+// four elements each, thread groups by the item's slots in turn, with several loads in flight.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) tree_attn_combine_kernel(const __grid_constant__ AttnArgs a, int rows, int grid) {
-  constexpr int kWide = D / 4, kGroups = 128 / kWide;
+__global__ void __launch_bounds__(256) tree_attn_combine_kernel(const __grid_constant__ AttnArgs a, int rows, int grid) {
+  constexpr int kWide = D / 4, kGroups = 256 / kWide;
   __shared__ long long before[kAttnMaxBatch + 1];
-  __shared__ long long scratch[4];
+  __shared__ long long scratch[8];
   __shared__ float4 part[kGroups][kWide];
-  __shared__ float2 stat[kGroups];
-  const int tid = threadIdx.x, x = tid % kWide, y = tid / kWide;
-  pdl_wait();
+  __shared__ float factor[kAttnMaxGrid];
+  __shared__ float red[8], red2[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, x = tid % kWide, y = tid / kWide;
+  // the lengths were there before the launch whose partials these are: only those are waited for
   attn_prefix(a, rows, before, scratch, false);
   const long long total = before[a.B];
-  if (total == 0) return;
   const long long G = total < (long long)grid ? total : (long long)grid;
   const int n = blockIdx.x, hq = blockIdx.y;
   // the request that holds node n
@@ -422,45 +420,63 @@ __global__ void __launch_bounds__(128) tree_attn_combine_kernel(const __grid_con
     else hi = mid;
   }
   const AttnReq rq = attn_request(a, lo, false);
-  if (n < rq.n0 || n >= rq.n0 + rq.nodes) return;
-  const AttnShape sh = attn_shape(a, rq, rows);
-  const int head = hq / a.group, row = (n - rq.n0) * a.group + hq % a.group;
-  const int item = head * sh.row_tiles + row / rows, r = row % rows;
-  const long long item0 = before[lo] + (long long)item * sh.key_tiles, item1 = item0 + sh.key_tiles;
-  const int c0 = attn_cta_of(item0, total, G), c1 = attn_cta_of(item1 - 1, total, G);
+  const bool held = total > 0 && n >= rq.n0 && n < rq.n0 + rq.nodes;
+  int c0 = 0, c1 = 0, r = 0;
+  if (held) {
+    const AttnShape sh = attn_shape(a, rq, rows);
+    const int head = hq / a.group, row = (n - rq.n0) * a.group + hq % a.group;
+    const int item = head * sh.row_tiles + row / rows;
+    r = row % rows;
+    const long long item0 = before[lo] + (long long)item * sh.key_tiles, item1 = item0 + sh.key_tiles;
+    c0 = attn_cta_of(item0, total, G);
+    c1 = attn_cta_of(item1 - 1, total, G);
+  }
+  pdl_wait();
   if (c0 == c1) return;  // written by the one CTA that held it
   const int64_t size = attn_slot_floats(rows, D);
+  // slot of contributor i: the item's first CTA holds its beginning, the others hold it from their start
+  auto slot = [&](int i) { return a.partials + (2ll * (c0 + i) + (i == 0 ? 1 : 0)) * size; };
+  const int count = c1 - c0 + 1;  // at most the grid
+  float2 st = make_float2(-INFINITY, 0.f);
+  if (tid < count) st = __ldcg(reinterpret_cast<const float2*>(slot(tid) + (int64_t)rows * D + 2 * r));
+  float top = st.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  const float f = exp2_fast(st.x - ref);
+  if (tid < count) factor[tid] = f;
+  float sum = tid < count ? st.y * f : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red2[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += red2[w];
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float top = -INFINITY, sum = 0.f;
-  for (int c = c0 + y; c <= c1; c += kGroups) {
-    const float* slot = a.partials + (2ll * c + (c == c0 ? 1 : 0)) * size;
-    const float2 st = __ldcg(reinterpret_cast<const float2*>(slot + (int64_t)rows * D + 2 * r));
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(slot + (int64_t)r * D + 4 * x));
-    const float mx = fmaxf(top, st.x), ref = mx == -INFINITY ? 0.f : mx;
-    const float f0 = exp2_fast(top - ref), f1 = exp2_fast(st.x - ref);
-    acc.x = acc.x * f0 + v.x * f1;
-    acc.y = acc.y * f0 + v.y * f1;
-    acc.z = acc.z * f0 + v.z * f1;
-    acc.w = acc.w * f0 + v.w * f1;
-    sum = sum * f0 + st.y * f1;
-    top = mx;
+#pragma unroll 8
+  for (int i = y; i < count; i += kGroups) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (int64_t)r * D + 4 * x));
+    const float g = factor[i];
+    acc.x += v.x * g;
+    acc.y += v.y * g;
+    acc.z += v.z * g;
+    acc.w += v.w * g;
   }
   part[y][x] = acc;
-  if (x == 0) stat[y] = make_float2(top, sum);
   __syncthreads();
   if (y != 0) return;
 #pragma unroll
   for (int z = 1; z < kGroups; ++z) {
-    const float2 st = stat[z];
     const float4 v = part[z][x];
-    const float mx = fmaxf(top, st.x), ref = mx == -INFINITY ? 0.f : mx;
-    const float f0 = exp2_fast(top - ref), f1 = exp2_fast(st.x - ref);
-    acc.x = acc.x * f0 + v.x * f1;
-    acc.y = acc.y * f0 + v.y * f1;
-    acc.z = acc.z * f0 + v.z * f1;
-    acc.w = acc.w * f0 + v.w * f1;
-    sum = sum * f0 + st.y * f1;
-    top = mx;
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   T* to = reinterpret_cast<T*>(a.out) + (int64_t)n * a.o_sn + (int64_t)hq * a.o_sh + 4 * x;
@@ -491,10 +507,11 @@ int launch_d(const AttnArgs& a, cudaStream_t stream) {
   else if (most <= 32) rc = launch_form<T, D, 2, 4>(a, stream, grid, rows);
   else rc = launch_form<T, D, 4, 2>(a, stream, grid, rows);
   if (rc) return rc;
+  if (grid > kAttnMaxGrid) return 2;
   if (a.max_context + a.max_nodes <= kKeyTile) return 0;  // one key tile: no item is split
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.N, a.Hq);
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

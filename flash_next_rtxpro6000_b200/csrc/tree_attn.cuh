@@ -17,6 +17,7 @@ namespace fnx {
 
 constexpr int kKeyTile = 64;
 constexpr int kAttnMaxBatch = 128;  // requests of one launch
+constexpr int kAttnMaxGrid = 256;   // CTAs of one launch (one per SM)
 
 struct AttnReq {
   int ctx, nodes, n0;  // context length, drafted nodes, first row in q

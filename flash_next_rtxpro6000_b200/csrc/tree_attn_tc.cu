@@ -7,15 +7,22 @@
 //   O += P V    A = P (128 x 64, tensor memory, written over S), B = the tile's values as they lie
 //               in the cache (N contiguous), D = O (128 x D fp32, tensor memory)
 //
-// RT row tiles of 128 share every key tile that is loaded (RT = 2: up to 256 rows, D <= 128).
-// Keys and values travel through one ring of 64-row chunks, in 64-element blocks of 128-byte rows with
-// the 128-byte swizzle: the same layout serves K-major keys and N-major values.
+// Two groups of softmax warps work side by side: on two row tiles of 128 (RT = 2: up to 256 rows that
+// share every key tile that is loaded), or on every other key tile of one (KS = 2), each group with its
+// own maximum, sum and O, joined at the end.  At D = 256 tensor memory has room for one O only.
+// Keys and values travel through rings of 64-row chunks, in 64-element blocks of 128-byte rows with the
+// 128-byte swizzle: the same layout serves K-major keys and N-major values.
 //
-// Roles: 4 RT softmax warps (a thread has a row: its scores come from tensor memory in one piece, so
-// the row's maximum and sum need no shuffles), 4 loading warps (cp.async, any page size), 1 warp that
-// issues the products.  O is rescaled only when a row's maximum has risen by more than 2^8: until then
-// weights may be larger than one, which costs nothing in floating point.
+// Roles: 4 softmax warps a group (a thread has a row: its scores come from tensor memory in one piece, so
+// the row's maximum and sum need no shuffles), 4 warps that load keys and 4 that load values (cp.async, any page size), one
+// warp that issues the first product and one the second.  O is rescaled only when a row's maximum has risen by more than 2^8: until then weights may
+// be larger than one, which costs nothing in floating point.
 // Every wait is bounded and records an error code; roles then fall through to the end.
+//
+// Measured before the second group and the separate loaders (24 requests, D = 128): a key tile took
+// 2,060 cycles, of which the softmax warps were busy for 1,560 and the loaders for 1,580.
+#include <type_traits>
+
 #include "tree_attn.cuh"
 
 namespace fnx {
@@ -26,26 +33,31 @@ constexpr int kTile = kKeyTile;
 constexpr int kBlockBytes = kTile * 128;  // 64 rows of a 64-element block
 constexpr float kRise = 8.0f;
 
-template <int D, int RT>
+template <int D, int RT, int KS>
 struct TcAttn {
+  static constexpr int kGroups = RT * KS;               // of softmax warps
   static constexpr int kBlocks = D / 64;
   static constexpr int kChunk = kBlocks * kBlockBytes;  // keys or values of a tile
   static constexpr int kQTile = kBlocks * 128 * 128;    // a row tile of queries
-  static constexpr int kChunks = D == 256 ? 5 : D == 128 ? (RT == 2 ? 9 : 11) : 16;
-  static constexpr int kLag = D == 256 ? 3 : D == 128 ? 6 : 10;  // chunks in flight behind the last one
-  static_assert(kLag <= kChunks - 2, "a chunk's product may need the next chunk");
-  static constexpr int kThreads = (4 * RT + 5) * 32;
-  static constexpr int kCols = RT * D + RT * 2 * kTile <= 256 ? 256 : 512;
-  static_assert(RT * D + RT * 2 * kTile <= 512, "tensor memory");
+  static constexpr int kK = D == 256 ? 2 : D == 128 ? (RT == 2 ? 4 : 5) : 8;  // chunks of the rings
+  static constexpr int kV = D == 256 ? 3 : D == 128 ? (RT == 2 ? 5 : 6) : 8;
+  static constexpr int kLoad = 4 * kGroups, kIssue = kLoad + 8;  // first loading, first issuing warp
+  static constexpr int kThreads = (kIssue + 4) * 32;  // the issuing warps are the last two of four
+  static constexpr int kCols = kGroups * (D + 2 * kTile) <= 256 ? 256 : 512;
+  static_assert(kGroups * (D + 2 * kTile) <= 512, "tensor memory");
   struct Smem {
     uint8_t q[RT][kQTile];
-    uint8_t ring[kChunks][kChunk];
+    uint8_t k[kK][kChunk];
+    uint8_t v[kV][kChunk];
     long long before[kAttnMaxBatch + 1];
-    unsigned long long full[kChunks], empty[kChunks];
-    unsigned long long sfull[RT][2], pfull[RT][2], odone[RT], qfull[RT];
+    unsigned long long kfull[kK], kempty[kK], vfull[kV], vempty[kV];
+    unsigned long long sfull[kGroups][2], pfull[kGroups][2], odone[kGroups][2], qfull[RT];
+    unsigned long long joined[3];  // softmax warps of each group, of all
+    unsigned long long other;      // the second group is done with its key tiles
     unsigned long long drain;
-    unsigned long long joined[2];  // softmax warps of one row tile, of all
-    unsigned long long odd;  // drafted tokens of the segment whose values are not all finite
+    // drafted tokens whose values are not all finite, of this segment, the one before and the next
+    unsigned long long odd[3];
+    float2 stat[KS == 2 ? 128 : 1];  // the second group's maxima and sums
     uint32_t tmem;
   };
 };
@@ -178,10 +190,10 @@ struct Segments {
 
 }  // namespace
 
-template <typename T, int D, int RT>
-__global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
-  using Cfg = TcAttn<D, RT>;
-  constexpr int NC = Cfg::kChunks, kBlocks = Cfg::kBlocks, kRows = 128 * RT;
+template <typename T, int D, int RT, int KS>
+__global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
+  using Cfg = TcAttn<D, RT, KS>;
+  constexpr int NK = Cfg::kK, NV = Cfg::kV, kBlocks = Cfg::kBlocks, kRows = 128 * RT, kGroups = Cfg::kGroups;
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   typename Cfg::Smem& s = *reinterpret_cast<typename Cfg::Smem*>(base);
@@ -190,25 +202,23 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
   attn_prefix(a, kRows, s.before, reinterpret_cast<long long*>(s.q), blockIdx.x == 0);
   const long long total = s.before[a.B];
   const long long G = total < (long long)gridDim.x ? total : (long long)gridDim.x;
-  if (blockIdx.x >= G) {
-    pdl_trigger();
-    return;
-  }
+  pdl_trigger();  // the launch that joins the partials may get ready
+  if (blockIdx.x >= G) return;
   if (tid == 0) {
-    for (int i = 0; i < NC; ++i) mbar_init(bar(s.full[i]), 4), mbar_init(bar(s.empty[i]), 1);
-    for (int r = 0; r < RT; ++r) {
-      for (int i = 0; i < 2; ++i) mbar_init(bar(s.sfull[r][i]), 1), mbar_init(bar(s.pfull[r][i]), 4);
-      mbar_init(bar(s.odone[r]), 1);
-      mbar_init(bar(s.qfull[r]), 4);
-    }
-    mbar_init(bar(s.drain), 1);
-    mbar_init(bar(s.joined[0]), 4);
-    mbar_init(bar(s.joined[1]), 4 * RT);
-    s.odd = 0ull;
+    for (int i = 0; i < NK; ++i) mbar_init(bar(s.kfull[i]), 4), mbar_init(bar(s.kempty[i]), 1);
+    for (int i = 0; i < NV; ++i) mbar_init(bar(s.vfull[i]), 4), mbar_init(bar(s.vempty[i]), 1);
+    for (int w = 0; w < kGroups; ++w)
+      for (int i = 0; i < 2; ++i)
+        mbar_init(bar(s.sfull[w][i]), 1), mbar_init(bar(s.pfull[w][i]), 4), mbar_init(bar(s.odone[w][i]), 1);
+    for (int r = 0; r < RT; ++r) mbar_init(bar(s.qfull[r]), 4);
+    for (int i = 0; i < 3; ++i) mbar_init(bar(s.joined[i]), i < 2 ? 4 : 4 * kGroups);
+    mbar_init(bar(s.other), 4);
+    mbar_init(bar(s.drain), 2);
+    s.odd[0] = s.odd[1] = s.odd[2] = 0ull;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
-  if (warp == 4 * RT + 4) {
+  if (warp == Cfg::kIssue) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)),
                  "r"(Cfg::kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -218,39 +228,45 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
   fence_after();
   const uint32_t tm = s.tmem;
   Segments sg(a, s.before, kRows, total, G);
-
-  if (warp >= 4 * RT && warp < 4 * RT + 4) {
+  // With two groups of softmax warps the others' registers go to them: 256 * 144 + 384 * 56 are no more
+  // than the launch's 640 * 96.
+  if (warp >= Cfg::kLoad && warp < Cfg::kIssue) {
     // ------------------------------------------------------------------ loading warps
+    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     constexpr int kLanesRow = D / 8 < 32 ? D / 8 : 32;  // lanes of a row: 16 bytes each
     constexpr int kRowsPer = 32 / kLanesRow;            // rows of one instruction
-    const int pw = warp - 4 * RT;                       // rows 16 pw .. + 15 of every chunk
+    const int pw = warp & 3;                            // rows 16 pw .. + 15 of every chunk
     const int col = lane % kLanesRow;                   // 16-byte unit of the row
-    const T* kc = reinterpret_cast<const T*>(a.k_cache);
-    const T* vc = reinterpret_cast<const T*>(a.v_cache);
-    int i = 0;
-    bool ok = true;
-    auto landed = [&](int chunk) {  // the thread's copies of the chunk are done
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(s.full[chunk % NC]));
-    };
-    while (ok && sg.next()) {
-      const int len = sg.rq.ctx + sg.rq.nodes;
-      int64_t ko, vo, kn, vn;
-      attn_place(a, sg.b, sg.t0 * kTile + pw * 16 + (lane & 15), len, sg.head, kn, vn);
-      for (int t = sg.t0; ok && t < sg.t1; ++t) {
-        ko = kn, vo = vn;
-        if (t + 1 < sg.t1) attn_place(a, sg.b, (t + 1) * kTile + pw * 16 + (lane & 15), len, sg.head, kn, vn);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!all_wait(s.empty[i % NC], ((i / NC) & 1) ^ 1)) {
+    auto run = [&](auto stages, const T* from, uint8_t* ring, unsigned long long* full, unsigned long long* empty,
+                   bool values) {
+      // chunks in flight behind the last one: few enough that a chunk is not told of only when the one
+      // before it has been used up
+      constexpr int N = decltype(stages)::value, kLag = N / 2;
+      int i = 0;
+      bool ok = true;
+      auto landed = [&](int chunk) {  // the thread's copies of the chunk are done
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(full[chunk % N]));
+      };
+      while (ok && sg.next()) {
+        const int len = sg.rq.ctx + sg.rq.nodes;
+        int64_t place, ahead, unused;
+        auto find = [&](int t) {
+          const int pos = t * kTile + pw * 16 + (lane & 15);
+          if (values) attn_place(a, sg.b, pos, len, sg.head, unused, ahead);
+          else attn_place(a, sg.b, pos, len, sg.head, ahead, unused);
+        };
+        find(sg.t0);
+        for (int t = sg.t0; t < sg.t1; ++t) {
+          place = ahead;
+          if (t + 1 < sg.t1) find(t + 1);
+          if (!all_wait(empty[i % N], ((i / N) & 1) ^ 1)) {
             if (lane == 0) record_error(a.err, ERR_WAIT_EMPTY);
             ok = false;
             break;
           }
-          const uint32_t to = smem_u32(s.ring[i % NC]) + (col >> 3) * kBlockBytes;
-          const T* from = (kv ? vc : kc) + col * 8;
-          const int64_t place = kv ? vo : ko;
+          const uint32_t to = smem_u32(ring + (i % N) * Cfg::kChunk) + (col >> 3) * kBlockBytes;
 #pragma unroll
           for (int j = 0; j < 16 / kRowsPer; ++j) {
             const int rr = j * kRowsPer + lane / kLanesRow;  // row within the warp's 16
@@ -258,43 +274,47 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
             const int r = pw * 16 + rr;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                              to + r * 128 + (((col & 7) ^ (r & 7)) << 4)),
-                         "l"(from + (at < 0 ? 0 : at)), "r"(at < 0 ? 0 : 16)
+                         "l"(from + col * 8 + (at < 0 ? 0 : at)), "r"(at < 0 ? 0 : 16)
                          : "memory");
           }
           asm volatile("cp.async.commit_group;" ::: "memory");
           ++i;
-          if (i > Cfg::kLag) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kLag) : "memory");
-            landed(i - 1 - Cfg::kLag);
+          if (i > kLag) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+            landed(i - 1 - kLag);
           }
         }
       }
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    for (int j = i > Cfg::kLag ? i - Cfg::kLag : 0; j < i; ++j) landed(j);
-  } else if (warp == 4 * RT + 4) {
-    // ------------------------------------------------------------------ products
-    constexpr uint32_t kIdS = attn_idesc(TcType<T>::kCode, 0, kTile), kIdO = attn_idesc(TcType<T>::kCode, 1, D);
-    int i = 0, n[RT], segs[RT];  // chunk of the next keys; tiles and segments of each row tile
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      for (int j = i > kLag ? i - kLag : 0; j < i; ++j) landed(j);
+    };
+    if (warp < Cfg::kLoad + 4)
+      run(std::integral_constant<int, NK>{}, reinterpret_cast<const T*>(a.k_cache), s.k[0], s.kfull, s.kempty, false);
+    else
+      run(std::integral_constant<int, NV>{}, reinterpret_cast<const T*>(a.v_cache), s.v[0], s.vfull, s.vempty, true);
+  } else if (warp == Cfg::kIssue + 2) {
+    // ------------------------------------------------------------------ S = Q K^T
+    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    constexpr uint32_t kId = attn_idesc(TcType<T>::kCode, 0, kTile);
+    int i = 0;                  // tile of the CTA
+    int n[kGroups], segs[RT];  // tiles of each group, segments of each row tile
 #pragma unroll
-    for (int r = 0; r < RT; ++r) n[r] = segs[r] = 0;
+    for (int w = 0; w < kGroups; ++w) n[w] = 0;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) segs[r] = 0;
     int code = 0;
-    auto scores = [&](int r, int chunk) {
-      const uint32_t d = tm + RT * D + (r * 2 + (n[r] & 1)) * kTile;
-      const uint32_t q = smem_u32(s.q[r]), k = smem_u32(s.ring[chunk % NC]);
+    auto scores = [&](int w, int chunk) {
+      // the weights of the buffer's tile before have been used
+      if (!all_wait(s.odone[w][n[w] & 1], ((n[w] >> 1) & 1) ^ 1)) { code = ERR_WAIT_RFREE; return; }
+      fence_after();
+      const uint32_t q = smem_u32(s.q[KS == 2 ? 0 : w]), k = smem_u32(s.k[chunk]);
+      const uint32_t d = tm + kGroups * D + (w * 2 + (n[w] & 1)) * kTile;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x)
         mma_ss(d, desc_sw128(q + (x >> 2) * (128 * 128) + (x & 3) * 32, 16, 1024),
-               desc_sw128(k + (x >> 2) * kBlockBytes + (x & 3) * 32, 16, 1024), kIdS, x > 0);
-      commit_to(s.sfull[r][n[r] & 1]);
-    };
-    auto values = [&](int r, int m, int chunk, bool add) {  // tile m of row tile r
-      const uint32_t p = tm + RT * D + (r * 2 + (m & 1)) * kTile;
-      const uint32_t v = smem_u32(s.ring[chunk % NC]);
-#pragma unroll
-      for (int x = 0; x < kTile / 16; ++x)
-        mma_ts(tm + r * D, p + 8 * x, desc_sw128(v + x * 2048, kBlockBytes, 1024), kIdO, add || x > 0);
-      commit_to(s.odone[r]);
+               desc_sw128(k + (x >> 2) * kBlockBytes + (x & 3) * 32, 16, 1024), kId, x > 0);
+      commit_to(s.sfull[w][n[w] & 1]);
+      ++n[w];
     };
     while (code == 0 && sg.next()) {
       const int rts = RT == 1 ? 1 : (sg.live + 127) / 128;
@@ -304,65 +324,86 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
         if (!all_wait(s.qfull[r], segs[r] & 1)) code = ERR_WAIT_X;
         ++segs[r];
       }
-      for (int t = sg.t0; code == 0 && t <= sg.t1; ++t) {
-        if (t < sg.t1) {
-          if (!all_wait(s.full[i % NC], (i / NC) & 1)) { code = ERR_WAIT_FULL; break; }
-          fence_after();
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            if (r >= rts) break;
-            // the buffer's previous tile (its weights) has been used; a segment's first tile comes after the
-            // softmax warps have seen all products of the segment before
-            if (t > sg.t0 && n[r] >= 2 && !all_wait(s.odone[r], n[r] & 1)) { code = ERR_WAIT_RFREE; break; }
-            fence_after();
-            scores(r, i);
-          }
-          commit_to(s.empty[i % NC]);
-        }
-        if (t > sg.t0 && code == 0) {
-          const int vchunk = i - 1;
-          if (!all_wait(s.full[vchunk % NC], (vchunk / NC) & 1)) { code = ERR_WAIT_FULL; break; }
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            if (r >= rts) break;
-            const int m = n[r] - 1;
-            if (!all_wait(s.pfull[r][m & 1], (m >> 1) & 1)) { code = ERR_WAIT_RED; break; }
-            fence_after();
-            values(r, m, vchunk, t - 1 > sg.t0);
-          }
-          commit_to(s.empty[vchunk % NC]);
-        }
-        if (t < sg.t1) {
-          i += 2;
+      for (int t = sg.t0; code == 0 && t < sg.t1; ++t, ++i) {
+        const int c = i % NK;
+        if (!all_wait(s.kfull[c], (i / NK) & 1)) { code = ERR_WAIT_FULL; break; }
+        fence_after();
+        if (KS == 2) {
+          if ((t - sg.t0) & 1) scores(kGroups - 1, c);
+          else scores(0, c);
+        } else {
 #pragma unroll
           for (int r = 0; r < RT; ++r)
-            if (r < rts) ++n[r];
+            if (r < rts && code == 0) scores(r, c);
         }
+        commit_to(s.kempty[c]);
       }
     }
     if (code && lane == 0) record_error(a.err, code);
     commit_to(s.drain);  // nothing runs any more when the tensor memory is freed
     if (!all_wait(s.drain, 0) && lane == 0) record_error(a.err, ERR_DRAIN);
-  } else {
+  } else if (warp == Cfg::kIssue + 3) {
+    // ------------------------------------------------------------------ O += P V
+    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    constexpr uint32_t kId = attn_idesc(TcType<T>::kCode, 1, D);
+    int i = 0, n[kGroups];
+#pragma unroll
+    for (int w = 0; w < kGroups; ++w) n[w] = 0;
+    int code = 0;
+    auto values = [&](int w, int chunk, bool add) {
+      if (!all_wait(s.pfull[w][n[w] & 1], (n[w] >> 1) & 1)) { code = ERR_WAIT_RED; return; }
+      fence_after();
+      const uint32_t v = smem_u32(s.v[chunk]), p = tm + kGroups * D + (w * 2 + (n[w] & 1)) * kTile;
+#pragma unroll
+      for (int x = 0; x < kTile / 16; ++x)
+        mma_ts(tm + w * D, p + 8 * x, desc_sw128(v + x * 2048, kBlockBytes, 1024), kId, add || x > 0);
+      commit_to(s.odone[w][n[w] & 1]);
+      ++n[w];
+    };
+    while (code == 0 && sg.next()) {
+      const int rts = RT == 1 ? 1 : (sg.live + 127) / 128;
+      for (int t = sg.t0; code == 0 && t < sg.t1; ++t, ++i) {
+        const int c = i % NV, j = t - sg.t0;
+        if (!all_wait(s.vfull[c], (i / NV) & 1)) { code = ERR_WAIT_FULL; break; }
+        if (KS == 2) {
+          if (j & 1) values(kGroups - 1, c, j > 1);
+          else values(0, c, j > 1);
+        } else {
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            if (r < rts && code == 0) values(r, c, j > 0);
+        }
+        commit_to(s.vempty[c]);
+      }
+    }
+    if (code && lane == 0) record_error(a.err, code);
+    commit_to(s.drain);
+    if (!all_wait(s.drain, 0) && lane == 0) record_error(a.err, ERR_DRAIN);
+  } else if (warp < Cfg::kLoad) {
     // ------------------------------------------------------------------ softmax
-    const int rt = warp >> 2, quad = warp & 3;
+    if (kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    const int w = warp >> 2, quad = warp & 3;  // group
+    const int rt = KS == 2 ? 0 : w;
     const int row = quad * 32 + lane;  // of the row tile, and its lane in tensor memory
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const float c2 = a.scale * 1.4426950408889634f;
-    int n = 0, tiles = 0;  // tiles of this row tile, and of the CTA
-    int joins[2] = {0, 0};
-    auto join = [&](int all) {  // a barrier of the live row tiles' warps, with a bounded wait
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(s.joined[all]));
-      return all_wait(s.joined[all], joins[all]++ & 1);
-    };
+    // tiles of the group and of the CTA, segments, segments with a second group
+    int n = 0, tiles = 0, seg = 0, ends = 0;
     bool ok = true;
+    int joins[3] = {0, 0, 0};
+    auto join = [&](int who) {  // a barrier of one group's warps, or of all, with a bounded wait
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(s.joined[who]));
+      return all_wait(s.joined[who], joins[who]++ & 1);
+    };
+    auto o_is_done = [&]() { return all_wait(s.odone[w][(n - 1) & 1], ((n - 1) >> 1) & 1); };
     while (ok && sg.next()) {
       const int first_tile = tiles;
       tiles += sg.t1 - sg.t0;
+      unsigned long long* odds = &s.odd[seg % 3];
+      ++seg;
       if (rt * 128 >= sg.live) continue;
-      const int all_live = RT == 2 && sg.live > 128 ? 1 : 0, threads = all_live ? 256 : 128;
-      unsigned long long odd = 0ull;
+      const int who = RT == 2 && sg.live > 128 ? 2 : w, threads = who == 2 ? 256 : 128;
       const int r = rt * 128 + row;
       const bool mine = r < sg.live;
       const bool busy = rt * 128 + quad * 32 < sg.live;  // the warp has a live row
@@ -370,7 +411,7 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
       const int hq = sg.head * a.group + (sg.row0 + r) % a.group;
       const int64_t qn = sg.rq.n0 + node;
       const unsigned long long mask = mine ? attn_mask(a, sg.rq, node) : 0ull;
-      {
+      if (KS == 1 || w == 0) {
         const T* q = reinterpret_cast<const T*>(a.q) + qn * a.q_sn + (int64_t)hq * a.q_sh;
         uint8_t* to = s.q[rt] + row * 128;
 #pragma unroll 8
@@ -378,56 +419,52 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
           const uint4 x = mine ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
           *reinterpret_cast<uint4*>(to + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = x;
         }
-        if (tid == 0) s.odd = 0ull;
+        if (tid == 0) s.odd[seg % 3] = 0ull;  // the next segment's
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(s.qfull[rt]));
       }
       float ref = -INFINITY, sum = 0.f;
       const int len = sg.rq.ctx + sg.rq.nodes;
-      for (int t = sg.t0; t < sg.t1; ++t, ++n) {
+      const int begin = sg.t0 + (KS == 2 ? w : 0);
+      for (int t = begin; t < sg.t1; t += KS, ++n) {
         const int pos0 = t * kTile;
         const bool tail = pos0 + kTile > sg.rq.ctx;
-        if (tail) {
-          // A drafted token hidden from a row has weight 0 there, but 0 times an infinite or NaN value is
-          // NaN: such tokens' values are cleared here and added at the end for the rows that see them.
-          const int chunk = 2 * (first_tile + t - sg.t0) + 1;
-          if (!all_wait(s.full[chunk % NC], (chunk / NC) & 1)) {
-            if (lane == 0) record_error(a.err, ERR_WAIT_FULL);
-            ok = false;
-            break;
-          }
-          ok = join(all_live);
-          uint8_t* v = s.ring[chunk % NC];
-          for (int u = rt * 128 + row; u < kTile * kBlocks * 8; u += threads) {
-            const int j = (u >> 3) % kTile;  // unit u: block, row, place
-            if (pos0 + j < sg.rq.ctx || pos0 + j >= len) continue;
-            const uint4 x = lds128(v + u * 16);
-            if (odd_pair<T>(x.x) || odd_pair<T>(x.y) || odd_pair<T>(x.z) || odd_pair<T>(x.w))
-              atomicOr(&s.odd, 1ull << (pos0 + j - sg.rq.ctx));
-          }
-          ok = ok && join(all_live);
-          odd = s.odd;
-          if (odd) {
-            for (int u = rt * 128 + row; u < kTile * kBlocks * 8; u += threads) {
-              const int d = pos0 + (u >> 3) % kTile - sg.rq.ctx;
-              if (d >= 0 && d < sg.rq.nodes && (odd >> d & 1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-          }
-          ok = ok && join(all_live);
-          if (!ok) {
-            if (lane == 0) record_error(a.err, ERR_WAIT_RED);
-            break;
-          }
-        }
-        if (!all_wait(s.sfull[rt][n & 1], (n >> 1) & 1)) {
+        if (!all_wait(s.sfull[w][n & 1], (n >> 1) & 1)) {
           if (lane == 0) record_error(a.err, ERR_WAIT_RED);
           ok = false;
           break;
         }
         fence_after();
-        const uint32_t sp = tm + lanes + RT * D + (rt * 2 + (n & 1)) * kTile;
+        if (tail) {
+          // A drafted token hidden from a row has weight 0 there, but 0 times an infinite or NaN value is
+          // NaN: such tokens' values are cleared here and added at the end for the rows that see them.
+          const int chunk = first_tile + t - sg.t0;
+          ok = all_wait(s.vfull[chunk % NV], (chunk / NV) & 1) && join(who);
+          uint8_t* v = s.v[chunk % NV];
+          for (int u = (who == 2 ? rt * 128 : 0) + row; u < kTile * kBlocks * 8; u += threads) {
+            const int j = (u >> 3) % kTile;  // unit u: block, row, place
+            if (pos0 + j < sg.rq.ctx || pos0 + j >= len) continue;
+            const uint4 x = lds128(v + u * 16);
+            if (odd_pair<T>(x.x) || odd_pair<T>(x.y) || odd_pair<T>(x.z) || odd_pair<T>(x.w))
+              atomicOr(odds, 1ull << (pos0 + j - sg.rq.ctx));
+          }
+          ok = ok && join(who);
+          const unsigned long long odd = *reinterpret_cast<volatile unsigned long long*>(odds);
+          if (odd) {
+            for (int u = (who == 2 ? rt * 128 : 0) + row; u < kTile * kBlocks * 8; u += threads) {
+              const int d = pos0 + (u >> 3) % kTile - sg.rq.ctx;
+              if (d >= 0 && d < sg.rq.nodes && (odd >> d & 1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+          }
+          ok = ok && join(who);
+          if (!ok) {
+            if (lane == 0) record_error(a.err, ERR_WAIT_RED);
+            break;
+          }
+        }
+        const uint32_t sp = tm + lanes + kGroups * D + (w * 2 + (n & 1)) * kTile;
         if (busy) {
           float x[kTile];
           ld32(sp, reinterpret_cast<uint32_t*>(x));
@@ -437,24 +474,18 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
 #pragma unroll
             for (int j = 0; j < kTile; ++j) {
               const int d = pos0 + j - sg.rq.ctx;
-              x[j] = d >= 0 && (d >= sg.rq.nodes || !(mask >> (d & 63) & 1)) ? -INFINITY : x[j] * c2;
+              if (d >= 0 && (d >= sg.rq.nodes || !(mask >> (d & 63) & 1))) x[j] = -INFINITY;
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < kTile; ++j) x[j] *= c2;
           }
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < kTile; j += 4) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m4[e] = fmaxf(m4[e], x[j + e]);
-          }
-          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          for (int j = 0; j < kTile; ++j) m4[j & 3] = fmaxf(m4[j & 3], x[j]);
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c2;
           const bool rise = mx > ref + kRise || (ref == -INFINITY && mx > ref);
-          if (t == sg.t0) {
+          if (t == begin) {
             ref = mx;
           } else if (__any_sync(0xffffffffu, rise)) {
-            if (!all_wait(s.odone[rt], (n - 1) & 1)) {
+            if (!o_is_done()) {
               if (lane == 0) record_error(a.err, ERR_WAIT_RED);
               ok = false;
               break;
@@ -465,27 +496,25 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               float o[32];
-              ld32(tm + lanes + rt * D + c, reinterpret_cast<uint32_t*>(o));
+              ld32(tm + lanes + w * D + c, reinterpret_cast<uint32_t*>(o));
               wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] *= f;
-              st32(tm + lanes + rt * D + c, reinterpret_cast<const uint32_t*>(o));
+              st32(tm + lanes + w * D + c, reinterpret_cast<const uint32_t*>(o));
             }
             sum *= f;
             ref = to;
           }
-          const float zero = ref == -INFINITY ? 0.f : ref;
+          const float zero = ref == -INFINITY ? 0.f : -ref;
           float s4[4] = {0.f, 0.f, 0.f, 0.f};
           uint32_t p[kTile / 2];
 #pragma unroll
-          for (int j = 0; j < kTile; j += 4) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[j + e] = exp2_fast(x[j + e] - zero);
-              s4[e] += x[j + e];
-            }
+          for (int j = 0; j < kTile; j += 2) {
+            x[j] = exp2_fast(fmaf(x[j], c2, zero));
+            x[j + 1] = exp2_fast(fmaf(x[j + 1], c2, zero));
+            s4[j & 2] += x[j];
+            s4[(j & 2) + 1] += x[j + 1];
             p[j / 2] = pack2<T>(x[j], x[j + 1]);
-            p[j / 2 + 1] = pack2<T>(x[j + 2], x[j + 3]);
           }
           sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
           st32(sp, p);
@@ -493,30 +522,51 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
           fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(s.pfull[rt][n & 1]));
+        if (lane == 0) mbar_arrive(bar(s.pfull[w][n & 1]));
       }
       if (!ok) break;
-      if (!all_wait(s.odone[rt], (n - 1) & 1)) {
+      const bool two = KS == 2 && sg.t1 - sg.t0 > 1;  // the second group has a part of the sums
+      if (begin < sg.t1 && !o_is_done()) {
         if (lane == 0) record_error(a.err, ERR_WAIT_RED);
         break;
       }
       fence_after();
+      if (KS == 2 && w == 1) {
+        if (two) {
+          s.stat[row] = make_float2(ref, sum);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(s.other));
+        }
+        continue;
+      }
+      float ref2 = -INFINITY, sum2 = 0.f;
+      if (two) {
+        if (!all_wait(s.other, ends++ & 1)) {
+          if (lane == 0) record_error(a.err, ERR_WAIT_RED);
+          break;
+        }
+        fence_after();
+        ref2 = s.stat[row].x;
+        sum2 = s.stat[row].y;
+      }
       if (busy) {
-        const uint32_t oa = tm + lanes + rt * D;
+        const uint32_t oa = tm + lanes + w * D;
+        unsigned long long odd = sg.t1 * kTile > sg.rq.ctx ? *reinterpret_cast<volatile unsigned long long*>(odds) : 0ull;
+        const bool added = odd != 0ull;
         while (odd) {  // rare: values that are not finite, for the rows that see them
           const int d = __ffsll((long long)odd) - 1;
           odd &= odd - 1;
           int64_t ko, vo;
           attn_place(a, sg.b, sg.rq.ctx + d, len, sg.head, ko, vo);
+          const bool add = mine && (mask >> d & 1) && vo >= 0;
           float wgt = 0.f;
-          if (mine && (mask >> d & 1) && ko >= 0) {
+          if (add) {
             const T* q = reinterpret_cast<const T*>(a.q) + qn * a.q_sn + (int64_t)hq * a.q_sh;
             const T* k = reinterpret_cast<const T*>(a.k_cache) + ko;
             float dot = 0.f;
             for (int e = 0; e < D; ++e) dot += to_f32(q[e]) * to_f32(k[e]);
             wgt = exp2_fast(dot * c2 - (ref == -INFINITY ? 0.f : ref));
           }
-          const bool add = mine && (mask >> d & 1) && vo >= 0;
           const T* v = reinterpret_cast<const T*>(a.v_cache) + (vo >= 0 ? vo : 0);
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -533,24 +583,37 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
           }
           wait_st();
         }
+        const float top = fmaxf(ref, ref2), zero = top == -INFINITY ? 0.f : top;
+        const float f1 = exp2_fast((added && ref == -INFINITY ? 0.f : ref) - zero), f2 = exp2_fast(ref2 - zero);
+        sum = two ? sum * f1 + sum2 * f2 : sum;
         const bool all = sg.first && sg.last;
-        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        const float inv = all ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
+        const float g1 = two ? f1 * inv : inv, g2 = f2 * inv;
         T* out = reinterpret_cast<T*>(a.out) + qn * a.o_sn + (int64_t)hq * a.o_sh;
         float* slot = a.partials + (2ll * blockIdx.x + (sg.first ? 1 : 0)) * attn_slot_floats(kRows, D);
-#pragma unroll 2
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float o[32];
           __syncwarp();
           ld32(oa + c, reinterpret_cast<uint32_t*>(o));
           wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= g1;
+          if (KS == 2 && two) {
+            float o2[32];
+            ld32(oa + D + c, reinterpret_cast<uint32_t*>(o2));
+            wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] += o2[e] * g2;
+          }
           if (mine && all) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint4 y;
-              y.x = pack2<T>(o[e] * inv, o[e + 1] * inv);
-              y.y = pack2<T>(o[e + 2] * inv, o[e + 3] * inv);
-              y.z = pack2<T>(o[e + 4] * inv, o[e + 5] * inv);
-              y.w = pack2<T>(o[e + 6] * inv, o[e + 7] * inv);
+              y.x = pack2<T>(o[e], o[e + 1]);
+              y.y = pack2<T>(o[e + 2], o[e + 3]);
+              y.z = pack2<T>(o[e + 4], o[e + 5]);
+              y.w = pack2<T>(o[e + 6], o[e + 7]);
               *reinterpret_cast<uint4*>(out + c + e) = y;
             }
           } else if (mine) {
@@ -560,18 +623,19 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
           }
         }
         if (mine && all && a.lse)
-          a.lse[qn * a.Hq + hq] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+          a.lse[qn * a.Hq + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
         if (mine && !all)
-          *reinterpret_cast<float2*>(slot + (int64_t)kRows * D + 2 * r) = make_float2(ref, sum);
+          *reinterpret_cast<float2*>(slot + (int64_t)kRows * D + 2 * r) = make_float2(top, sum);
       }
       __syncwarp();
       fence_before();
     }
+  } else if (kGroups == 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   }
-  pdl_trigger();
   fence_before();
   __syncthreads();
-  if (warp == 4 * RT + 4) {
+  if (warp == Cfg::kIssue) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(Cfg::kCols) : "memory");
   }
@@ -579,22 +643,24 @@ __global__ void __launch_bounds__((4 * RT + 5) * 32, 1) tree_attn_tc_kernel(cons
 
 namespace {
 
-template <typename T, int D, int RT>
+template <typename T, int D, int RT, int KS>
 int launch_tc(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
-  const void* k = (const void*)tree_attn_tc_kernel<T, D, RT>;
+  using Cfg = TcAttn<D, RT, KS>;
+  const void* k = (const void*)tree_attn_tc_kernel<T, D, RT, KS>;
   if (!prepare_kernel(k)) return 2;
   grid = num_sms();
   rows = 128 * RT;
-  return launch_with_pdl(k, a, grid, TcAttn<D, RT>::kThreads, sizeof(typename TcAttn<D, RT>::Smem) + 1024, a.pdl, stream);
+  return launch_with_pdl(k, a, grid, Cfg::kThreads, sizeof(typename Cfg::Smem) + 1024, a.pdl, stream);
 }
 
 template <typename T>
 int launch_tc_t(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
   const bool wide = a.max_nodes * a.group > 128;
-  if (a.D == 64) return wide ? launch_tc<T, 64, 2>(a, stream, grid, rows) : launch_tc<T, 64, 1>(a, stream, grid, rows);
+  if (a.D == 64)
+    return wide ? launch_tc<T, 64, 2, 1>(a, stream, grid, rows) : launch_tc<T, 64, 1, 2>(a, stream, grid, rows);
   if (a.D == 128)
-    return wide ? launch_tc<T, 128, 2>(a, stream, grid, rows) : launch_tc<T, 128, 1>(a, stream, grid, rows);
-  return launch_tc<T, 256, 1>(a, stream, grid, rows);
+    return wide ? launch_tc<T, 128, 2, 1>(a, stream, grid, rows) : launch_tc<T, 128, 1, 2>(a, stream, grid, rows);
+  return launch_tc<T, 256, 1, 1>(a, stream, grid, rows);
 }
 
 }  // namespace

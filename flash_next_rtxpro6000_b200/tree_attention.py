@@ -62,7 +62,7 @@ def tree_attention(
 
     Node i attends the context and the drafted tokens whose bit is set in tree_mask[i].  Returns
     (out [nodes, q_heads, dim], lse fp32 [nodes, q_heads]), lse being the natural logarithm of the
-    sum of exp(scale q k) (scale: dim ** -0.5 unless given); a row that sees nothing gives 0 and -inf.
+    sum of exp(scale q k) (scale: dim ** -0.5 unless given, positive); a row that sees nothing gives 0 and -inf.
     ``max_context`` bounds context_lens (default: what the page table holds).  Lengths are read on the
     device, so a captured call follows them; lengths beyond the bounds and pages outside the cache are
     reported by ``check_device_errors``."""

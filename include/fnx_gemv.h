@@ -500,7 +500,7 @@ int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
  * table entries past a request's last page are not read.
  *  q, out [nodes, q_heads, dim] with strides (elements) over nodes and heads; caches as in
  *  fnx_rotary_append, the type of q (FNX_T_BF16 or FNX_T_F16); dim 64, 128 or 256; rows and
- *  strides 16-byte aligned.  max_context: a bound on context_lens.  partials: scratch of
+ *  strides 16-byte aligned; scale positive and finite.  max_context: a bound on context_lens.  partials: scratch of
  *  fnx_tree_attention_workspace_floats fp32, not shared by calls that may overlap.
  * Lengths outside the bounds record FNX_DEVERR_LENGTHS and leave the request's rows unwritten;
  * page numbers outside [0, num_pages) record FNX_DEVERR_PAGE and their keys count as zeros.

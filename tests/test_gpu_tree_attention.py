@@ -304,7 +304,8 @@ def test_no_nodes_and_refusals():
         (dict(page_table=c.table[:1]), ValueError), (dict(context_lens=c.ctx.long()), ValueError),
         (dict(node_offsets=c.offsets[:2]), ValueError), (dict(tree_mask=c.mask[:1]), ValueError),
         (dict(tree_mask=c.mask.int()), ValueError), (dict(max_nodes=65), NotImplementedError),
-        (dict(max_nodes=0), ValueError), (dict(max_context=-1), ValueError),
+        (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=float("nan")), ValueError),
+        (dict(scale=float("inf")), ValueError), (dict(max_nodes=0), ValueError), (dict(max_context=-1), ValueError),
         (dict(lse=torch.zeros(5, 4, dtype=torch.float64, device=dev())), ValueError),
         (dict(out=c.q.half()), ValueError), (dict(q=c.q.cpu()), ValueError),
         (dict(q=torch.zeros(5 * 4 * 64 + 1, dtype=torch.bfloat16, device=dev())[1:].view(5, 4, 64)), ValueError),
@@ -353,3 +354,32 @@ def test_tree_layout():
     for i, x in ((0, args[0].long()), (1, offsets[:2]), (2, args[2].long()), (3, table.to(d)[:2])):
         with pytest.raises(ValueError):
             fx.tree_layout(*(args[:i] + [x] + args[i + 1:]))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,T", [(4, 9), (4, 30), (8, 64)])
+def test_rising_scores(D, Hq, T):
+    """Keys whose scores keep rising along the context, so that every tile raises every row's maximum
+    far enough for the sums to be rescaled; and falling ones."""
+    for sign in (1, -1):
+        c = Case([2500, 300], [T, T], Hq, 1, D, 16, torch.bfloat16, seed=D + T)
+        c.q = c.q * 0.1
+        c.q[:, :, 0] = 1.0
+        pos = torch.arange(2500, device=dev())
+        for b, n in enumerate((2500, 300)):
+            slots = c.table[b].long()[pos[:n] // 16] * 16 + pos[:n] % 16
+            c.k.view(-1, 1, D)[slots, 0, 0] = (sign * pos[:n].float() * 0.05 * D**0.5).bfloat16()
+        c.check()
+
+
+@pytest.mark.parametrize("ctx", [1, 60, 61, 64, 65, 127, 128, 129])
+def test_trees_across_key_tiles(ctx):
+    """64 drafted tokens that lie in one key tile or in two, with values that are not finite in both."""
+    c = Case([ctx, ctx + 3], [64, 61], 8, 2, 128, 16, torch.float16, seed=ctx, garbage=True)
+    for j in (0, 3, 63):
+        slot = int(c.table[0][(ctx + j) // 16]) * 16 + (ctx + j) % 16
+        c.v.view(-1, 2, 128)[slot, :, j] = float("nan")
+    out, _ = c.check()
+    for j in (0, 3, 63):
+        sees = torch.tensor([bool(c.masks[i] >> j & 1) for i in range(64)], device=dev())
+        assert torch.equal(out[:64, 2, j].isnan(), sees)
