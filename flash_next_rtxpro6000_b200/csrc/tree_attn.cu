@@ -395,11 +395,12 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn_kernel(const __grid
   }
 }
 
-// Adds up the partial results of the items that several CTAs held: one block per (node, query head).
+// Adds up the partial results of the items that several CTAs held: one block per node and `heads` query
+// heads of a kv head (one, or all of a group where there are many nodes).
 // First the slots' maxima and sums, which give each slot its factor; then the sums, D / 4 threads by
 // four elements each, thread groups by the item's slots in turn, with several loads in flight.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) tree_attn_combine_kernel(const __grid_constant__ AttnArgs a, int rows, int grid) {
+__global__ void __launch_bounds__(256) tree_attn_combine_kernel(const __grid_constant__ AttnArgs a, int rows, int grid, int heads) {
   constexpr int kWide = D / 4, kGroups = 256 / kWide;
   __shared__ long long before[kAttnMaxBatch + 1];
   __shared__ long long scratch[8];
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(256) tree_attn_combine_kernel(const __grid_con
   attn_prefix(a, rows, before, scratch, false);
   const long long total = before[a.B];
   const long long G = total < (long long)grid ? total : (long long)grid;
-  const int n = blockIdx.x, hq = blockIdx.y;
+  const int n = blockIdx.x;
   // the request that holds node n
   int lo = 0, hi = a.B;
   while (hi - lo > 1) {
@@ -421,68 +422,67 @@ __global__ void __launch_bounds__(256) tree_attn_combine_kernel(const __grid_con
   }
   const AttnReq rq = attn_request(a, lo, false);
   const bool held = total > 0 && n >= rq.n0 && n < rq.n0 + rq.nodes;
-  int c0 = 0, c1 = 0, r = 0;
-  if (held) {
-    const AttnShape sh = attn_shape(a, rq, rows);
-    const int head = hq / a.group, row = (n - rq.n0) * a.group + hq % a.group;
-    const int item = head * sh.row_tiles + row / rows;
-    r = row % rows;
-    const long long item0 = before[lo] + (long long)item * sh.key_tiles, item1 = item0 + sh.key_tiles;
-    c0 = attn_cta_of(item0, total, G);
-    c1 = attn_cta_of(item1 - 1, total, G);
-  }
   pdl_wait();
-  if (c0 == c1) return;  // written by the one CTA that held it
+  if (!held) return;
+  const AttnShape sh = attn_shape(a, rq, rows);
   const int64_t size = attn_slot_floats(rows, D);
-  // slot of contributor i: the item's first CTA holds its beginning, the others hold it from their start
-  auto slot = [&](int i) { return a.partials + (2ll * (c0 + i) + (i == 0 ? 1 : 0)) * size; };
-  const int count = c1 - c0 + 1;  // at most the grid
-  float2 st = make_float2(-INFINITY, 0.f);
-  if (tid < count) st = __ldcg(reinterpret_cast<const float2*>(slot(tid) + (int64_t)rows * D + 2 * r));
-  float top = st.x;
+  for (int hq = blockIdx.y * heads; hq < (int)(blockIdx.y + 1) * heads; ++hq) {
+    const int head = hq / a.group, row = (n - rq.n0) * a.group + hq % a.group;
+    const int item = head * sh.row_tiles + row / rows, r = row % rows;
+    const long long item0 = before[lo] + (long long)item * sh.key_tiles, item1 = item0 + sh.key_tiles;
+    const int c0 = attn_cta_of(item0, total, G), c1 = attn_cta_of(item1 - 1, total, G);
+    if (c0 == c1) continue;  // written by the one CTA that held it
+    // slot of contributor i: the item's first CTA holds its beginning, the others from their start
+    auto slot = [&](int i) { return a.partials + (2ll * (c0 + i) + (i == 0 ? 1 : 0)) * size; };
+    const int count = c1 - c0 + 1;  // at most the grid
+    float2 st = make_float2(-INFINITY, 0.f);
+    if (tid < count) st = __ldcg(reinterpret_cast<const float2*>(slot(tid) + (int64_t)rows * D + 2 * r));
+    float top = st.x;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    __syncthreads();  // the head before is done with shared memory
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  const float f = exp2_fast(st.x - ref);
-  if (tid < count) factor[tid] = f;
-  float sum = tid < count ? st.y * f : 0.f;
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float f = exp2_fast(st.x - ref);
+    if (tid < count) factor[tid] = f;
+    float sum = tid < count ? st.y * f : 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) red2[warp] = sum;
-  __syncthreads();
-  sum = 0.f;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) red2[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) sum += red2[w];
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < 8; ++w) sum += red2[w];
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int i = y; i < count; i += kGroups) {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (int64_t)r * D + 4 * x));
-    const float g = factor[i];
-    acc.x += v.x * g;
-    acc.y += v.y * g;
-    acc.z += v.z * g;
-    acc.w += v.w * g;
-  }
-  part[y][x] = acc;
-  __syncthreads();
-  if (y != 0) return;
+    for (int i = y; i < count; i += kGroups) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (int64_t)r * D + 4 * x));
+      const float g = factor[i];
+      acc.x += v.x * g;
+      acc.y += v.y * g;
+      acc.z += v.z * g;
+      acc.w += v.w * g;
+    }
+    part[y][x] = acc;
+    __syncthreads();
+    if (y != 0) continue;
 #pragma unroll
-  for (int z = 1; z < kGroups; ++z) {
-    const float4 v = part[z][x];
-    acc.x += v.x;
-    acc.y += v.y;
-    acc.z += v.z;
-    acc.w += v.w;
+    for (int z = 1; z < kGroups; ++z) {
+      const float4 v = part[z][x];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    T* to = reinterpret_cast<T*>(a.out) + (int64_t)n * a.o_sn + (int64_t)hq * a.o_sh + 4 * x;
+    *reinterpret_cast<uint2*>(to) = make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
+    if (a.lse && x == 0)
+      a.lse[(int64_t)n * a.Hq + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
   }
-  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  T* to = reinterpret_cast<T*>(a.out) + (int64_t)n * a.o_sn + (int64_t)hq * a.o_sh + 4 * x;
-  *reinterpret_cast<uint2*>(to) = make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
-  if (a.lse && x == 0)
-    a.lse[(int64_t)n * a.Hq + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 namespace {
@@ -510,7 +510,9 @@ int launch_d(const AttnArgs& a, cudaStream_t stream) {
   if (grid > kAttnMaxGrid) return 2;
   if (a.max_context + a.max_nodes <= kKeyTile) return 0;  // one key tile: no item is split
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.N, a.Hq);
+  // About two blocks an SM at least; the more heads a block has, the less it costs where nothing was split.
+  int heads = (int)((int64_t)a.N * a.Hq / (4 * num_sms()) >= a.group ? a.group : 1);
+  cfg.gridDim = dim3(a.N, a.Hq / heads);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -519,7 +521,7 @@ int launch_d(const AttnArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   AttnArgs args = a;
-  void* params[3] = {&args, &rows, &grid};
+  void* params[4] = {&args, &rows, &grid, &heads};
   return cudaLaunchKernelExC(&cfg, (const void*)tree_attn_combine_kernel<T, D>, params) == cudaSuccess ? 0 : 2;
 }
 

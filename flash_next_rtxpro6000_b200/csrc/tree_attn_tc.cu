@@ -7,9 +7,8 @@
 //   O += P V    A = P (128 x 64, tensor memory, written over S), B = the tile's values as they lie
 //               in the cache (N contiguous), D = O (128 x D fp32, tensor memory)
 //
-// Two groups of softmax warps work side by side: on two row tiles of 128 (RT = 2: up to 256 rows that
-// share every key tile that is loaded), or on every other key tile of one (KS = 2), each group with its
-// own maximum, sum and O, joined at the end.  At D = 256 tensor memory has room for one O only.
+// RT row tiles of 128 share every key tile that is loaded (RT = 2: up to 256 rows, D <= 128), each with
+// its own group of softmax warps.
 // Keys and values travel through rings of 64-row chunks, in 64-element blocks of 128-byte rows with the
 // 128-byte swizzle: the same layout serves K-major keys and N-major values.
 //
@@ -18,9 +17,6 @@
 // warp that issues the first product and one the second.  O is rescaled only when a row's maximum has risen by more than 2^8: until then weights may
 // be larger than one, which costs nothing in floating point.
 // Every wait is bounded and records an error code; roles then fall through to the end.
-//
-// Measured before the second group and the separate loaders (24 requests, D = 128): a key tile took
-// 2,060 cycles, of which the softmax warps were busy for 1,560 and the loaders for 1,580.
 #include <type_traits>
 
 #include "tree_attn.cuh"
@@ -33,31 +29,28 @@ constexpr int kTile = kKeyTile;
 constexpr int kBlockBytes = kTile * 128;  // 64 rows of a 64-element block
 constexpr float kRise = 8.0f;
 
-template <int D, int RT, int KS>
+template <int D, int RT>
 struct TcAttn {
-  static constexpr int kGroups = RT * KS;               // of softmax warps
   static constexpr int kBlocks = D / 64;
   static constexpr int kChunk = kBlocks * kBlockBytes;  // keys or values of a tile
   static constexpr int kQTile = kBlocks * 128 * 128;    // a row tile of queries
   static constexpr int kK = D == 256 ? 2 : D == 128 ? (RT == 2 ? 4 : 5) : 8;  // chunks of the rings
   static constexpr int kV = D == 256 ? 3 : D == 128 ? (RT == 2 ? 5 : 6) : 8;
-  static constexpr int kLoad = 4 * kGroups, kIssue = kLoad + 8;  // first loading, first issuing warp
+  static constexpr int kLoad = 4 * RT, kIssue = kLoad + 8;  // first loading, first issuing warp
   static constexpr int kThreads = (kIssue + 4) * 32;  // the issuing warps are the last two of four
-  static constexpr int kCols = kGroups * (D + 2 * kTile) <= 256 ? 256 : 512;
-  static_assert(kGroups * (D + 2 * kTile) <= 512, "tensor memory");
+  static constexpr int kCols = RT * (D + 2 * kTile) <= 256 ? 256 : 512;
+  static_assert(RT * (D + 2 * kTile) <= 512, "tensor memory");
   struct Smem {
     uint8_t q[RT][kQTile];
     uint8_t k[kK][kChunk];
     uint8_t v[kV][kChunk];
     long long before[kAttnMaxBatch + 1];
     unsigned long long kfull[kK], kempty[kK], vfull[kV], vempty[kV];
-    unsigned long long sfull[kGroups][2], pfull[kGroups][2], odone[kGroups][2], qfull[RT];
-    unsigned long long joined[3];  // softmax warps of each group, of all
-    unsigned long long other;      // the second group is done with its key tiles
+    unsigned long long sfull[RT][2], pfull[RT][2], odone[RT][2], qfull[RT];
+    unsigned long long joined[2];  // softmax warps of the first row tile, of both
     unsigned long long drain;
     // drafted tokens whose values are not all finite, of this segment, the one before and the next
     unsigned long long odd[3];
-    float2 stat[KS == 2 ? 128 : 1];  // the second group's maxima and sums
     uint32_t tmem;
   };
 };
@@ -190,10 +183,10 @@ struct Segments {
 
 }  // namespace
 
-template <typename T, int D, int RT, int KS>
-__global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
-  using Cfg = TcAttn<D, RT, KS>;
-  constexpr int NK = Cfg::kK, NV = Cfg::kV, kBlocks = Cfg::kBlocks, kRows = 128 * RT, kGroups = Cfg::kGroups;
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
+  using Cfg = TcAttn<D, RT>;
+  constexpr int NK = Cfg::kK, NV = Cfg::kV, kBlocks = Cfg::kBlocks, kRows = 128 * RT;
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   typename Cfg::Smem& s = *reinterpret_cast<typename Cfg::Smem*>(base);
@@ -207,12 +200,13 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
   if (tid == 0) {
     for (int i = 0; i < NK; ++i) mbar_init(bar(s.kfull[i]), 4), mbar_init(bar(s.kempty[i]), 1);
     for (int i = 0; i < NV; ++i) mbar_init(bar(s.vfull[i]), 4), mbar_init(bar(s.vempty[i]), 1);
-    for (int w = 0; w < kGroups; ++w)
+    for (int r = 0; r < RT; ++r) {
       for (int i = 0; i < 2; ++i)
-        mbar_init(bar(s.sfull[w][i]), 1), mbar_init(bar(s.pfull[w][i]), 4), mbar_init(bar(s.odone[w][i]), 1);
-    for (int r = 0; r < RT; ++r) mbar_init(bar(s.qfull[r]), 4);
-    for (int i = 0; i < 3; ++i) mbar_init(bar(s.joined[i]), i < 2 ? 4 : 4 * kGroups);
-    mbar_init(bar(s.other), 4);
+        mbar_init(bar(s.sfull[r][i]), 1), mbar_init(bar(s.pfull[r][i]), 4), mbar_init(bar(s.odone[r][i]), 1);
+      mbar_init(bar(s.qfull[r]), 4);
+    }
+    mbar_init(bar(s.joined[0]), 4);
+    mbar_init(bar(s.joined[1]), 8);
     mbar_init(bar(s.drain), 2);
     s.odd[0] = s.odd[1] = s.odd[2] = 0ull;
     mbar_fence_init();
@@ -228,11 +222,11 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
   fence_after();
   const uint32_t tm = s.tmem;
   Segments sg(a, s.before, kRows, total, G);
-  // With two groups of softmax warps the others' registers go to them: 256 * 144 + 384 * 56 are no more
+  // With two row tiles the other warps' registers go to them: 256 * 144 + 384 * 56 are no more
   // than the launch's 640 * 96.
   if (warp >= Cfg::kLoad && warp < Cfg::kIssue) {
     // ------------------------------------------------------------------ loading warps
-    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     constexpr int kLanesRow = D / 8 < 32 ? D / 8 : 32;  // lanes of a row: 16 bytes each
     constexpr int kRowsPer = 32 / kLanesRow;            // rows of one instruction
     const int pw = warp & 3;                            // rows 16 pw .. + 15 of every chunk
@@ -294,21 +288,19 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
       run(std::integral_constant<int, NV>{}, reinterpret_cast<const T*>(a.v_cache), s.v[0], s.vfull, s.vempty, true);
   } else if (warp == Cfg::kIssue + 2) {
     // ------------------------------------------------------------------ S = Q K^T
-    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     constexpr uint32_t kId = attn_idesc(TcType<T>::kCode, 0, kTile);
     int i = 0;                  // tile of the CTA
-    int n[kGroups], segs[RT];  // tiles of each group, segments of each row tile
+    int n[RT], segs[RT];       // tiles and segments of each row tile
 #pragma unroll
-    for (int w = 0; w < kGroups; ++w) n[w] = 0;
-#pragma unroll
-    for (int r = 0; r < RT; ++r) segs[r] = 0;
+    for (int r = 0; r < RT; ++r) n[r] = segs[r] = 0;
     int code = 0;
     auto scores = [&](int w, int chunk) {
       // the weights of the buffer's tile before have been used
       if (!all_wait(s.odone[w][n[w] & 1], ((n[w] >> 1) & 1) ^ 1)) { code = ERR_WAIT_RFREE; return; }
       fence_after();
-      const uint32_t q = smem_u32(s.q[KS == 2 ? 0 : w]), k = smem_u32(s.k[chunk]);
-      const uint32_t d = tm + kGroups * D + (w * 2 + (n[w] & 1)) * kTile;
+      const uint32_t q = smem_u32(s.q[w]), k = smem_u32(s.k[chunk]);
+      const uint32_t d = tm + RT * D + (w * 2 + (n[w] & 1)) * kTile;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x)
         mma_ss(d, desc_sw128(q + (x >> 2) * (128 * 128) + (x & 3) * 32, 16, 1024),
@@ -328,14 +320,9 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
         const int c = i % NK;
         if (!all_wait(s.kfull[c], (i / NK) & 1)) { code = ERR_WAIT_FULL; break; }
         fence_after();
-        if (KS == 2) {
-          if ((t - sg.t0) & 1) scores(kGroups - 1, c);
-          else scores(0, c);
-        } else {
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-            if (r < rts && code == 0) scores(r, c);
-        }
+        for (int r = 0; r < RT; ++r)
+          if (r < rts && code == 0) scores(r, c);
         commit_to(s.kempty[c]);
       }
     }
@@ -344,16 +331,16 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
     if (!all_wait(s.drain, 0) && lane == 0) record_error(a.err, ERR_DRAIN);
   } else if (warp == Cfg::kIssue + 3) {
     // ------------------------------------------------------------------ O += P V
-    if (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     constexpr uint32_t kId = attn_idesc(TcType<T>::kCode, 1, D);
-    int i = 0, n[kGroups];
+    int i = 0, n[RT];
 #pragma unroll
-    for (int w = 0; w < kGroups; ++w) n[w] = 0;
+    for (int r = 0; r < RT; ++r) n[r] = 0;
     int code = 0;
     auto values = [&](int w, int chunk, bool add) {
       if (!all_wait(s.pfull[w][n[w] & 1], (n[w] >> 1) & 1)) { code = ERR_WAIT_RED; return; }
       fence_after();
-      const uint32_t v = smem_u32(s.v[chunk]), p = tm + kGroups * D + (w * 2 + (n[w] & 1)) * kTile;
+      const uint32_t v = smem_u32(s.v[chunk]), p = tm + RT * D + (w * 2 + (n[w] & 1)) * kTile;
 #pragma unroll
       for (int x = 0; x < kTile / 16; ++x)
         mma_ts(tm + w * D, p + 8 * x, desc_sw128(v + x * 2048, kBlockBytes, 1024), kId, add || x > 0);
@@ -363,16 +350,11 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
     while (code == 0 && sg.next()) {
       const int rts = RT == 1 ? 1 : (sg.live + 127) / 128;
       for (int t = sg.t0; code == 0 && t < sg.t1; ++t, ++i) {
-        const int c = i % NV, j = t - sg.t0;
+        const int c = i % NV;
         if (!all_wait(s.vfull[c], (i / NV) & 1)) { code = ERR_WAIT_FULL; break; }
-        if (KS == 2) {
-          if (j & 1) values(kGroups - 1, c, j > 1);
-          else values(0, c, j > 1);
-        } else {
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-            if (r < rts && code == 0) values(r, c, j > 0);
-        }
+        for (int r = 0; r < RT; ++r)
+          if (r < rts && code == 0) values(r, c, t > sg.t0);
         commit_to(s.vempty[c]);
       }
     }
@@ -381,29 +363,27 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
     if (!all_wait(s.drain, 0) && lane == 0) record_error(a.err, ERR_DRAIN);
   } else if (warp < Cfg::kLoad) {
     // ------------------------------------------------------------------ softmax
-    if (kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
-    const int w = warp >> 2, quad = warp & 3;  // group
-    const int rt = KS == 2 ? 0 : w;
+    if (RT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    const int rt = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;  // of the row tile, and its lane in tensor memory
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const float c2 = a.scale * 1.4426950408889634f;
-    // tiles of the group and of the CTA, segments, segments with a second group
-    int n = 0, tiles = 0, seg = 0, ends = 0;
+    int n = 0, tiles = 0, seg = 0;  // tiles of the row tile and of the CTA, segments
     bool ok = true;
-    int joins[3] = {0, 0, 0};
-    auto join = [&](int who) {  // a barrier of one group's warps, or of all, with a bounded wait
+    int joins[2] = {0, 0};
+    auto join = [&](int who) {  // a barrier of the live row tiles' warps, with a bounded wait
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(s.joined[who]));
       return all_wait(s.joined[who], joins[who]++ & 1);
     };
-    auto o_is_done = [&]() { return all_wait(s.odone[w][(n - 1) & 1], ((n - 1) >> 1) & 1); };
+    auto o_is_done = [&]() { return all_wait(s.odone[rt][(n - 1) & 1], ((n - 1) >> 1) & 1); };
     while (ok && sg.next()) {
       const int first_tile = tiles;
       tiles += sg.t1 - sg.t0;
       unsigned long long* odds = &s.odd[seg % 3];
       ++seg;
       if (rt * 128 >= sg.live) continue;
-      const int who = RT == 2 && sg.live > 128 ? 2 : w, threads = who == 2 ? 256 : 128;
+      const int who = RT == 2 && sg.live > 128 ? 1 : 0, threads = who ? 256 : 128;
       const int r = rt * 128 + row;
       const bool mine = r < sg.live;
       const bool busy = rt * 128 + quad * 32 < sg.live;  // the warp has a live row
@@ -411,7 +391,7 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
       const int hq = sg.head * a.group + (sg.row0 + r) % a.group;
       const int64_t qn = sg.rq.n0 + node;
       const unsigned long long mask = mine ? attn_mask(a, sg.rq, node) : 0ull;
-      if (KS == 1 || w == 0) {
+      {
         const T* q = reinterpret_cast<const T*>(a.q) + qn * a.q_sn + (int64_t)hq * a.q_sh;
         uint8_t* to = s.q[rt] + row * 128;
 #pragma unroll 8
@@ -426,11 +406,10 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
       }
       float ref = -INFINITY, sum = 0.f;
       const int len = sg.rq.ctx + sg.rq.nodes;
-      const int begin = sg.t0 + (KS == 2 ? w : 0);
-      for (int t = begin; t < sg.t1; t += KS, ++n) {
+      for (int t = sg.t0; t < sg.t1; ++t, ++n) {
         const int pos0 = t * kTile;
         const bool tail = pos0 + kTile > sg.rq.ctx;
-        if (!all_wait(s.sfull[w][n & 1], (n >> 1) & 1)) {
+        if (!all_wait(s.sfull[rt][n & 1], (n >> 1) & 1)) {
           if (lane == 0) record_error(a.err, ERR_WAIT_RED);
           ok = false;
           break;
@@ -442,7 +421,7 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
           const int chunk = first_tile + t - sg.t0;
           ok = all_wait(s.vfull[chunk % NV], (chunk / NV) & 1) && join(who);
           uint8_t* v = s.v[chunk % NV];
-          for (int u = (who == 2 ? rt * 128 : 0) + row; u < kTile * kBlocks * 8; u += threads) {
+          for (int u = rt * 128 + row; u < kTile * kBlocks * 8; u += threads) {
             const int j = (u >> 3) % kTile;  // unit u: block, row, place
             if (pos0 + j < sg.rq.ctx || pos0 + j >= len) continue;
             const uint4 x = lds128(v + u * 16);
@@ -452,7 +431,7 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
           ok = ok && join(who);
           const unsigned long long odd = *reinterpret_cast<volatile unsigned long long*>(odds);
           if (odd) {
-            for (int u = (who == 2 ? rt * 128 : 0) + row; u < kTile * kBlocks * 8; u += threads) {
+            for (int u = rt * 128 + row; u < kTile * kBlocks * 8; u += threads) {
               const int d = pos0 + (u >> 3) % kTile - sg.rq.ctx;
               if (d >= 0 && d < sg.rq.nodes && (odd >> d & 1)) *reinterpret_cast<uint4*>(v + u * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
@@ -464,7 +443,7 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
             break;
           }
         }
-        const uint32_t sp = tm + lanes + kGroups * D + (w * 2 + (n & 1)) * kTile;
+        const uint32_t sp = tm + lanes + RT * D + (rt * 2 + (n & 1)) * kTile;
         if (busy) {
           float x[kTile];
           ld32(sp, reinterpret_cast<uint32_t*>(x));
@@ -482,7 +461,7 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
           for (int j = 0; j < kTile; ++j) m4[j & 3] = fmaxf(m4[j & 3], x[j]);
           const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c2;
           const bool rise = mx > ref + kRise || (ref == -INFINITY && mx > ref);
-          if (t == begin) {
+          if (t == sg.t0) {
             ref = mx;
           } else if (__any_sync(0xffffffffu, rise)) {
             if (!o_is_done()) {
@@ -496,11 +475,11 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               float o[32];
-              ld32(tm + lanes + w * D + c, reinterpret_cast<uint32_t*>(o));
+              ld32(tm + lanes + rt * D + c, reinterpret_cast<uint32_t*>(o));
               wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] *= f;
-              st32(tm + lanes + w * D + c, reinterpret_cast<const uint32_t*>(o));
+              st32(tm + lanes + rt * D + c, reinterpret_cast<const uint32_t*>(o));
             }
             sum *= f;
             ref = to;
@@ -522,37 +501,18 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
           fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(s.pfull[w][n & 1]));
+        if (lane == 0) mbar_arrive(bar(s.pfull[rt][n & 1]));
       }
       if (!ok) break;
-      const bool two = KS == 2 && sg.t1 - sg.t0 > 1;  // the second group has a part of the sums
-      if (begin < sg.t1 && !o_is_done()) {
+      if (!o_is_done()) {
         if (lane == 0) record_error(a.err, ERR_WAIT_RED);
         break;
       }
       fence_after();
-      if (KS == 2 && w == 1) {
-        if (two) {
-          s.stat[row] = make_float2(ref, sum);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(s.other));
-        }
-        continue;
-      }
-      float ref2 = -INFINITY, sum2 = 0.f;
-      if (two) {
-        if (!all_wait(s.other, ends++ & 1)) {
-          if (lane == 0) record_error(a.err, ERR_WAIT_RED);
-          break;
-        }
-        fence_after();
-        ref2 = s.stat[row].x;
-        sum2 = s.stat[row].y;
-      }
       if (busy) {
-        const uint32_t oa = tm + lanes + w * D;
+        const uint32_t oa = tm + lanes + rt * D;
         unsigned long long odd = sg.t1 * kTile > sg.rq.ctx ? *reinterpret_cast<volatile unsigned long long*>(odds) : 0ull;
-        const bool added = odd != 0ull;
+
         while (odd) {  // rare: values that are not finite, for the rows that see them
           const int d = __ffsll((long long)odd) - 1;
           odd &= odd - 1;
@@ -583,12 +543,8 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
           }
           wait_st();
         }
-        const float top = fmaxf(ref, ref2), zero = top == -INFINITY ? 0.f : top;
-        const float f1 = exp2_fast((added && ref == -INFINITY ? 0.f : ref) - zero), f2 = exp2_fast(ref2 - zero);
-        sum = two ? sum * f1 + sum2 * f2 : sum;
         const bool all = sg.first && sg.last;
         const float inv = all ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
-        const float g1 = two ? f1 * inv : inv, g2 = f2 * inv;
         T* out = reinterpret_cast<T*>(a.out) + qn * a.o_sn + (int64_t)hq * a.o_sh;
         float* slot = a.partials + (2ll * blockIdx.x + (sg.first ? 1 : 0)) * attn_slot_floats(kRows, D);
 #pragma unroll 1
@@ -598,14 +554,7 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
           ld32(oa + c, reinterpret_cast<uint32_t*>(o));
           wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= g1;
-          if (KS == 2 && two) {
-            float o2[32];
-            ld32(oa + D + c, reinterpret_cast<uint32_t*>(o2));
-            wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] += o2[e] * g2;
-          }
+          for (int e = 0; e < 32; ++e) o[e] *= inv;
           if (mine && all) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
@@ -623,14 +572,14 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
           }
         }
         if (mine && all && a.lse)
-          a.lse[qn * a.Hq + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+          a.lse[qn * a.Hq + hq] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
         if (mine && !all)
-          *reinterpret_cast<float2*>(slot + (int64_t)kRows * D + 2 * r) = make_float2(top, sum);
+          *reinterpret_cast<float2*>(slot + (int64_t)kRows * D + 2 * r) = make_float2(ref, sum);
       }
       __syncwarp();
       fence_before();
     }
-  } else if (kGroups == 2) {
+  } else if (RT == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   }
   fence_before();
@@ -643,10 +592,10 @@ __global__ void __launch_bounds__((4 * RT * KS + 12) * 32, 1) tree_attn_tc_kerne
 
 namespace {
 
-template <typename T, int D, int RT, int KS>
+template <typename T, int D, int RT>
 int launch_tc(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
-  using Cfg = TcAttn<D, RT, KS>;
-  const void* k = (const void*)tree_attn_tc_kernel<T, D, RT, KS>;
+  using Cfg = TcAttn<D, RT>;
+  const void* k = (const void*)tree_attn_tc_kernel<T, D, RT>;
   if (!prepare_kernel(k)) return 2;
   grid = num_sms();
   rows = 128 * RT;
@@ -657,10 +606,10 @@ template <typename T>
 int launch_tc_t(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
   const bool wide = a.max_nodes * a.group > 128;
   if (a.D == 64)
-    return wide ? launch_tc<T, 64, 2, 1>(a, stream, grid, rows) : launch_tc<T, 64, 1, 2>(a, stream, grid, rows);
+    return wide ? launch_tc<T, 64, 2>(a, stream, grid, rows) : launch_tc<T, 64, 1>(a, stream, grid, rows);
   if (a.D == 128)
-    return wide ? launch_tc<T, 128, 2, 1>(a, stream, grid, rows) : launch_tc<T, 128, 1, 2>(a, stream, grid, rows);
-  return launch_tc<T, 256, 1, 1>(a, stream, grid, rows);
+    return wide ? launch_tc<T, 128, 2>(a, stream, grid, rows) : launch_tc<T, 128, 1>(a, stream, grid, rows);
+  return launch_tc<T, 256, 1>(a, stream, grid, rows);
 }
 
 }  // namespace
