@@ -395,94 +395,122 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn_kernel(const __grid
   }
 }
 
-// Adds up the partial results of the items that several CTAs held: one block per node and `heads` query
-// heads of a kv head (one, or all of a group where there are many nodes).
-// First the slots' maxima and sums, which give each slot its factor; then the sums, D / 4 threads by
-// four elements each, thread groups by the item's slots in turn, with several loads in flight.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) tree_attn_combine_kernel(const __grid_constant__ AttnArgs a, int rows, int grid, int heads) {
-  constexpr int kWide = D / 4, kGroups = 256 / kWide;
-  __shared__ long long before[kAttnMaxBatch + 1];
-  __shared__ long long scratch[8];
-  __shared__ float4 part[kGroups][kWide];
-  __shared__ float factor[kAttnMaxGrid];
-  __shared__ float red[8], red2[8];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, x = tid % kWide, y = tid / kWide;
-  // the lengths were there before the launch whose partials these are: only those are waited for
-  attn_prefix(a, rows, before, scratch, false);
-  const long long total = before[a.B];
-  const long long G = total < (long long)grid ? total : (long long)grid;
-  const int n = blockIdx.x;
-  // the request that holds node n
+// Where the partial results of (node n, head hq) are: the CTAs c0 .. c1 that held its item, and its row in
+// their slots; c0 == c1 where one CTA held the item and wrote the result itself, or there is none.
+struct Parts {
+  int c0, c1, row;
+};
+__device__ __forceinline__ Parts find_parts(const AttnArgs& a, const AttnReq& rq, long long ahead, long long total,
+                                            long long G, int rows, int n, int hq) {
+  if (total == 0 || n < rq.n0 || n >= rq.n0 + rq.nodes) return Parts{0, 0, 0};
+  const AttnShape sh = attn_shape(a, rq, rows);
+  const int row = (n - rq.n0) * a.group + hq % a.group;
+  const int item = hq / a.group * sh.row_tiles + row / rows;
+  const long long item0 = ahead + (long long)item * sh.key_tiles, item1 = item0 + sh.key_tiles;
+  return Parts{attn_cta_of(item0, total, G), attn_cta_of(item1 - 1, total, G), row % rows};
+}
+
+// The request that holds node n.
+__device__ __forceinline__ int request_of(const AttnArgs& a, int n) {
   int lo = 0, hi = a.B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (a.node_offsets[mid] <= n) lo = mid;
     else hi = mid;
   }
-  const AttnReq rq = attn_request(a, lo, false);
-  const bool held = total > 0 && n >= rq.n0 && n < rq.n0 + rq.nodes;
+  return lo;
+}
+
+// Adds up the partial results of the items that several CTAs held.  First the slots' maxima and sums, which
+// give each slot its factor; then the sums, with several loads in flight.  WPR warps share a row (a node's
+// query head): 8 where rows are few and their slots many, 1 where there are rows for every warp (measured
+// at 24 ragged requests: 14 us less than a block a row; at 256 rows of 74 slots a block a row is faster).
+template <typename T, int D, int WPR>
+__global__ void __launch_bounds__(256) tree_attn_combine_kernel(const __grid_constant__ AttnArgs a, int rows, int grid) {
+  constexpr int kPer = D / 32;  // columns of a lane: pairs or fours, 32 lanes apart
+  constexpr int kVec = kPer < 4 ? kPer : 4, kN = kPer / kVec;
+  __shared__ long long before[kAttnMaxBatch + 1];
+  __shared__ long long scratch[8];
+  __shared__ float factor[8 / WPR][kAttnMaxGrid];
+  __shared__ float part[WPR == 8 ? 8 : 1][WPR == 8 ? D : 1];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // the lengths were there before the launch whose partials these are: only those are waited for
+  attn_prefix(a, rows, before, scratch, false);
+  const long long total = before[a.B];
+  const long long G = total < (long long)grid ? total : (long long)grid;
+  const int n = blockIdx.x, hq = WPR == 8 ? blockIdx.y : blockIdx.y * 8 + warp;
+  const int b = request_of(a, n);
+  const Parts p = hq < a.Hq ? find_parts(a, attn_request(a, b, false), before[b], total, G, rows, n, hq) : Parts{0, 0, 0};
   pdl_wait();
-  if (!held) return;
-  const AttnShape sh = attn_shape(a, rq, rows);
+  if (p.c0 == p.c1) return;
   const int64_t size = attn_slot_floats(rows, D);
-  for (int hq = blockIdx.y * heads; hq < (int)(blockIdx.y + 1) * heads; ++hq) {
-    const int head = hq / a.group, row = (n - rq.n0) * a.group + hq % a.group;
-    const int item = head * sh.row_tiles + row / rows, r = row % rows;
-    const long long item0 = before[lo] + (long long)item * sh.key_tiles, item1 = item0 + sh.key_tiles;
-    const int c0 = attn_cta_of(item0, total, G), c1 = attn_cta_of(item1 - 1, total, G);
-    if (c0 == c1) continue;  // written by the one CTA that held it
-    // slot of contributor i: the item's first CTA holds its beginning, the others from their start
-    auto slot = [&](int i) { return a.partials + (2ll * (c0 + i) + (i == 0 ? 1 : 0)) * size; };
-    const int count = c1 - c0 + 1;  // at most the grid
-    float2 st = make_float2(-INFINITY, 0.f);
-    if (tid < count) st = __ldcg(reinterpret_cast<const float2*>(slot(tid) + (int64_t)rows * D + 2 * r));
-    float top = st.x;
+  // slot of contributor i: the item's first CTA holds its beginning, the others from their start
+  auto slot = [&](int i) { return a.partials + (2ll * (p.c0 + i) + (i == 0 ? 1 : 0)) * size; };
+  const int count = p.c1 - p.c0 + 1;  // at most the grid
+  float2 st[kAttnMaxGrid / 32];
+  float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    __syncthreads();  // the head before is done with shared memory
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float f = exp2_fast(st.x - ref);
-    if (tid < count) factor[tid] = f;
-    float sum = tid < count ? st.y * f : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) red2[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) sum += red2[w];
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = y; i < count; i += kGroups) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (int64_t)r * D + 4 * x));
-      const float g = factor[i];
-      acc.x += v.x * g;
-      acc.y += v.y * g;
-      acc.z += v.z * g;
-      acc.w += v.w * g;
-    }
-    part[y][x] = acc;
-    __syncthreads();
-    if (y != 0) continue;
-#pragma unroll
-    for (int z = 1; z < kGroups; ++z) {
-      const float4 v = part[z][x];
-      acc.x += v.x;
-      acc.y += v.y;
-      acc.z += v.z;
-      acc.w += v.w;
-    }
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    T* to = reinterpret_cast<T*>(a.out) + (int64_t)n * a.o_sn + (int64_t)hq * a.o_sh + 4 * x;
-    *reinterpret_cast<uint2*>(to) = make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
-    if (a.lse && x == 0)
-      a.lse[(int64_t)n * a.Hq + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  for (int z = 0; z < kAttnMaxGrid / 32; ++z) {
+    const int i = z * 32 + lane;
+    st[z] = i < count ? __ldcg(reinterpret_cast<const float2*>(slot(i) + (int64_t)rows * D + 2 * p.row))
+                      : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, st[z].x);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float ref = top == -INFINITY ? 0.f : top;
+  float* mine = factor[WPR == 8 ? 0 : warp];  // WPR = 8: every warp writes the same
+#pragma unroll
+  for (int z = 0; z < kAttnMaxGrid / 32; ++z) {
+    const float f = exp2_fast(st[z].x - ref);
+    sum += st[z].y * f;
+    if (z * 32 + lane < count) mine[z * 32 + lane] = f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncwarp();
+  float acc[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+#pragma unroll 8
+  for (int i = WPR == 8 ? warp : 0; i < count; i += WPR) {
+    const float* from = slot(i) + (int64_t)p.row * D + lane * kVec;
+    const float g = mine[i];
+#pragma unroll
+    for (int z = 0; z < kN; ++z) {
+      if (kVec == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + z * 128));
+        acc[z * 4] += v.x * g, acc[z * 4 + 1] += v.y * g, acc[z * 4 + 2] += v.z * g, acc[z * 4 + 3] += v.w * g;
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(from));
+        acc[0] += v.x * g, acc[1] += v.y * g;
+      }
+    }
+  }
+  if (WPR == 8) {
+#pragma unroll
+    for (int z = 0; z < kN; ++z)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) part[warp][z * 128 + lane * kVec + e] = acc[z * kVec + e];
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int z = 0; z < kN; ++z)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) acc[z * kVec + e] += part[w][z * 128 + lane * kVec + e];
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  T* to = reinterpret_cast<T*>(a.out) + (int64_t)n * a.o_sn + (int64_t)hq * a.o_sh + lane * kVec;
+#pragma unroll
+  for (int z = 0; z < kN; ++z)
+#pragma unroll
+    for (int e = 0; e < kVec; e += 2)
+      *reinterpret_cast<uint32_t*>(to + z * 128 + e) =
+          Mma<T>::pack(acc[z * kVec + e] * inv, acc[z * kVec + e + 1] * inv);
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)n * a.Hq + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 namespace {
@@ -502,7 +530,13 @@ template <typename T, int D>
 int launch_d(const AttnArgs& a, cudaStream_t stream) {
   int grid = 0, rows = 0, rc;
   const int most = a.max_nodes * a.group;
-  if (most > 32) rc = launch_tree_attn_tc(a, stream, grid, rows);
+  // The tensor-memory form needs some tiles a CTA to pay for its start-up and its row tiles of 128.  In
+  // key tiles an SM, times row tiles of 32: one token over 1,000 keys (0.2) 12.1 us here and 15.2 there,
+  // 4 requests of 16 nodes over 1,000 (7.4) 23.7 and 29.1, one token over 32k (7) 29.4 and 32.3, 8 nodes
+  // over 32k (14) 43.8 and 36.7, 16 nodes over 32k (28) 63.8 and 38.9, 16 requests of one token over 8k
+  // (111) 117 and 88.
+  const int64_t tiles = (int64_t)a.B * a.Hk * ((a.max_context + a.max_nodes + kKeyTile - 1) / kKeyTile);
+  if (tiles * ((most + 31) / 32) > 8 * num_sms()) rc = launch_tree_attn_tc(a, stream, grid, rows);
   else if (most <= 16) rc = launch_form<T, D, 1, 4>(a, stream, grid, rows);
   else if (most <= 32) rc = launch_form<T, D, 2, 4>(a, stream, grid, rows);
   else rc = launch_form<T, D, 4, 2>(a, stream, grid, rows);
@@ -510,9 +544,8 @@ int launch_d(const AttnArgs& a, cudaStream_t stream) {
   if (grid > kAttnMaxGrid) return 2;
   if (a.max_context + a.max_nodes <= kKeyTile) return 0;  // one key tile: no item is split
   cudaLaunchConfig_t cfg = {};
-  // About two blocks an SM at least; the more heads a block has, the less it costs where nothing was split.
-  int heads = (int)((int64_t)a.N * a.Hq / (4 * num_sms()) >= a.group ? a.group : 1);
-  cfg.gridDim = dim3(a.N, a.Hq / heads);
+  const bool many = (int64_t)a.N * a.Hq >= 8 * num_sms();  // a row for each of eight warps an SM
+  cfg.gridDim = dim3(a.N, many ? (a.Hq + 7) / 8 : a.Hq);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -521,8 +554,9 @@ int launch_d(const AttnArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   AttnArgs args = a;
-  void* params[4] = {&args, &rows, &grid, &heads};
-  return cudaLaunchKernelExC(&cfg, (const void*)tree_attn_combine_kernel<T, D>, params) == cudaSuccess ? 0 : 2;
+  void* params[3] = {&args, &rows, &grid};
+  const void* k = many ? (const void*)tree_attn_combine_kernel<T, D, 1> : (const void*)tree_attn_combine_kernel<T, D, 8>;
+  return cudaLaunchKernelExC(&cfg, k, params) == cudaSuccess ? 0 : 2;
 }
 
 template <typename T>

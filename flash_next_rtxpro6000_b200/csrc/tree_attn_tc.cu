@@ -1,22 +1,30 @@
-// Tree attention on the 5th-generation tensor cores (tcgen05), for the requests whose nodes and query
-// heads fill a good part of a 128-row operand.  The operator, the split of the work and the partial
-// results are those of tree_attn.cu; here the two products run asynchronously with their operands and
-// sums in shared and tensor memory, so loading, products and softmax of different key tiles overlap:
+// Tree attention on the 5th-generation tensor cores (tcgen05), for launches with several key tiles an
+// SM.  The operator, the split of the work and the partial results are those of tree_attn.cu; here the
+// two products run asynchronously with their operands and sums in shared and tensor memory, so loading,
+// products and softmax of different key tiles overlap:
 //
 //   S = Q K^T   A = Q (128 rows x D, shared memory), B = a tile of 64 keys (shared memory)
 //   O += P V    A = P (128 x 64, tensor memory, written over S), B = the tile's values as they lie
 //               in the cache (N contiguous), D = O (128 x D fp32, tensor memory)
 //
 // RT row tiles of 128 share every key tile that is loaded (RT = 2: up to 256 rows, D <= 128), each with
-// its own group of softmax warps.
-// Keys and values travel through rings of 64-row chunks, in 64-element blocks of 128-byte rows with the
-// 128-byte swizzle: the same layout serves K-major keys and N-major values.
+// its own group of softmax warps.  Keys and values travel through rings of 64-row chunks, in 64-element
+// blocks of 128-byte rows with the 128-byte swizzle: the same layout serves K-major keys and N-major
+// values.
 //
-// Roles: 4 softmax warps a group (a thread has a row: its scores come from tensor memory in one piece, so
-// the row's maximum and sum need no shuffles), 4 warps that load keys and 4 that load values (cp.async, any page size), one
-// warp that issues the first product and one the second.  O is rescaled only when a row's maximum has risen by more than 2^8: until then weights may
-// be larger than one, which costs nothing in floating point.
-// Every wait is bounded and records an error code; roles then fall through to the end.
+// Roles: 4 softmax warps a row tile (a thread has a row: its scores come from tensor memory in one
+// piece, so the row's maximum and sum need no shuffles), 4 warps that load keys and 4 that load values
+// (cp.async, any page size), one warp that issues the first product and one the second.  O is rescaled
+// only when a row's maximum has risen by more than 2^8: until then weights may be larger than one, which
+// costs nothing in floating point.  Every wait is bounded and records an error code; roles then fall
+// through to the end.
+//
+// Measured (B200): 24 ragged requests, D = 128 fp16, 357 MB: 103 us, 3.4 TB/s; 4 requests of 64 nodes
+// over 131,072 keys, 1.48 GB and 171 GFLOP: 397 us, 3.7 TB/s and 430 TFLOP/s.  Loading alone (the rings
+// emptied at once) takes 234 us at the latter.  What bounds it is the softmax warps' chain per tile:
+// about 1,800 cycles from scores to weights, of which the exponentials' unit is busy for 512 a row tile.
+// A second group on every other key tile of the same rows gained nothing (the rows' quarter of the SM
+// has one unit for both groups), nor did deeper rings.
 #include <type_traits>
 
 #include "tree_attn.cuh"
@@ -145,6 +153,18 @@ __device__ __forceinline__ bool odd_pair(uint32_t w) {
   return (w & e) == e || ((w >> 16) & e) == e;
 }
 
+// The softmax warps hold a row's 64 scores and take registers that the others do not need: with one row
+// tile 128 * 192 + 384 * 104 are no more than the launch's 512 * 128, with two 256 * 144 + 384 * 56 no
+// more than 640 * 96.
+template <int RT> __device__ __forceinline__ void give_registers() {
+  if (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+}
+template <int RT> __device__ __forceinline__ void take_registers() {
+  if (RT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+}
+
 // The CTA's segments, one after the other: the same for every role.
 struct Segments {
   const AttnArgs& a;
@@ -222,11 +242,9 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
   fence_after();
   const uint32_t tm = s.tmem;
   Segments sg(a, s.before, kRows, total, G);
-  // With two row tiles the other warps' registers go to them: 256 * 144 + 384 * 56 are no more
-  // than the launch's 640 * 96.
   if (warp >= Cfg::kLoad && warp < Cfg::kIssue) {
     // ------------------------------------------------------------------ loading warps
-    if (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    give_registers<RT>();
     constexpr int kLanesRow = D / 8 < 32 ? D / 8 : 32;  // lanes of a row: 16 bytes each
     constexpr int kRowsPer = 32 / kLanesRow;            // rows of one instruction
     const int pw = warp & 3;                            // rows 16 pw .. + 15 of every chunk
@@ -288,7 +306,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
       run(std::integral_constant<int, NV>{}, reinterpret_cast<const T*>(a.v_cache), s.v[0], s.vfull, s.vempty, true);
   } else if (warp == Cfg::kIssue + 2) {
     // ------------------------------------------------------------------ S = Q K^T
-    if (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    give_registers<RT>();
     constexpr uint32_t kId = attn_idesc(TcType<T>::kCode, 0, kTile);
     int i = 0;                  // tile of the CTA
     int n[RT], segs[RT];       // tiles and segments of each row tile
@@ -331,7 +349,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
     if (!all_wait(s.drain, 0) && lane == 0) record_error(a.err, ERR_DRAIN);
   } else if (warp == Cfg::kIssue + 3) {
     // ------------------------------------------------------------------ O += P V
-    if (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    give_registers<RT>();
     constexpr uint32_t kId = attn_idesc(TcType<T>::kCode, 1, D);
     int i = 0, n[RT];
 #pragma unroll
@@ -363,7 +381,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
     if (!all_wait(s.drain, 0) && lane == 0) record_error(a.err, ERR_DRAIN);
   } else if (warp < Cfg::kLoad) {
     // ------------------------------------------------------------------ softmax
-    if (RT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    take_registers<RT>();
     const int rt = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;  // of the row tile, and its lane in tensor memory
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
@@ -394,7 +412,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
       {
         const T* q = reinterpret_cast<const T*>(a.q) + qn * a.q_sn + (int64_t)hq * a.q_sh;
         uint8_t* to = s.q[rt] + row * 128;
-#pragma unroll 8
+#pragma unroll 16
         for (int c = 0; c < D / 8; ++c) {
           const uint4 x = mine ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0u, 0u, 0u, 0u);
           *reinterpret_cast<uint4*>(to + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = x;
@@ -543,7 +561,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
           }
           wait_st();
         }
-        const bool all = sg.first && sg.last;
+        const bool all = sg.first && sg.last, dense = sg.live - rt * 128 - quad * 32 > 8;
         const float inv = all ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
         T* out = reinterpret_cast<T*>(a.out) + qn * a.o_sn + (int64_t)hq * a.o_sh;
         float* slot = a.partials + (2ll * blockIdx.x + (sg.first ? 1 : 0)) * attn_slot_floats(kRows, D);
@@ -565,10 +583,27 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
               y.w = pack2<T>(o[e + 6], o[e + 7]);
               *reinterpret_cast<uint4*>(out + c + e) = y;
             }
-          } else if (mine) {
+          }
+          if (mine && !all && !dense) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<float4*>(slot + (int64_t)r * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+          if (!all && dense) {
+            // A row a thread would touch 32 lines a store: the warp's 32 rows x 32 columns go through the
+            // queries' place of its rows (they have been used), and out four whole lines a store.
+            uint8_t* turn = s.q[rt] + quad * 32 * 128;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(turn + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                  make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int y = e * 4 + (lane >> 3), k = lane & 7, ry = rt * 128 + quad * 32 + y;
+              const float4 v = *reinterpret_cast<const float4*>(turn + y * 128 + ((k ^ (y & 7)) << 4));
+              if (ry < sg.live) *reinterpret_cast<float4*>(slot + (int64_t)ry * D + c + 4 * k) = v;
+            }
           }
         }
         if (mine && all && a.lse)
@@ -579,8 +614,8 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
       __syncwarp();
       fence_before();
     }
-  } else if (RT == 2) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  } else {
+    give_registers<RT>();
   }
   fence_before();
   __syncthreads();

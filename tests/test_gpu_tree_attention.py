@@ -383,3 +383,58 @@ def test_trees_across_key_tiles(ctx):
     for j in (0, 3, 63):
         sees = torch.tensor([bool(c.masks[i] >> j & 1) for i in range(64)], device=dev())
         assert torch.equal(out[:64, 2, j].isnan(), sees)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,Hq,Hk,T", [(64, 8, 4, 1), (64, 12, 12, 33), (64, 8, 2, 64), (128, 16, 4, 1), (128, 16, 4, 20),
+                                       (128, 16, 4, 64), (256, 16, 4, 1), (256, 8, 4, 64), (256, 16, 2, 40)])
+def test_batches_that_fill_the_gpu(D, Hq, Hk, T, dtype):
+    """Enough key tiles for the tensor-memory form, with short, empty and odd requests among long ones."""
+    lens = [5000, 0, 1, 63, 64, 4000, 129, 3000, 7, 4999, 2500, 4095]
+    counts = [T, 1, T, T, 0, max(1, T - 1), T, 1, T, T, 2, T]
+    counts = [min(c, T) for c in counts]
+    big = 12 * Hk * 80 > 8 * 148  # what the launch goes by: requests, kv heads, key tiles of the longest
+    assert big
+    Case(lens, counts, Hq, Hk, D, 16, dtype, seed=T + D, garbage=True).check()
+
+
+@pytest.mark.parametrize("D,T", [(64, 40), (128, 20), (128, 64), (256, 24)])
+@pytest.mark.parametrize("how", ["any", "none"])
+def test_batches_with_any_mask(D, T, how):
+    lens = [6000, 0, 0, 70, 5999, 64, 5000, 1]
+    c = Case(lens, [T, T, 1, T, T, 3, T, T], 8, 4, D, 24, torch.bfloat16, seed=3, how=how)
+    out, lse = c.check()
+    if how == "none":
+        assert bool((out[T:2 * T] == 0).all()) and bool((lse[T:2 * T] == -float("inf")).all())
+
+
+@pytest.mark.parametrize("D,T", [(64, 40), (128, 20), (128, 64), (256, 24)])
+def test_batches_not_finite_where_hidden(D, T):
+    lens = [6000, 3, 64 * 60 - 5, 5999, 5000]
+    c = Case(lens, [T] * 5, 8, 4, D, 16, torch.bfloat16, seed=13, garbage=True)
+    for b in range(5):
+        for j in (T // 2, T - 1):
+            slot = int(c.table[b][(lens[b] + j) // 16]) * 16 + (lens[b] + j) % 16
+            c.v.view(-1, 4, D)[slot, :, j] = float("nan") if b % 2 else float("inf")
+            if b == 3:
+                c.k.view(-1, 4, D)[slot] = float("nan")
+    out, lse = c.run()
+    want, _, wlse, _ = c.reference()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf())
+    assert torch.equal(lse.isnan(), wlse.isnan())
+    fine = want.isfinite()
+    assert float((out.double() - want)[fine].abs().max()) < 2.0**-6
+    _fx().check_device_errors()
+
+
+@pytest.mark.parametrize("D,Hq,T", [(64, 4, 30), (128, 4, 9), (128, 8, 64), (256, 4, 30)])
+def test_batches_with_rising_scores(D, Hq, T):
+    c = Case([6000] * 16, [T] * 16, Hq, 1, D, 16, torch.bfloat16, seed=D + T)
+    c.q = c.q * 0.1
+    c.q[:, :, 0] = 1.0
+    pos = torch.arange(6000, device=dev())
+    for b in range(16):
+        slots = c.table[b].long()[pos // 16] * 16 + pos % 16
+        sign = 1 if b % 2 else -1
+        c.k.view(-1, 1, D)[slots, 0, 0] = (sign * pos.float() * 0.02 * D**0.5).bfloat16()
+    c.check()
