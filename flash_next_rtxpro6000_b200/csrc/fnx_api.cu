@@ -72,6 +72,16 @@ int cuda_fail(const char* what) {
   return fail(FNX_ECUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// A launch's status; no C++ exception (the host's memory running out) leaves the C entry points.
+template <typename F>
+int launched(F&& f) noexcept {
+  try {
+    return f();
+  } catch (...) {
+    return 2;
+  }
+}
+
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 int chunk_k(int wt) {
@@ -1330,7 +1340,7 @@ int fnx_rotary_append(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
   for (int64_t st : {q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh}) ok = ok && vec8(st);
   for (int i = 0; i < 3; ++i) ok = ok && vec8(a.kc_st[i]) && vec8(a.vc_st[i]);
   a.vectors = ok;
-  if (fnx::launch_rotary(a, static_cast<cudaStream_t>(stream))) return cuda_fail("rotary launch");
+  if (launched([&] { return fnx::launch_rotary(a, static_cast<cudaStream_t>(stream)); })) return cuda_fail("rotary launch");
   return FNX_OK;
 }
 
@@ -1363,7 +1373,7 @@ int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
   a.slots = slots;
   a.err = error_flag;
   a.pdl = pdl;
-  if (fnx::launch_tree_layout(a, static_cast<cudaStream_t>(stream)))
+  if (launched([&] { return fnx::launch_tree_layout(a, static_cast<cudaStream_t>(stream)); }))
     return cuda_fail("tree layout launch");
   return FNX_OK;
 }
@@ -1444,7 +1454,7 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
     a.page_table = page_table + (int64_t)b0 * table_ld;
     a.context_lens = context_lens + b0;
     a.node_offsets = node_offsets + b0;
-    if (fnx::launch_tree_attn(a, static_cast<cudaStream_t>(stream)))
+    if (launched([&] { return fnx::launch_tree_attn(a, static_cast<cudaStream_t>(stream)); }))
       return cuda_fail("tree attention launch");
   }
   return FNX_OK;
@@ -1477,7 +1487,7 @@ int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const f
   a.tokens = tokens;
   a.probs = probs;
   a.pdl = pdl;
-  if (fnx::launch_sample(a, static_cast<cudaStream_t>(stream))) return cuda_fail("sampling launch");
+  if (launched([&] { return fnx::launch_sample(a, static_cast<cudaStream_t>(stream)); })) return cuda_fail("sampling launch");
   return FNX_OK;
 }
 

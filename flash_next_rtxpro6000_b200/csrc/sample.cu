@@ -26,6 +26,10 @@
 //     both values' intervals are sent at once.  An interval with more tokens than the list holds
 //     (many ties, or one token far from the others) is split again by order key and token index
 //     until it fits.
+// Measured (B200): one row of 151,936 bf16 logits 10 us with a top-k of 50, 25 to 31 without top-k (of some
+// 57,000 cycles the histogram's pass takes 15,000 to 19,000, its exponentials and shared-memory adds in
+// equal parts, the gathering 9,000, the exchanges about 1,500 each); 16 such rows in fp32 28 to 32 us; 128
+// rows of 248,320 137 us.
 #include <cooperative_groups.h>
 
 #include <type_traits>
