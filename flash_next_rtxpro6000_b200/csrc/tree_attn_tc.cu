@@ -423,6 +423,8 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
         if (lane == 0) mbar_arrive(bar(s.qfull[rt]));
       }
       float ref = -INFINITY, sum = 0.f;
+      // held by each thread: the other row tile's warps may be segments ahead of these, or behind
+      unsigned long long odd = 0ull;
       const int len = sg.rq.ctx + sg.rq.nodes;
       for (int t = sg.t0; t < sg.t1; ++t, ++n) {
         const int pos0 = t * kTile;
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
               atomicOr(odds, 1ull << (pos0 + j - sg.rq.ctx));
           }
           ok = ok && join(who);
-          const unsigned long long odd = *reinterpret_cast<volatile unsigned long long*>(odds);
+          odd = *reinterpret_cast<volatile unsigned long long*>(odds);  // this tile's and those before
           if (odd) {
             for (int u = rt * 128 + row; u < kTile * kBlocks * 8; u += threads) {
               const int d = pos0 + (u >> 3) % kTile - sg.rq.ctx;
@@ -529,8 +531,6 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
       fence_after();
       if (busy) {
         const uint32_t oa = tm + lanes + rt * D;
-        unsigned long long odd = sg.t1 * kTile > sg.rq.ctx ? *reinterpret_cast<volatile unsigned long long*>(odds) : 0ull;
-
         while (odd) {  // rare: values that are not finite, for the rows that see them
           const int d = __ffsll((long long)odd) - 1;
           odd &= odd - 1;

@@ -25,7 +25,8 @@ def sample_tokens(
     min_p: Optional[torch.Tensor] = None,
     pdl: Optional[bool] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(tokens int64 [M], probs fp32 [M]) of logits [M, V] (fp32, bf16 or fp16, rows contiguous).
+    """(tokens int64 [M], probs fp32 [M]) of logits [M, V] (fp32, bf16 or fp16, rows contiguous, V at
+    most 2^21).
 
     uniforms fp32 [M] in [0, 1); temperature, top_p, min_p fp32 [M], top_k int32 [M], each None for
     off.  In the order of falling logits (lower token first on ties) top-k keeps ``top_k`` tokens,

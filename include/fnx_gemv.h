@@ -517,7 +517,8 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
                        fnx_stream_t stream);
 
 /*
- * Sampling: tokens[m] drawn from row m of logits (fp32, bf16 or fp16, row stride ldl) by
+ * Sampling: tokens[m] drawn from row m of logits (fp32, bf16 or fp16, row stride ldl, V at most
+ * 2^21) by
  * uniforms[m] in [0, 1), and its probability among the tokens kept.  In the order of falling
  * logits (lower token first on ties) top-k keeps top_k tokens, top-p the shortest prefix whose
  * probability reaches top_p of those, min-p the tokens with at least min_p of the largest

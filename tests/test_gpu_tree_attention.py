@@ -438,3 +438,25 @@ def test_batches_with_rising_scores(D, Hq, T):
         sign = 1 if b % 2 else -1
         c.k.view(-1, 1, D)[slots, 0, 0] = (sign * pos.float() * 0.02 * D**0.5).bfloat16()
     c.check()
+
+
+def test_batches_not_finite_with_uneven_row_tiles():
+    """Requests whose rows fill both row tiles next to ones that fill one, a segment each, all with a
+    drafted token that is not finite: no segment takes another's for its own."""
+    counts = [64, 3, 40, 64, 1, 33, 64, 9] * 6
+    lens = [700 + 13 * b for b in range(len(counts))]
+    c = Case(lens, counts, 8, 2, 128, 16, torch.bfloat16, seed=21)
+    for b, (ctx, t) in enumerate(zip(lens, counts)):
+        j = (t - 1) // 2
+        slot = int(c.table[b][(ctx + j) // 16]) * 16 + (ctx + j) % 16
+        c.v.view(-1, 2, 128)[slot, b % 2, b] = float("nan")
+    out, _ = c.run()
+    n = 0
+    for b, t in enumerate(counts):
+        j = (t - 1) // 2
+        sees = torch.tensor([bool(c.masks[n + i] >> j & 1) for i in range(t)], device=dev())
+        got = out[n:n + t].view(t, 2, 4, 128).isnan()
+        want = torch.zeros_like(got)
+        want[:, b % 2, :, b] = sees[:, None]
+        assert torch.equal(got, want), b
+        n += t
