@@ -5,7 +5,8 @@
 // over the keys j < L of the request's context and the drafted tokens L + n whose bit n is set in node
 // i's mask; lse_i = log sum_j exp(scale q_i k_j).  A row that sees nothing gives 0 and -inf.  One pass
 // over the keys with a running maximum and sum; scores, weights' sums and outputs are held in fp32,
-// the weights are rounded to the cache's type for the second product (as wide as its other operand).
+// the weights are rounded to the cache's type for the second product (as wide as its other operand; fp16
+// weights relative to a reference that keeps them in its range, tree_attn.cuh).
 //
 // Bound: the cache's bytes, each read once for all G query heads and all nodes that share a kv head:
 // the G * T rows of a kv head are one matrix operand.  mma.sync.m16n8k16 with keys and values in
@@ -169,7 +170,9 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn_kernel(const __grid
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    constexpr float kHead = kNarrow<T> ? 15.f : 0.f, kFall = 22.f;
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // reference, sum of weights
+    float peak[2] = {-INFINITY, -INFINITY};                      // the highest reference so far
     const int g = lane >> 2, q2 = (lane & 3) * 2;
 
     for (int t = t0; t < t1; ++t) {
@@ -236,11 +239,16 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn_kernel(const __grid
       float rescale[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float mx = top[h];
+        float mx = kNarrow<T> ? -INFINITY : top[h];
 #pragma unroll
         for (int i = 0; i < kKeys / 8; ++i) mx = fmaxf(mx, fmaxf(sc[i][2 * h], sc[i][2 * h + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (kNarrow<T>) {
+          const float at = mx - kHead;
+          peak[h] = fmaxf(peak[h], at);
+          mx = at < top[h] - kFall && at > -INFINITY ? fmaxf(at, peak[h] - kSpan) : fmaxf(at, top[h]);
+        }
         const float ref = mx == -INFINITY ? 0.f : mx;
         rescale[h] = exp2_fast(top[h] - ref);
         top[h] = mx;

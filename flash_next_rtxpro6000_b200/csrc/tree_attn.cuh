@@ -120,6 +120,18 @@ __device__ __forceinline__ void attn_place(const AttnArgs& a, int b, int pos, in
   v = (int64_t)page * a.vc_st[0] + (int64_t)in * a.vc_st[1] + (int64_t)head * a.vc_st[2];
 }
 
+// Weights are exp2(score - reference) of a row's own reference, which the row's sums and partial results
+// carry along.  They are rounded to the cache's type for the second product.  bf16 has the exponents of
+// fp32: the reference is the running maximum, and nothing is lost.  fp16 ends at 2^-24, and weights below
+// that would count in the sum but not in the result, all of which may be theirs where the large weights'
+// values are small (the first token's often are).  So with fp16 the reference lies some bits (the form's
+// "head") below the running maximum, which uses fp16's range above 1, and where a key tile's largest score
+// is more than kFall bits below the reference's, the reference follows it down, to kSpan bits below the
+// running maximum at most (sums then stay below 2^102).  A tile's largest weight is 2^-7 at least.
+template <typename T> constexpr bool kNarrow = false;  // few exponents
+template <> constexpr bool kNarrow<__half> = true;
+constexpr float kSpan = 40.0f;
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -15,8 +15,8 @@
 // Roles: 4 softmax warps a row tile (a thread has a row: its scores come from tensor memory in one
 // piece, so the row's maximum and sum need no shuffles), 4 warps that load keys and 4 that load values
 // (cp.async, any page size), one warp that issues the first product and one the second.  O is rescaled
-// only when a row's maximum has risen by more than 2^8: until then weights may be larger than one, which
-// costs nothing in floating point.  Every wait is bounded and records an error code; roles then fall
+// only when a row's maximum has risen by more than 2^8 (or, with fp16, fallen far: tree_attn.cuh): until
+// then weights may be larger than one, which costs nothing in floating point.  Every wait is bounded and records an error code; roles then fall
 // through to the end.
 //
 // Measured (B200): 24 ragged requests, D = 128 fp16, 357 MB: 103 us, 3.4 TB/s; 4 requests of 64 nodes
@@ -35,7 +35,8 @@ namespace {
 
 constexpr int kTile = kKeyTile;
 constexpr int kBlockBytes = kTile * 128;  // 64 rows of a 64-element block
-constexpr float kRise = 8.0f;
+constexpr float kRise = 8.0f, kFall = 14.0f;
+template <typename T> constexpr float kHead = kNarrow<T> ? 7.0f : 0.0f;  // weights are at most 2^(kHead + kRise)
 
 template <int D, int RT>
 struct TcAttn {
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(s.qfull[rt]));
       }
-      float ref = -INFINITY, sum = 0.f;
+      float ref = -INFINITY, sum = 0.f, peak = -INFINITY;  // reference, weights' sum, highest reference so far
       // held by each thread: the other row tile's warps may be segments ahead of these, or behind
       unsigned long long odd = 0ull;
       const int len = sg.rq.ctx + sg.rq.nodes;
@@ -479,18 +480,26 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int j = 0; j < kTile; ++j) m4[j & 3] = fmaxf(m4[j & 3], x[j]);
-          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c2;
-          const bool rise = mx > ref + kRise || (ref == -INFINITY && mx > ref);
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c2 - kHead<T>;
+          bool move = mx > ref + kRise || (ref == -INFINITY && mx > ref);
+          float next = mx;
+          if (kNarrow<T>) {
+            peak = fmaxf(peak, mx);
+            if (mx < ref - kFall && mx > -INFINITY) {
+              next = fmaxf(mx, peak - kSpan);
+              move = next < ref;
+            }
+          }
           if (t == sg.t0) {
             ref = mx;
-          } else if (__any_sync(0xffffffffu, rise)) {
+          } else if (__any_sync(0xffffffffu, move)) {
             if (!o_is_done()) {
               if (lane == 0) record_error(a.err, ERR_WAIT_RED);
               ok = false;
               break;
             }
             fence_after();
-            const float to = rise ? mx : ref;
+            const float to = move ? next : ref;
             const float f = to == ref ? 1.f : exp2_fast(ref - to);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {

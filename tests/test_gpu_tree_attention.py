@@ -460,3 +460,71 @@ def test_batches_not_finite_with_uneven_row_tiles():
         want[:, b % 2, :, b] = sees[:, None]
         assert torch.equal(got, want), b
         n += t
+
+
+def _sinks(D, Hq, T, n, B, gap, seed):
+    """B requests over n keys: every score is a unit normal's but one key's a request, which lies `gap` above and
+    has value 0; the others' values lie between 500 and 1,500."""
+    c = Case([n] * B, [T] * B, Hq, 1, D, 64, torch.float16, seed=seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    c.q.zero_()
+    c.q[..., 0] = D**0.5  # the score is the key's first element
+    pos = torch.arange(n + T, device=dev())
+    slots = c.table.long()[:, pos // 64] * 64 + pos % 64
+    c.v.view(-1, D)[slots] = (500 + 1000 * torch.rand(B, n + T, D, generator=g)).half().to(dev())
+    c.k.view(-1, D)[slots, 0] = torch.randn(B, n + T, generator=g).half().to(dev())
+    c.k.view(-1, D)[slots[:, n // 3], 0] = gap
+    c.v.view(-1, D)[slots[:, n // 3]] = 0
+    return c, slots
+
+
+def _whole(c, slots, n, T):
+    """(out, weighted mean of |v|) of all rows in 64 bits, for one kv head."""
+    N, Hq, D = c.q.shape
+    outs, means = [], []
+    for b in range(N // T):
+        keys, vals = c.k.view(-1, D)[slots[b]].double(), c.v.view(-1, D)[slots[b]].double()
+        see = torch.tensor([[True] * n + [bool(m >> j & 1) for j in range(T)] for m in c.masks[b * T:b * T + T]],
+                           device=dev())
+        s = (c.q[b * T:b * T + T].double() @ keys.T * D**-0.5).masked_fill(~see[:, None], -float("inf"))
+        w = torch.softmax(s, -1)
+        outs.append(w @ vals)
+        means.append(w @ vals.abs())
+    return torch.cat(outs), torch.cat(means)
+
+
+SINKS = [(64, 1, 1, 70000, 1), (64, 4, 1, 500, 100), (128, 4, 8, 500, 100), (256, 2, 5, 500, 100),
+         (64, 8, 8, 250, 100), (256, 8, 8, 250, 100),                           # mma.sync, 16 to 64 rows
+         (64, 8, 8, 131072, 1), (64, 8, 5, 6000, 20), (64, 8, 32, 3000, 60), (128, 16, 2, 6000, 20),
+         (128, 8, 40, 3000, 60), (256, 8, 9, 6000, 20), (256, 8, 20, 3000, 40)]  # tensor memory
+
+
+@pytest.mark.parametrize("gap", [10.0, 18.0, 20.0, 24.0])
+@pytest.mark.parametrize("D,Hq,T,n,B", SINKS)
+def test_fp16_weights_far_below_the_largest(D, Hq, T, n, B, gap):
+    """Many small weights under one large one whose value is 0: what the row gives is all theirs.
+
+    A weight's rounding is 2^-11 of it, or 2^-25 where fp16 has no smaller step.  A key tile's largest
+    weight is at least 2^-7 (the row's reference follows the tiles down), so the second kind costs a tile
+    of 64 at most 64 * 2^-25 / 2^-7 = 2^-12 of its weight times the largest |v|, three times the mean here;
+    in the large weight's own tile, where that one is at least 2^7, 64 * 2^-32 of the largest |v|."""
+    c, slots = _sinks(D, Hq, T, n, B, gap, seed=D + T)
+    out, _ = c.run()
+    want, mean = _whole(c, slots, n, T)
+    u = UNIT[torch.float16]
+    tol = (u + 2.0**-12 + 3 * 2.0**-12) * mean + u * want.abs() + 64 * 2.0**-32 * 1500 + 2.0**-25
+    err = (out.double() - want).abs()
+    assert bool((err <= tol).all()), (float((err / want.abs()).max()), float((err - tol).max()))
+    _fx().check_device_errors()
+
+
+@pytest.mark.parametrize("D,Hq,T,n,B", SINKS)
+def test_fp16_infinite_value_under_a_small_weight(D, Hq, T, n, B):
+    """An infinite value that a row sees makes the row infinite, however small its weight (that of a key
+    at its tile's average: within 2^7 of the tile's largest)."""
+    c, slots = _sinks(D, Hq, T, n, B, 24.0, seed=D + T)
+    c.k.view(-1, D)[slots[:, n - 70], 0] = 0.0
+    c.v.view(-1, D)[slots[:, n - 70], 5] = float("inf")
+    out, _ = c.run()
+    assert bool((out[..., 5] == float("inf")).all())
+    assert bool(out[..., 6:].isfinite().all()) and bool(out[..., :5].isfinite().all())
