@@ -66,7 +66,7 @@ def tree_attention(
     ``max_context`` bounds context_lens (default: what the page table holds).  Lengths are read on the
     device, so a captured call follows them; lengths beyond the bounds and pages outside the cache are
     reported by ``check_device_errors``."""
-    flag, partials = _scratch(q)
+    flag, partials, _ = _scratch(q)
     return _lib.ops().tree_attention(q, k_cache, v_cache, page_table, context_lens, node_offsets, tree_mask,
                                      max_nodes, max_context, scale, out, lse, partials, flag,
                                      PDL if pdl is None else pdl)

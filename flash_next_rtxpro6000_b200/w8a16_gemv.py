@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import logging
 import os
+import threading
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
@@ -35,6 +36,7 @@ _SLOT = 0
 _WS: dict = {}
 _ONES: dict = {}
 _ADDRESSES: dict = {}
+_WS_LOCK = threading.RLock()
 
 
 def _env_flag(name: str, default: str = "0") -> bool:
@@ -112,8 +114,10 @@ def _workspace_slot(device, slot: int) -> Workspace:
     key = (_norm_device(device), slot)
     ws = _WS.get(key)
     if ws is None:
-        ws = Workspace(key[0])
-        _WS[key] = ws
+        with _WS_LOCK:  # one workspace a slot, whoever comes first
+            ws = _WS.get(key)
+            if ws is None:
+                ws = _WS[key] = Workspace(key[0])
     return ws
 
 
@@ -121,21 +125,25 @@ def _workspace(device) -> Workspace:
     return _workspace_slot(device, _SLOT)
 
 
-def _addresses(index: int, slot: int) -> Tuple[int, int]:
+def _addresses(index: int, slot: int) -> tuple:
     ws = _workspace_slot(torch.device("cuda", index), slot)
-    n = ctypes.c_int64()
-    _lib.check(_lib.lib().fnx_tree_attention_workspace_floats(ctypes.byref(n)), "scratch")
-    ws.attention = torch.empty(n.value, dtype=torch.float32, device=ws.device)
-    got = _ADDRESSES[(index, slot)] = (ptr(ws.error_flag), ptr(ws.attention))
+    with _WS_LOCK:  # an address is published once, and its tensor is never replaced
+        got = _ADDRESSES.get((index, slot))
+        if got is None:
+            n = ctypes.c_int64()
+            _lib.check(_lib.lib().fnx_tree_attention_workspace_floats(ctypes.byref(n)), "scratch")
+            ws.attention = torch.empty(n.value, dtype=torch.float32, device=ws.device)
+            got = _ADDRESSES[(index, slot)] = (ptr(ws.error_flag), ptr(ws.attention), ws)
     return got
 
 
-def _scratch(t: torch.Tensor) -> Tuple[int, int]:
+def _scratch(t: torch.Tensor) -> tuple:
     """(error flag, attention scratch) addresses of the current slot on t's device, for the native
-    binding of the verify-step operators; (0, 0) for a tensor on the host, which it refuses."""
+    binding of the verify-step operators, and the workspace that owns them; (0, 0, None) for a tensor
+    on the host, which it refuses."""
     got = _ADDRESSES.get((t.get_device(), _SLOT))
     if got is None:
-        return _addresses(t.get_device(), _SLOT) if t.is_cuda else (0, 0)
+        return _addresses(t.get_device(), _SLOT) if t.is_cuda else (0, 0, None)
     return got
 
 
