@@ -131,7 +131,8 @@ def _addresses(index: int, slot: int) -> tuple:
         got = _ADDRESSES.get((index, slot))
         if got is None:
             n = ctypes.c_int64()
-            _lib.check(_lib.lib().fnx_tree_attention_workspace_floats(ctypes.byref(n)), "scratch")
+            with torch.cuda.device(index):  # the size follows from the SMs of the current device
+                _lib.check(_lib.lib().fnx_tree_attention_workspace_floats(ctypes.byref(n)), "scratch")
             ws.attention = torch.empty(n.value, dtype=torch.float32, device=ws.device)
             got = _ADDRESSES[(index, slot)] = (ptr(ws.error_flag), ptr(ws.attention), ws)
     return got

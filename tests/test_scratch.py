@@ -50,8 +50,21 @@ def slots(monkeypatch):
     monkeypatch.setattr(w8a16_gemv, "Workspace", FakeWorkspace)
     for name in ("_WS", "_ADDRESSES"):
         monkeypatch.setattr(w8a16_gemv, name, {})
+    monkeypatch.setattr(w8a16_gemv, "_ONES", {torch.device("cuda", i): None for i in range(2)})
     fake = FakeLib()
     monkeypatch.setattr(_lib, "_lib", fake)
+
+    class Device:  # torch.cuda.device
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, fake.current = fake.current, self.index
+
+        def __exit__(self, *exc):
+            fake.current = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
     return fake
 
 
@@ -70,3 +83,12 @@ def test_first_calls_of_many_threads_share_one_live_scratch(slots):
     (ws,) = w8a16_gemv._WS.values()
     live = (ws.error_flag.data_ptr(), ws.attention.data_ptr())
     assert set(got) == {live} and tuple(w8a16_gemv._scratch(On())[:2]) == live
+
+
+def test_the_scratch_is_sized_for_its_own_device(slots):
+    w8a16_gemv.prealloc("cuda:1")  # while device 0 is current
+    assert slots.current == 0
+    for slot in (0, 1):
+        assert w8a16_gemv._WS[(torch.device("cuda", 1), slot)].attention.numel() == slots.floats[1]
+    w8a16_gemv._scratch(On(0))
+    assert w8a16_gemv._WS[(torch.device("cuda", 0), 0)].attention.numel() == slots.floats[0]
