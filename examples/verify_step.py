@@ -57,7 +57,7 @@ class VerifyStep:
         self.temperature = torch.full((nodes,), temperature, device=device)
         self.top_k = torch.full((nodes,), top_k, **i32)
         self.top_p = torch.full((nodes,), top_p, device=device)
-        fx.prealloc(device)
+        fx.prealloc(device, attention=True)
 
     def run(self):
         mask, positions, self.slots = fx.tree_layout(self.parents, self.offsets, self.context, self.page_table,

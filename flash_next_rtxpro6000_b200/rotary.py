@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .w8a16_gemv import PDL, _scratch
+from .w8a16_gemv import PDL, _flag
 
 
 @dataclass(frozen=True)
@@ -95,4 +95,4 @@ def rotary_append(
     tokens may have the same slot.  Positions outside the table and slots outside the cache are
     reported by ``check_device_errors``."""
     return _lib.ops().rotary_append(q, k, v, positions, slots, table, k_cache, v_cache, interleaved, out,
-                                    _scratch(q)[0], PDL if pdl is None else pdl)
+                                    _flag(q), PDL if pdl is None else pdl)

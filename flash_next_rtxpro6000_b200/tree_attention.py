@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .w8a16_gemv import PDL, _scratch
+from .w8a16_gemv import PDL, _flag, _scratch
 
 MAX_NODES = 64
 
@@ -36,7 +36,7 @@ def tree_layout(
     position is the context length plus its depth, its slot that of the context's length plus its
     index."""
     return _lib.ops().tree_layout(parents, node_offsets, context_lens, page_table, page_size, num_pages,
-                                  _scratch(parents)[0], PDL if pdl is None else pdl)
+                                  _flag(parents), PDL if pdl is None else pdl)
 
 
 def tree_attention(

@@ -35,6 +35,7 @@ _N_SLOTS = 2
 _SLOT = 0
 _WS: dict = {}
 _ONES: dict = {}
+_FLAGS: dict = {}
 _ADDRESSES: dict = {}
 _WS_LOCK = threading.RLock()
 
@@ -140,21 +141,35 @@ def _addresses(index: int, slot: int) -> tuple:
 
 def _scratch(t: torch.Tensor) -> tuple:
     """(error flag, attention scratch) addresses of the current slot on t's device, for the native
-    binding of the verify-step operators, and the workspace that owns them; (0, 0, None) for a tensor
-    on the host, which it refuses."""
+    binding of the attention, and the workspace that owns them; (0, 0, None) for a tensor on the
+    host, which it refuses."""
     got = _ADDRESSES.get((t.get_device(), _SLOT))
     if got is None:
         return _addresses(t.get_device(), _SLOT) if t.is_cuda else (0, 0, None)
     return got
 
 
-def prealloc(device) -> None:
+def _flag(t: torch.Tensor) -> int:
+    """The address of the current slot's error flag on t's device, for the native binding of the
+    operators that need no scratch; 0 for a tensor on the host, which it refuses."""
+    key = (t.get_device(), _SLOT)
+    got = _FLAGS.get(key)
+    if got is None:
+        if not t.is_cuda:
+            return 0
+        ws = _workspace_slot(torch.device("cuda", key[0]), key[1])
+        got = _FLAGS[key] = (ptr(ws.error_flag), ws)
+    return got[0]
+
+
+def prealloc(device, attention: bool = False) -> None:
     """Materialise every slot's scratch before any CUDA graph is captured
-    (w8a16_gemv.py:383-395)."""
+    (w8a16_gemv.py:383-395); with ``attention`` also that of ``tree_attention`` (some 40 MB a
+    slot), which its first call makes otherwise."""
     d = _norm_device(device)
     for slot in range(_N_SLOTS):
         _workspace_slot(device, slot)
-        if d.type == "cuda" and (d.index, slot) not in _ADDRESSES:
+        if attention and d.type == "cuda":
             _addresses(d.index, slot)
     if d not in _ONES:
         _ONES[d] = torch.ones(1, dtype=torch.float32, device=d)

@@ -48,7 +48,7 @@ class On:
 @pytest.fixture
 def slots(monkeypatch):
     monkeypatch.setattr(w8a16_gemv, "Workspace", FakeWorkspace)
-    for name in ("_WS", "_ADDRESSES"):
+    for name in ("_WS", "_ADDRESSES", "_FLAGS"):
         monkeypatch.setattr(w8a16_gemv, name, {})
     monkeypatch.setattr(w8a16_gemv, "_ONES", {torch.device("cuda", i): None for i in range(2)})
     fake = FakeLib()
@@ -86,9 +86,20 @@ def test_first_calls_of_many_threads_share_one_live_scratch(slots):
 
 
 def test_the_scratch_is_sized_for_its_own_device(slots):
-    w8a16_gemv.prealloc("cuda:1")  # while device 0 is current
+    w8a16_gemv.prealloc("cuda:1", attention=True)  # while device 0 is current
     assert slots.current == 0
     for slot in (0, 1):
         assert w8a16_gemv._WS[(torch.device("cuda", 1), slot)].attention.numel() == slots.floats[1]
     w8a16_gemv._scratch(On(0))
     assert w8a16_gemv._WS[(torch.device("cuda", 0), 0)].attention.numel() == slots.floats[0]
+
+
+def test_only_the_attention_makes_its_scratch(slots):
+    w8a16_gemv.prealloc("cuda:0")
+    flag = w8a16_gemv._flag(On())
+    (ws, other) = w8a16_gemv._WS.values()
+    assert flag == ws.error_flag.data_ptr() and ws.attention is None and other.attention is None
+    assert w8a16_gemv._scratch(On())[:2] == (flag, ws.attention.data_ptr())
+    assert other.attention is None
+    w8a16_gemv.prealloc("cuda:0", attention=True)
+    assert other.attention is not None and w8a16_gemv._scratch(On())[1] == ws.attention.data_ptr()
