@@ -595,8 +595,9 @@ __global__ void __launch_bounds__(128) tree_layout_kernel(const __grid_constant_
       if (a.node_offsets[mid] <= n) lo = mid;
       else hi = mid;
     }
-    const int n0 = a.node_offsets[lo], i = n - n0;
-    if (i < 0 || i >= 64 || n >= a.node_offsets[lo + 1]) {
+    const int n0 = a.node_offsets[lo], n1 = a.node_offsets[lo + 1], i = n - n0;
+    // the attention's test of a request: its nodes are rows of the arrays, 64 at most
+    if (n0 < 0 || i < 0 || n >= n1 || n1 > a.N || n1 - n0 > 64) {
       record_error(a.err, ERR_LENGTHS);
       if (a.mask) a.mask[n] = 0ull;
       if (a.positions) a.positions[n] = 0;

@@ -481,7 +481,8 @@ int fnx_rotary_append(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
  * int64 [nodes]; each may be NULL (page_table too, when slots is).  At most 64 nodes a
  * request.  A parent that is not an earlier node records FNX_DEVERR_TREE and counts as -1;
  * lengths beyond the table record FNX_DEVERR_LENGTHS, pages outside [0, num_pages)
- * FNX_DEVERR_PAGE, with slot -1.
+ * FNX_DEVERR_PAGE, with slot -1.  A request whose offsets are not 0 <= first <= last <= nodes, or that
+ * has more than 64, records FNX_DEVERR_LENGTHS; its nodes get mask 0, position 0 and slot -1.
  */
 int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
                     const int32_t* context_lens, const int32_t* page_table, int64_t table_ld,

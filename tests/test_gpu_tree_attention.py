@@ -528,3 +528,41 @@ def test_fp16_infinite_value_under_a_small_weight(D, Hq, T, n, B):
     out, _ = c.run()
     assert bool((out[..., 5] == float("inf")).all())
     assert bool(out[..., 6:].isfinite().all()) and bool(out[..., :5].isfinite().all())
+
+
+@pytest.mark.parametrize("offsets,bad", [
+    ([-3, 2, 6, 8], [0, 1]), ([-70, 2, 6, 8], [0, 1]), ([0, 2, 6, 9], [6, 7]), ([0, 2, 6, 2**31 - 1], [6, 7]),
+    ([-2**31, 2, 6, 8], [0, 1]),
+])
+def test_tree_layout_of_requests_outside_the_arrays(offsets, bad):
+    """Offsets below 0 or past the rows are reported and not followed: the request's rows see nothing and are
+    stored nowhere, the others' are as ever."""
+    fx = _fx()
+    i32 = dict(dtype=torch.int32, device=dev())
+    parents = torch.tensor([-1, 0, -1, 0, 0, 2, -1, 0], **i32)
+    ctx, table = torch.tensor([5, 20, 0], **i32), torch.arange(9, **i32).view(3, 3)
+    whole = fx.tree_layout(parents, torch.tensor([0, 2, 6, 8], **i32), ctx, table, 16, 9)
+    fx.check_device_errors()
+    got = fx.tree_layout(parents, torch.tensor(offsets, **i32), ctx, table, 16, 9)
+    with pytest.raises(fx.DeviceWaitError) as e:
+        fx.check_device_errors()
+    assert [c for _, c in e.value.codes] == [14]
+    for x, want, none in zip(got, whole, (0, 0, -1)):
+        want = want.clone()
+        want[bad] = none
+        assert torch.equal(x, want)
+
+
+def test_tree_layout_of_a_request_with_too_many_nodes():
+    fx = _fx()
+    i32 = dict(dtype=torch.int32, device=dev())
+    parents = torch.arange(-1, 69, **i32)
+    parents[65] = -1
+    parents[66:] = 0
+    mask, pos, slots = fx.tree_layout(parents, torch.tensor([0, 65, 70], **i32), torch.tensor([3, 7], **i32),
+                                      torch.arange(12, **i32).view(2, 6), 16, 12)
+    with pytest.raises(fx.DeviceWaitError) as e:
+        fx.check_device_errors()
+    assert [c for _, c in e.value.codes] == [14]
+    assert bool((mask[:65] == 0).all()) and bool((pos[:65] == 0).all()) and bool((slots[:65] == -1).all())
+    assert mask[65:].tolist() == [1, 3, 5, 9, 17] and slots[65:].tolist() == [96 + 7 + j for j in range(5)]
