@@ -1451,6 +1451,8 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
   a.pdl = pdl;
   for (int b0 = 0; b0 < batch; b0 += fnx::kAttnMaxBatch) {  // requests of one launch
     a.B = std::min(batch - b0, fnx::kAttnMaxBatch);
+    a.head = b0 == 0;
+    a.tail = b0 + a.B == batch;
     a.page_table = page_table + (int64_t)b0 * table_ld;
     a.context_lens = context_lens + b0;
     a.node_offsets = node_offsets + b0;

@@ -635,6 +635,7 @@ struct AttnArgs {
   int64_t table_ld, num_pages;
   int table_width, page_size;
   int B, N, Hq, Hk, group, D, max_nodes, max_context;
+  int head, tail;  // whether the launch has the call's first and last request
   float scale;
   int f16;
   float* partials;

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn_kernel(const __grid
   const T* vc = reinterpret_cast<const T*>(a.v_cache);
   const float c2 = a.scale * 1.4426950408889634f;  // scores in base-2 units
   pdl_wait();
-  attn_prefix(a, kRows, s.before, s.scratch, blockIdx.x == 0);
+  attn_unowned(a, attn_prefix(a, kRows, s.before, s.scratch, blockIdx.x == 0));
   const long long total = s.before[a.B];
   const long long G = total < (long long)gridDim.x ? total : (long long)gridDim.x;
   pdl_trigger();  // the launch that joins the partials may get ready
@@ -595,14 +595,17 @@ __global__ void __launch_bounds__(128) tree_layout_kernel(const __grid_constant_
       if (a.node_offsets[mid] <= n) lo = mid;
       else hi = mid;
     }
-    const int n0 = a.node_offsets[lo], n1 = a.node_offsets[lo + 1], i = n - n0;
-    // the attention's test of a request: its nodes are rows of the arrays, 64 at most
-    if (n0 < 0 || i < 0 || n >= n1 || n1 > a.N || n1 - n0 > 64) {
-      record_error(a.err, ERR_LENGTHS);
+    const int n0 = a.node_offsets[lo], n1 = a.node_offsets[lo + 1];
+    // Nodes of no request, ahead of the first and behind the last, see nothing.  Then the attention's test of a
+    // request: its nodes are rows of the arrays, 64 at most.
+    const bool none = n < n0 || n >= n1;
+    if (none || n0 < 0 || n1 > a.N || n1 - n0 > 64) {
+      if (!none) record_error(a.err, ERR_LENGTHS);
       if (a.mask) a.mask[n] = 0ull;
       if (a.positions) a.positions[n] = 0;
       if (a.slots) a.slots[n] = -1;
     } else {
+      const int i = n - n0;
       unsigned long long seen = 1ull << i;
       int depth = 0;
       for (int at = i;;) {

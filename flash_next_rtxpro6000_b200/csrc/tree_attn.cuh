@@ -21,6 +21,7 @@ constexpr int kAttnMaxGrid = 256;   // CTAs of one launch (one per SM)
 
 struct AttnReq {
   int ctx, nodes, n0;  // context length, drafted nodes, first row in q
+  bool refused;
 };
 
 // Request b's lengths; anything inconsistent is recorded and leaves the request without nodes.
@@ -30,8 +31,9 @@ __device__ __forceinline__ AttnReq attn_request(const AttnArgs& a, int b, bool r
   r.n0 = a.node_offsets[b];
   r.nodes = a.node_offsets[b + 1] - r.n0;
   const int64_t room = (int64_t)a.table_width * a.page_size;
-  if (r.ctx < 0 || r.ctx > a.max_context || r.n0 < 0 || r.nodes < 0 || r.nodes > a.max_nodes ||
-      r.n0 > a.N - r.nodes || (int64_t)r.ctx + r.nodes > room) {
+  r.refused = r.ctx < 0 || r.ctx > a.max_context || r.n0 < 0 || r.nodes < 0 || r.nodes > a.max_nodes ||
+              r.n0 > a.N - r.nodes || (int64_t)r.ctx + r.nodes > room;
+  if (r.refused) {
     if (report) record_error(a.err, ERR_LENGTHS);
     r.ctx = r.nodes = r.n0 = 0;
   }
@@ -51,15 +53,21 @@ __device__ __forceinline__ AttnShape attn_shape(const AttnArgs& a, const AttnReq
   return s;
 }
 
-// Fills before[b] = units of the requests ahead of b, before[B] = all units.  All threads of the
-// block take part; `scratch` holds one value per warp.
-__device__ __forceinline__ void attn_prefix(const AttnArgs& a, int rows, long long* before, long long* scratch,
+// Fills before[b] = units of the requests ahead of b, before[B] = all units; returns whether a request was
+// refused.  All threads of the block take part; `scratch` holds one value per warp.
+__device__ __forceinline__ bool attn_prefix(const AttnArgs& a, int rows, long long* before, long long* scratch,
                                             bool report) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   long long base = 0;
+  bool refused = false;
   for (int b0 = 0; b0 < a.B; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
-    const long long u = b < a.B ? attn_shape(a, attn_request(a, b, report), rows).units : 0;
+    long long u = 0;
+    if (b < a.B) {
+      const AttnReq r = attn_request(a, b, report);
+      refused |= r.refused;
+      u = attn_shape(a, r, rows).units;
+    }
     long long v = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -77,7 +85,27 @@ __device__ __forceinline__ void attn_prefix(const AttnArgs& a, int rows, long lo
     __syncthreads();
   }
   if (threadIdx.x == 0) before[a.B] = base;
-  __syncthreads();
+  return __syncthreads_or(refused);
+}
+
+// Rows of q that no request has get 0 and -inf, as rows that see nothing do: those of refused requests, and
+// those ahead of the first and behind the last (a captured call's, when it is replayed with fewer nodes).
+__device__ __forceinline__ void attn_unowned(const AttnArgs& a, bool refused) {
+  const int* off = a.node_offsets;
+  if (!refused && !(a.head && off[0] > 0) && !(a.tail && off[a.B] < a.N)) return;
+  for (int b = a.head ? -1 : 0; b < a.B + (a.tail ? 1 : 0); ++b) {
+    if (b >= 0 && b < a.B && !attn_request(a, b, false).refused) continue;
+    const int n0 = b < 0 ? 0 : max(off[b], 0), n1 = b == a.B ? a.N : min(off[b + 1], a.N);
+    const int units = a.D / 8;
+    const int64_t all = ((int64_t)n1 - n0) * a.Hq * units, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < all; u += step) {
+      const int64_t row = u / units, n = n0 + row / a.Hq;
+      const int h = (int)(row % a.Hq), c = (int)(u % units);
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + n * a.o_sn + (int64_t)h * a.o_sh + c * 8) =
+          make_uint4(0u, 0u, 0u, 0u);
+      if (a.lse && c == 0) a.lse[n * a.Hq + h] = -INFINITY;
+    }
+  }
 }
 
 // The request that holds unit w: the last one with before[b] <= w (those without units are passed).

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn_tc_kernel(con
   typename Cfg::Smem& s = *reinterpret_cast<typename Cfg::Smem*>(base);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
-  attn_prefix(a, kRows, s.before, reinterpret_cast<long long*>(s.q), blockIdx.x == 0);
+  attn_unowned(a, attn_prefix(a, kRows, s.before, reinterpret_cast<long long*>(s.q), blockIdx.x == 0));
   const long long total = s.before[a.B];
   const long long G = total < (long long)gridDim.x ? total : (long long)gridDim.x;
   pdl_trigger();  // the launch that joins the partials may get ready

@@ -34,7 +34,8 @@ def tree_layout(
     a root; node_offsets int32 [batch + 1]; context_lens int32 [batch]; page_table int32 [batch,
     pages].  Bit j of a node's mask is set where it sees node j: itself and its ancestors.  Its
     position is the context length plus its depth, its slot that of the context's length plus its
-    index."""
+    index.  Nodes of no request (ahead of node_offsets[0], from node_offsets[batch] on) get mask 0,
+    position 0 and slot -1, so a captured step may be replayed with fewer nodes."""
     return _lib.ops().tree_layout(parents, node_offsets, context_lens, page_table, page_size, num_pages,
                                   _flag(parents), PDL if pdl is None else pdl)
 
@@ -65,7 +66,8 @@ def tree_attention(
     sum of exp(scale q k) (scale: dim ** -0.5 unless given, positive); a row that sees nothing gives 0 and -inf.
     ``max_context`` bounds context_lens (default: what the page table holds).  Lengths are read on the
     device, so a captured call follows them; lengths beyond the bounds and pages outside the cache are
-    reported by ``check_device_errors``."""
+    reported by ``check_device_errors``.  Rows of no request, and those of one with lengths beyond the
+    bounds, give 0 and -inf."""
     flag, partials, _ = _scratch(q)
     return _lib.ops().tree_attention(q, k_cache, v_cache, page_table, context_lens, node_offsets, tree_mask,
                                      max_nodes, max_context, scale, out, lse, partials, flag,

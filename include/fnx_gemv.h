@@ -482,7 +482,8 @@ int fnx_rotary_append(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
  * request.  A parent that is not an earlier node records FNX_DEVERR_TREE and counts as -1;
  * lengths beyond the table record FNX_DEVERR_LENGTHS, pages outside [0, num_pages)
  * FNX_DEVERR_PAGE, with slot -1.  A request whose offsets are not 0 <= first <= last <= nodes, or that
- * has more than 64, records FNX_DEVERR_LENGTHS; its nodes get mask 0, position 0 and slot -1.
+ * has more than 64, records FNX_DEVERR_LENGTHS; its nodes get mask 0, position 0 and slot -1, as
+ * do nodes ahead of node_offsets[0] and from node_offsets[batch] on, which is no error.
  */
 int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
                     const int32_t* context_lens, const int32_t* page_table, int64_t table_ld,
@@ -503,8 +504,10 @@ int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
  *  fnx_rotary_append, the type of q (FNX_T_BF16 or FNX_T_F16); dim 64, 128 or 256; rows and
  *  strides 16-byte aligned; scale positive and finite.  max_context: a bound on context_lens.  partials: scratch of
  *  fnx_tree_attention_workspace_floats fp32, not shared by calls that may overlap.
- * Lengths outside the bounds record FNX_DEVERR_LENGTHS and leave the request's rows unwritten;
+ * Lengths outside the bounds record FNX_DEVERR_LENGTHS, and the request's rows get 0 and -inf;
  * page numbers outside [0, num_pages) record FNX_DEVERR_PAGE and their keys count as zeros.
+ * Rows of q ahead of node_offsets[0] and from node_offsets[batch] on get 0 and -inf (a captured call
+ * may be replayed with fewer nodes).  Offsets must not fall: where they do, rows are not defined.
  */
 int fnx_tree_attention_workspace_floats(int64_t* floats);
 int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,

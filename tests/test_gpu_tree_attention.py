@@ -566,3 +566,100 @@ def test_tree_layout_of_a_request_with_too_many_nodes():
     assert [c for _, c in e.value.codes] == [14]
     assert bool((mask[:65] == 0).all()) and bool((pos[:65] == 0).all()) and bool((slots[:65] == -1).all())
     assert mask[65:].tolist() == [1, 3, 5, 9, 17] and slots[65:].tolist() == [96 + 7 + j for j in range(5)]
+
+
+def _padded(c, ahead, behind):
+    """The case with rows of no request ahead of its own and behind them, and destinations that hold NaN."""
+    d = c.q.device
+    N, Hq, D = c.q.shape
+    q = torch.full((ahead + N + behind, Hq, D), float("nan"), dtype=c.q.dtype, device=d)
+    q[ahead:ahead + N] = c.q
+    mask = torch.full((ahead + N + behind,), -1, dtype=torch.int64, device=d)
+    mask[ahead:ahead + N] = c.mask
+    out = torch.full_like(q, float("nan"))
+    lse = torch.full(q.shape[:2], float("nan"), device=d)
+    return q, c.offsets + ahead, mask, out, lse
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens,counts,Hq,Hk", [
+    ([30], [3], 4, 2), ([50, 60, 0], [4, 9, 1], 4, 2), ([5000, 0, 3000], [16, 4, 9], 4, 1),
+    ([5000] * 12, [40, 1, 7] * 4, 8, 4), ([5000] * 12, [64, 1, 7] * 4, 16, 4), ([20, 100] * 100, [2, 3] * 100, 2, 1),
+])
+def test_rows_of_no_request(lens, counts, Hq, Hk, D):
+    """They give 0 and -inf, whatever q holds there, and are no error; the others are as without them."""
+    fx = _fx()
+    c = Case(lens, counts, Hq, Hk, D, 16, torch.bfloat16, seed=31)
+    ref, rlse = c.run()
+    N = c.q.shape[0]
+    for ahead, behind in ((0, 5), (3, 0), (2, 70)):
+        q, offsets, mask, out, lse = _padded(c, ahead, behind)
+        fx.tree_attention(q, c.k, c.v, c.table, c.ctx, offsets, mask, max_nodes=max(counts), max_context=max(lens),
+                          out=out, lse=lse)
+        fx.check_device_errors()
+        assert torch.equal(out[ahead:ahead + N], ref) and torch.equal(lse[ahead:ahead + N], rlse)
+        for rows in (slice(0, ahead), slice(ahead + N, None)):
+            assert bool((out[rows] == 0).all()) and bool((lse[rows] == -float("inf")).all())
+
+
+@pytest.mark.parametrize("D,Hk,ctx", [(64, 2, 60), (128, 2, 2000), (128, 4, 6000), (256, 4, 6000)])
+def test_rows_of_refused_requests(D, Hk, ctx):
+    """Requests whose lengths are out of bounds, among them the first and the last of a launch, give 0 and
+    -inf and the error; their neighbours are as ever."""
+    fx = _fx()
+    B = 140 if ctx == 60 else 12
+    counts = [3, 8, 1, 5] * (B // 4)
+    c = Case([ctx] * B, counts, 2 * Hk, Hk, D, 16, torch.bfloat16, seed=33)
+    ref, rlse = c.run()
+    refused = [0, 1, 5, B - 1] + ([127, 128] if B > 128 else [])
+    good = c.ctx.clone()
+    c.ctx[refused] = torch.tensor([-1, ctx + 1] * (len(refused) // 2), dtype=torch.int32, device=dev())
+    out, lse = torch.full_like(c.q, float("nan")), torch.full_like(rlse, float("nan"))
+    c.run(out=out, lse=lse)
+    with pytest.raises(fx.DeviceWaitError) as e:
+        fx.check_device_errors()
+    assert [x for _, x in e.value.codes] == [14]
+    off = c.offsets.tolist()
+    for b in range(B):
+        rows = slice(off[b], off[b + 1])
+        if b in refused:
+            assert bool((out[rows] == 0).all()) and bool((lse[rows] == -float("inf")).all()), b
+        else:  # the units are spread over the CTAs in another way, so sums may round differently
+            assert float((out[rows].float() - ref[rows].float()).abs().max()) <= 2 * 2.0**-8 * float(ref.float().abs().max())
+            assert float((lse[rows] - rlse[rows]).abs().max()) <= 2.0**-12, b
+    c.ctx.copy_(good)
+    again, alse = c.run()
+    assert torch.equal(again, ref) and torch.equal(alse, rlse)
+
+
+def test_a_captured_step_replayed_with_fewer_nodes():
+    """Layout, rotation and attention captured at 12 rows, replayed with 12, 5 and 0 nodes: the rest are 0."""
+    fx = _fx()
+    d, i32 = dev(), dict(dtype=torch.int32, device=dev())
+    c = Case([700, 40], [8, 4], 4, 2, 64, 16, torch.bfloat16, seed=35)
+    parents = torch.full((12,), -1, **i32)
+    table = fx.rotary_table(800, 64, device=d)
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(12, 2, 64, generator=g).bfloat16().to(d) for _ in range(2))
+
+    def step():
+        mask, pos, slots = fx.tree_layout(parents, c.offsets, c.ctx, c.table, 16, c.k.shape[0])
+        q = fx.rotary_append(c.q, k, v, pos, slots, table, c.k, c.v)
+        return fx.tree_attention(q, c.k, c.v, c.table, c.ctx, c.offsets, mask, max_nodes=8, max_context=700)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = step()
+    for offsets in ([0, 8, 12], [0, 3, 5], [0, 0, 0], [0, 8, 12]):
+        c.offsets.copy_(torch.tensor(offsets))
+        out.fill_(float("nan"))
+        lse.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        fx.check_device_errors()
+        n = offsets[2]
+        assert bool(out[:n].isfinite().all()) and bool(lse[:n].isfinite().all())
+        assert bool((out[n:] == 0).all()) and bool((lse[n:] == -float("inf")).all())
+        want, wlse = step()
+        assert torch.equal(out, want) and torch.equal(lse, wlse)
