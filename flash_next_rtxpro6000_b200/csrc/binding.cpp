@@ -62,6 +62,11 @@ int small(int64_t v, const char* name) {
   if (v < INT32_MIN || v > INT32_MAX) refuse(PyExc_NotImplementedError, "%s = %lld is too large", name, (long long)v);
   return (int)v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw std::bad_exception();
+  return v != 0;
+}
 double number(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw std::bad_exception();
@@ -172,7 +177,7 @@ PyObject* rotary_append(PyObject* const* a) {
                           ptr<int64_t>(slots), ptr<float>(table), table.stride(0), table.size(0), kc.data_ptr(),
                           kc.strides().data(), vc.data_ptr(), vc.strides().data(), kc.size(0),
                           small(kc.size(1), "page_size"), small(T, "tokens"), small(q.size(1), "q_heads"),
-                          small(Hk, "kv_heads"), small(D, "dim"), (int)R, PyObject_IsTrue(a[8]) == 1, type,
+                          small(Hk, "kv_heads"), small(D, "dim"), (int)R, truth(a[8]), type,
                           reinterpret_cast<int*>(integer(a[10])), (int)integer(a[11]), stream),
         "rotary_append");
   if (given(a[9])) {
