@@ -20,6 +20,13 @@
 
 namespace {
 
+// Other Python threads run while outputs are allocated and kernels launched: either may wait, for memory or
+// for room in the launch queue.  What is inside reads no Python object.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 struct Refused {
   PyObject* type;
   std::string what;
@@ -125,13 +132,21 @@ void caches(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) {
     refuse(PyExc_ValueError, "the elements of a cached head must be contiguous");
 }
 
-// Destination: a new tensor, or the caller's with as many heads.
-at::Tensor destination(PyObject* out, const at::Tensor& q) {
-  if (!given(out)) return at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+// The caller's destination, with as many heads, or null where a new one is wanted.
+const at::Tensor* destination(PyObject* out, const at::Tensor& q) {
+  if (!given(out)) return nullptr;
   const at::Tensor& t = tensor(out, "out");
   heads(t, "out", q.size(0), q.size(2), q);
   if (t.size(1) != q.size(1)) refuse(PyExc_ValueError, "out must have q's %lld heads", (long long)q.size(1));
-  return t;
+  return &t;
+}
+at::Tensor like(const at::Tensor& q) { return at::empty({q.size(0), q.size(1), q.size(2)}, q.options()); }
+
+// A result: the caller's own object, or a new tensor's.
+PyObject* result(PyObject* own, at::Tensor&& made) {
+  if (!given(own)) return THPVariable_Wrap(std::move(made));
+  Py_INCREF(own);
+  return own;
 }
 
 void page_table(const at::Tensor& t, int64_t batch, const at::Tensor& like) {
@@ -171,20 +186,24 @@ PyObject* rotary_append(PyObject* const* a) {
   if (kc.size(2) != Hk)
     refuse(PyExc_ValueError, "caches must have k's %lld heads, got %lld", (long long)Hk, (long long)kc.size(2));
   const cudaStream_t stream = stream_of(q);
-  at::Tensor out = destination(a[9], q);
-  check(fnx_rotary_append(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                          v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), ptr<int64_t>(pos),
-                          ptr<int64_t>(slots), ptr<float>(table), table.stride(0), table.size(0), kc.data_ptr(),
-                          kc.strides().data(), vc.data_ptr(), vc.strides().data(), kc.size(0),
-                          small(kc.size(1), "page_size"), small(T, "tokens"), small(q.size(1), "q_heads"),
-                          small(Hk, "kv_heads"), small(D, "dim"), (int)R, truth(a[8]), type,
-                          reinterpret_cast<int*>(integer(a[10])), (int)integer(a[11]), stream),
-        "rotary_append");
-  if (given(a[9])) {
-    Py_INCREF(a[9]);
-    return a[9];
+  const at::Tensor* to = destination(a[9], q);
+  const bool interleaved = truth(a[8]);
+  int* flag = reinterpret_cast<int*>(integer(a[10]));
+  const int pdl = (int)integer(a[11]);
+  at::Tensor made;
+  {
+    Unlocked others;
+    if (!to) made = like(q);
+    const at::Tensor& out = to ? *to : made;
+    check(fnx_rotary_append(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                            v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                            ptr<int64_t>(pos), ptr<int64_t>(slots), ptr<float>(table), table.stride(0), table.size(0),
+                            kc.data_ptr(), kc.strides().data(), vc.data_ptr(), vc.strides().data(), kc.size(0),
+                            small(kc.size(1), "page_size"), small(T, "tokens"), small(q.size(1), "q_heads"),
+                            small(Hk, "kv_heads"), small(D, "dim"), (int)R, interleaved, type, flag, pdl, stream),
+          "rotary_append");
   }
-  return THPVariable_Wrap(std::move(out));
+  return result(a[9], std::move(made));
 }
 
 // parents, node_offsets, context_lens, page_table, page_size, num_pages, error_flag, pdl
@@ -198,14 +217,20 @@ PyObject* tree_layout(PyObject* const* a) {
   index(ctx, "context_lens", B, at::kInt, parents);
   page_table(table, B, parents);
   const cudaStream_t stream = stream_of(parents);
-  at::Tensor out = at::empty({3, N}, parents.options().dtype(at::kLong));
-  int64_t* to = ptr<int64_t>(out);
-  check(fnx_tree_layout(ptr<int32_t>(parents), ptr<int32_t>(off), ptr<int32_t>(ctx), ptr<int32_t>(table),
-                        table.stride(0), small(table.size(1), "pages"), integer(a[5]),
-                        small(integer(a[4]), "page_size"), small(B, "batch"), small(N, "nodes"),
-                        reinterpret_cast<uint64_t*>(to), to + N, to + 2 * N, reinterpret_cast<int*>(integer(a[6])),
-                        (int)integer(a[7]), stream),
-        "tree_layout");
+  const int64_t page_size = integer(a[4]), num_pages = integer(a[5]);
+  int* flag = reinterpret_cast<int*>(integer(a[6]));
+  const int pdl = (int)integer(a[7]);
+  at::Tensor out;
+  {
+    Unlocked others;
+    out = at::empty({3, N}, parents.options().dtype(at::kLong));
+    int64_t* to = ptr<int64_t>(out);
+    check(fnx_tree_layout(ptr<int32_t>(parents), ptr<int32_t>(off), ptr<int32_t>(ctx), ptr<int32_t>(table),
+                          table.stride(0), small(table.size(1), "pages"), num_pages, small(page_size, "page_size"),
+                          small(B, "batch"), small(N, "nodes"), reinterpret_cast<uint64_t*>(to), to + N, to + 2 * N,
+                          flag, pdl, stream),
+          "tree_layout");
+  }
   PyObject* t = PyTuple_New(3);
   for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(out.select(0, i)));
   return t;
@@ -236,36 +261,38 @@ PyObject* tree_attention(PyObject* const* a) {
     mask = ptr<uint64_t>(m);
   }
   const cudaStream_t stream = stream_of(q);
-  at::Tensor out = destination(a[10], q), lse;
+  const at::Tensor *to = destination(a[10], q), *to_lse = nullptr;
   if (given(a[11])) {
-    lse = tensor(a[11], "lse");
+    const at::Tensor& lse = tensor(a[11], "lse");
     if (lse.dim() != 2 || lse.size(0) != N || lse.size(1) != Hq || lse.scalar_type() != at::kFloat ||
         lse.device() != q.device() || !lse.is_contiguous())
       refuse(PyExc_ValueError, "lse must be a contiguous fp32 [%lld, %lld] tensor on %s", (long long)N, (long long)Hq,
              q.device().str().c_str());
-  } else {
-    lse = at::empty({N, Hq}, q.options().dtype(at::kFloat));
+    to_lse = &lse;
   }
-  const int64_t room = table.size(1) * kc.size(1);
-  check(fnx_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), kc.strides().data(), vc.data_ptr(),
-                           vc.strides().data(), kc.size(0), small(kc.size(1), "page_size"), ptr<int32_t>(table),
-                           table.stride(0), small(table.size(1), "pages"), ptr<int32_t>(ctx), ptr<int32_t>(off), mask,
-                           out.data_ptr(), out.stride(0), out.stride(1), ptr<float>(lse), small(B, "batch"),
-                           small(N, "nodes"), small(Hq, "q_heads"), small(Hk, "kv_heads"), small(D, "dim"),
-                           small(integer(a[7]), "max_nodes"), given(a[8]) ? integer(a[8]) : room,
-                           given(a[9]) ? (float)number(a[9]) : 1.0f / std::sqrt((float)D), type,
-                           reinterpret_cast<float*>(integer(a[12])), reinterpret_cast<int*>(integer(a[13])),
-                           (int)integer(a[14]), stream),
-        "tree_attention");
+  const int max_nodes = small(integer(a[7]), "max_nodes");
+  const int64_t max_context = given(a[8]) ? integer(a[8]) : table.size(1) * kc.size(1);
+  const float scale = given(a[9]) ? (float)number(a[9]) : 1.0f / std::sqrt((float)D);
+  float* partials = reinterpret_cast<float*>(integer(a[12]));
+  int* flag = reinterpret_cast<int*>(integer(a[13]));
+  const int pdl = (int)integer(a[14]);
+  at::Tensor made, made_lse;
+  {
+    Unlocked others;
+    if (!to) made = like(q);
+    if (!to_lse) made_lse = at::empty({N, Hq}, q.options().dtype(at::kFloat));
+    const at::Tensor &out = to ? *to : made, &lse = to_lse ? *to_lse : made_lse;
+    check(fnx_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), kc.strides().data(), vc.data_ptr(),
+                             vc.strides().data(), kc.size(0), small(kc.size(1), "page_size"), ptr<int32_t>(table),
+                             table.stride(0), small(table.size(1), "pages"), ptr<int32_t>(ctx), ptr<int32_t>(off), mask,
+                             out.data_ptr(), out.stride(0), out.stride(1), ptr<float>(lse), small(B, "batch"),
+                             small(N, "nodes"), small(Hq, "q_heads"), small(Hk, "kv_heads"), small(D, "dim"), max_nodes,
+                             max_context, scale, type, partials, flag, pdl, stream),
+          "tree_attention");
+  }
   PyObject* t = PyTuple_New(2);
-  PyObject* given_out[2] = {a[10], a[11]};
-  at::Tensor made[2] = {std::move(out), std::move(lse)};
-  for (int i = 0; i < 2; ++i) {
-    PyObject* o = given_out[i];
-    if (given(o)) Py_INCREF(o);
-    else o = THPVariable_Wrap(std::move(made[i]));
-    PyTuple_SET_ITEM(t, i, o);
-  }
+  PyTuple_SET_ITEM(t, 0, result(a[10], std::move(made)));
+  PyTuple_SET_ITEM(t, 1, result(a[11], std::move(made_lse)));
   return t;
 }
 
@@ -290,13 +317,19 @@ PyObject* sample_tokens(PyObject* const* a) {
     p[i] = t.data_ptr();
   }
   const cudaStream_t stream = stream_of(x);
-  at::Tensor tokens = at::empty({M}, x.options().dtype(at::kLong)), probs = at::empty({M}, x.options().dtype(at::kFloat));
-  check(fnx_sample(x.data_ptr(), M > 1 ? x.stride(0) : std::max(x.stride(0), V),
-                   st == at::kFloat ? FNX_T_F32 : st == at::kHalf ? FNX_T_F16 : FNX_T_BF16, small(M, "rows"),
-                   small(V, "vocab"), ptr<float>(u), static_cast<const float*>(p[0]),
-                   static_cast<const int32_t*>(p[1]), static_cast<const float*>(p[2]), static_cast<const float*>(p[3]),
-                   ptr<int64_t>(tokens), ptr<float>(probs), (int)integer(a[6]), stream),
-        "sample_tokens");
+  const int pdl = (int)integer(a[6]);
+  at::Tensor tokens, probs;
+  {
+    Unlocked others;
+    tokens = at::empty({M}, x.options().dtype(at::kLong));
+    probs = at::empty({M}, x.options().dtype(at::kFloat));
+    check(fnx_sample(x.data_ptr(), M > 1 ? x.stride(0) : std::max(x.stride(0), V),
+                     st == at::kFloat ? FNX_T_F32 : st == at::kHalf ? FNX_T_F16 : FNX_T_BF16, small(M, "rows"),
+                     small(V, "vocab"), ptr<float>(u), static_cast<const float*>(p[0]),
+                     static_cast<const int32_t*>(p[1]), static_cast<const float*>(p[2]), static_cast<const float*>(p[3]),
+                     ptr<int64_t>(tokens), ptr<float>(probs), pdl, stream),
+          "sample_tokens");
+  }
   PyObject* t = PyTuple_New(2);
   PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(tokens)));
   PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(probs)));
