@@ -255,14 +255,14 @@ def ops():
     with _lock:
         if _ops is None:
             lib()
-            if not OPS_PATH.exists():
-                try:
-                    from .build import build_binding
+            from . import build
 
-                    build_binding()
+            if not build.binding_fits():
+                try:
+                    build.build_binding()
                 except Exception as e:  # pragma: no cover - depends on the toolchain
                     raise ImportError(
-                        f"{OPS_PATH.name} is missing and could not be built ({e}); run "
+                        f"{OPS_PATH.name} is missing, or of another torch, and could not be built ({e}); run "
                         "`python -m flash_next_rtxpro6000_b200.build`"
                     ) from e
             import importlib.machinery

@@ -48,8 +48,24 @@ def _inputs():
         sorted(INCLUDE.glob("*.h"))
 
 
+def binding_build() -> str:
+    """What a binding is made for: torch's C++ interface changes from build to build, the
+    interpreter's from version to version."""
+    import sysconfig
+
+    import torch
+
+    return (f"fnx binding for torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} "
+            f"python {sysconfig.get_config_var('SOABI')};")
+
+
+def binding_fits() -> bool:
+    """Whether ``_fnx_ops.so`` is there and was made for this torch and interpreter (it holds the text)."""
+    return OPS_PATH.exists() and binding_build().encode() in OPS_PATH.read_bytes()
+
+
 def up_to_date() -> bool:
-    if not LIB_PATH.exists() or not OPS_PATH.exists():
+    if not LIB_PATH.exists() or not binding_fits():
         return False
     t = min(LIB_PATH.stat().st_mtime, OPS_PATH.stat().st_mtime)
     return all(p.stat().st_mtime <= t for p in _inputs())
@@ -96,6 +112,7 @@ def build_binding() -> Path:
     tmp = OPS_PATH.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DFNX_BINDING_BUILD="{binding_build()}"',
            f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include",
            f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", str(CSRC / BINDING),
            "-o", str(tmp), f"-L{PKG}", "-l:_fnx.so", f"-L{root}/lib", "-lc10", "-lc10_cuda", "-ltorch",

@@ -365,7 +365,8 @@ PyMethodDef kMethods[] = {
     method<tree_attention, 15>("tree_attention"), method<sample_tokens, 7>("sample_tokens"),
     {nullptr, nullptr, 0, nullptr}};
 
-PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fnx_ops", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+// What the module was built for is its documentation, and looked for in the file before it is loaded.
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fnx_ops", FNX_BINDING_BUILD, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 
