@@ -233,9 +233,9 @@ def lib():
         if _lib is None:
             if not LIB_PATH.exists():
                 try:
-                    from .build import build
+                    from .build import build_library
 
-                    build()
+                    build_library()
                 except Exception as e:  # pragma: no cover - depends on the toolchain
                     raise ImportError(
                         f"{LIB_PATH.name} is missing and could not be built ({e}); run "

@@ -43,9 +43,13 @@ def nvcc() -> str:
     return cand
 
 
-def _inputs():
-    return [CSRC / s for s in SOURCES + [BINDING]] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + \
-        sorted(INCLUDE.glob("*.h"))
+def _newer(path: Path, inputs) -> bool:
+    return path.exists() and all(p.stat().st_mtime <= path.stat().st_mtime for p in inputs)
+
+
+def library_up_to_date() -> bool:
+    return _newer(LIB_PATH, [CSRC / s for s in SOURCES] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) +
+                  sorted(INCLUDE.glob("*.h")))
 
 
 def binding_build() -> str:
@@ -65,15 +69,21 @@ def binding_fits() -> bool:
 
 
 def up_to_date() -> bool:
-    if not LIB_PATH.exists() or not binding_fits():
-        return False
-    t = min(LIB_PATH.stat().st_mtime, OPS_PATH.stat().st_mtime)
-    return all(p.stat().st_mtime <= t for p in _inputs())
+    return library_up_to_date() and binding_fits() and \
+        _newer(OPS_PATH, [CSRC / BINDING] + sorted(INCLUDE.glob("*.h")))
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the library and the binding if any of their sources is newer; returns the library's path."""
+    if force or not up_to_date():
+        build_library(force, verbose)
+        build_binding()
+    return LIB_PATH
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
     """Compile the library if any source is newer than it; returns its path."""
-    if not force and up_to_date():
+    if not force and library_up_to_date():
         return LIB_PATH
     OBJ_DIR.mkdir(exist_ok=True)
     cc = nvcc()
@@ -97,7 +107,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
-    build_binding()
     return LIB_PATH
 
 

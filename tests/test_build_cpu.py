@@ -45,3 +45,34 @@ class Loader:  # what is loaded is not the point here, and a second copy of the 
 
     def exec_module(self, module):
         pass
+
+
+def test_the_library_needs_no_binding(tmp_path, monkeypatch):
+    """Where torch's or Python's headers are missing the GEMVs, MoE and router load as ever."""
+    path = tmp_path / build.LIB_PATH.name
+    monkeypatch.setattr(build, "LIB_PATH", path)
+    monkeypatch.setattr(_lib, "LIB_PATH", path)
+    monkeypatch.setattr(build, "OBJ_DIR", tmp_path / "objects")
+    monkeypatch.setattr(build, "nvcc", lambda: "nvcc")
+
+    class Done:
+        returncode, stdout, stderr = 0, "", ""
+
+    def compiler(cmd, **kw):
+        assert cmd[0] == "nvcc"
+        out = cmd[cmd.index("-o") + 1]
+        with open(out, "w") as f:
+            f.write("made")
+        return Done
+
+    def no_headers():
+        raise RuntimeError("Python.h: no such file")
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    monkeypatch.setattr(build, "build_binding", no_headers)
+    monkeypatch.setattr(_lib, "_declare", lambda handle: None)
+    monkeypatch.setattr(_lib.ctypes, "CDLL", lambda at: at)
+    monkeypatch.setattr(_lib, "_lib", None)
+    assert _lib.lib() == str(path) and path.read_text() == "made"
+    with pytest.raises(RuntimeError):  # the command still says so
+        build.build(force=True)
