@@ -38,6 +38,7 @@ DEVICE_ERRORS = {
     15: "PAGE: a page number outside the cache",
     16: "TREE: a parent that is not an earlier node",
 }
+ARGUMENT_ERRORS = (9, 11, 12, 13, 14, 15, 16)  # those that are no waits
 
 EXPORTED = (
     "fnx_set_dense_path",

@@ -3,11 +3,13 @@
 Every wait inside the kernels is bounded: a wait that runs out of time records an error
 code in its workspace's ``error_flag`` (the first code of a call wins), the kernel leaves
 its loop and the launch completes, so the CUDA context stays usable, but that call's
-outputs are wrong.  The launch itself reports success; the flag is how the host learns
-of it.  Nothing on the device clears a flag.
+outputs are wrong.  The verify-step operators record in the same way what only the device
+can see of their arguments: positions, cache slots, lengths, pages and parents out of
+bounds (codes 12 to 16), which are not followed.  The launch itself reports success; the
+flag is how the host learns of either.  Nothing on the device clears a flag.
 
-``check_device_errors`` reads every flag this process has created (the dense GEMV
-scratch slots, every MoE workspace from ``make_workspace``) in one device-to-host copy,
+``check_device_errors`` reads every flag this process has created (the scratch slots,
+every MoE workspace from ``make_workspace``) in one device-to-host copy,
 clears the ones that are set and raises ``DeviceWaitError`` naming them.  It
 synchronises the current stream, so call it outside CUDA graph capture, after the work
 whose results you are about to trust (for example once per decode step, or in tests).
@@ -21,17 +23,20 @@ from typing import List, Optional, Tuple
 
 import torch
 
-from ._lib import DEVICE_ERRORS
+from ._lib import ARGUMENT_ERRORS, DEVICE_ERRORS
 
 
 class DeviceWaitError(RuntimeError):
-    """A kernel's bounded wait ran out of time; ``codes`` lists (source, code) pairs."""
+    """A kernel recorded an error: a bounded wait that ran out of time, or an argument out of
+    bounds; ``codes`` lists (source, code) pairs."""
 
     def __init__(self, codes: List[Tuple[str, int]]):
         self.codes = codes
         msg = "; ".join(f"{src}: code {c} ({DEVICE_ERRORS.get(c, 'unknown')})" for src, c in codes)
-        super().__init__("device-side wait expired, results of the affected calls are invalid: "
-                         + msg)
+        what = [text for text, some in (
+            ("device-side wait expired", any(c not in ARGUMENT_ERRORS for _, c in codes)),
+            ("argument out of bounds on the device", any(c in ARGUMENT_ERRORS for _, c in codes))) if some]
+        super().__init__(f"{' and '.join(what)}, results of the affected calls are invalid: {msg}")
 
 
 _lock = threading.Lock()

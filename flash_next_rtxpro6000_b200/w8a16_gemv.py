@@ -68,7 +68,8 @@ class GemvConfig:
 
 
 class Workspace:
-    """Split-K partials + counters and argmax keys of one (device, slot)."""
+    """Split-K partials + counters, argmax keys and the error flag of one (device, slot), and the
+    attention's partials once they are wanted."""
 
     def __init__(self, device: torch.device):
         self.device = device
@@ -77,7 +78,8 @@ class Workspace:
         self.argmax_keys = torch.zeros(_lib.MAX_M, dtype=torch.int64, device=device)
         self.argmax_count = torch.zeros(1, dtype=torch.int32, device=device)
         self.error_flag = torch.zeros(1, dtype=torch.int32, device=device)
-        errors.register(self.error_flag, f"dense GEMV scratch on {device}")
+        self.attention = None
+        errors.register(self.error_flag, f"scratch slot on {device}")
         self.c = FnxWorkspace(ptr(self.partials), _WS_FLOATS, ptr(self.counters), _WS_COUNTERS,
                               ptr(self.argmax_keys), ptr(self.argmax_count),
                               ptr(self.error_flag))

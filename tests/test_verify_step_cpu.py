@@ -112,3 +112,12 @@ def test_rotary_table_on_the_host():
     assert t[0].tolist() == [1.0] * 4 + [0.0] * 4
     scaled = fx.rotary_table(10, 8, scaling=fx.RotaryScaling(2.0, "linear"), device="cpu")
     assert torch.equal(scaled[2], t[1].float())
+
+
+def test_device_errors_say_what_happened():
+    wait, slot = ("a", 3), ("b", 13)
+    assert str(fx.DeviceWaitError([wait])).startswith("device-side wait expired, ")
+    text = str(fx.DeviceWaitError([slot]))
+    assert "wait" not in text and "out of bounds" in text and "SLOT" in text
+    text = str(fx.DeviceWaitError([wait, slot]))
+    assert "wait expired and argument out of bounds" in text
