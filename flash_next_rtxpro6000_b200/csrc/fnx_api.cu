@@ -1409,6 +1409,8 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
   if (max_context > (1ll << 31) - 1 - 256)
     return fail(FNX_EUNSUPPORTED, "tree attention: contexts of 2^31 tokens");
   if (q_heads > 65535) return fail(FNX_EUNSUPPORTED, "tree attention: %d heads", q_heads);
+  if (fnx::num_sms() > fnx::kAttnMaxGrid)  // what the joining launch holds
+    return fail(FNX_EUNSUPPORTED, "tree attention: a GPU of %d SMs (at most %d)", fnx::num_sms(), fnx::kAttnMaxGrid);
   if (!(scale > 0.f) || scale > 3.0e38f)
     return fail(FNX_EINVAL, "tree attention: scale %g must be positive and finite", (double)scale);
   if (nodes == 0) return FNX_OK;

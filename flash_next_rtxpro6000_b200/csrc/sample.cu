@@ -56,7 +56,7 @@ constexpr float kReach = 28.0f;
 constexpr uint32_t kLowest = 0x00800000u;  // order bits of the lowest finite fp32 value
 
 enum Want : int { WANT_COUNT = 0, WANT_SHARE = 1, WANT_SUM = 2 };
-enum Op : int { OP_DONE = 0, OP_GATHER = 1, OP_SPLIT = 2, OP_BINS = 3 };
+enum Op : int { OP_DONE = 0, OP_GATHER = 1, OP_SPLIT = 2 };
 constexpr int kCluster = 8;  // CTAs of a row, at most
 
 struct Control {  // written by the first CTA, read by the cluster

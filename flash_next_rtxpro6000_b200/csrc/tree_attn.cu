@@ -549,7 +549,6 @@ int launch_d(const AttnArgs& a, cudaStream_t stream) {
   else if (most <= 32) rc = launch_form<T, D, 2, 4>(a, stream, grid, rows);
   else rc = launch_form<T, D, 4, 2>(a, stream, grid, rows);
   if (rc) return rc;
-  if (grid > kAttnMaxGrid) return 2;
   if (a.max_context + a.max_nodes <= kKeyTile) return 0;  // one key tile: no item is split
   cudaLaunchConfig_t cfg = {};
   const bool many = (int64_t)a.N * a.Hq >= 8 * num_sms();  // a row for each of eight warps an SM
@@ -578,7 +577,8 @@ int launch_t(const AttnArgs& a, cudaStream_t stream) {
 
 int64_t attn_workspace_floats() {
   // the widest slots: 256 rows of 128, 128 rows of 256
-  return 2ll * num_sms() * attn_slot_floats(256, 128); }
+  return 2ll * num_sms() * attn_slot_floats(256, 128);
+}
 
 int launch_tree_attn(const AttnArgs& a, cudaStream_t stream) {
   return a.f16 ? launch_t<__half>(a, stream) : launch_t<__nv_bfloat16>(a, stream);
