@@ -1297,6 +1297,7 @@ int fnx_rotary_append(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     return fail(FNX_EINVAL, "rotary: rotated=%d must be even and at most dim=%d", rotated, dim);
   if (page_size < 1 || num_pages < 0 || positions < 1 || table_ld < rotated)
     return fail(FNX_EINVAL, "rotary: bad table or cache shape");
+  if (tokens > 1 << 30) return fail(FNX_EUNSUPPORTED, "rotary: %d tokens (at most 2^30)", tokens);
   if (tokens == 0) return FNX_OK;
   if ((q_heads && (!q || !q_out)) || (kv_heads && (!k || !v || !k_cache || !v_cache)) || !pos ||
       !slots || !table)
@@ -1353,6 +1354,7 @@ int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
   if (batch < 0 || nodes < 0 || (slots && (page_size < 1 || table_width < 0 || num_pages < 0)))
     return fail(FNX_EINVAL, "tree layout: bad shape batch=%d nodes=%d page_size=%d", batch, nodes,
                 page_size);
+  if (nodes > 1 << 30) return fail(FNX_EUNSUPPORTED, "tree layout: %d nodes (at most 2^30)", nodes);
   if (nodes == 0) return FNX_OK;
   if (batch < 1 || !parents || !node_offsets || ((positions || slots) && !context_lens) ||
       (slots && !page_table))

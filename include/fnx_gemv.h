@@ -458,7 +458,7 @@ int fnx_static_ws_error(int clear, fnx_stream_t stream, int* code);
  *  pos int64 [tokens]; slots int64 [tokens]: token t's place in the cache (page * page_size
  *  + place in the page), -1 = not stored.  k_cache / v_cache [num_pages, page_size,
  *  kv_heads, dim] with *_strides = element strides of pages, places and heads.
- * Two tokens with the same slot race.  A position outside the table takes the nearest row and
+ * At most 2^30 tokens.  Two tokens with the same slot race.  A position outside the table takes the nearest row and
  * records FNX_DEVERR_POSITION; a slot outside the cache is not stored and records
  * FNX_DEVERR_SLOT (error_flag may be NULL).
  */

@@ -121,3 +121,10 @@ def test_device_errors_say_what_happened():
     assert "wait" not in text and "out of bounds" in text and "SLOT" in text
     text = str(fx.DeviceWaitError([wait, slot]))
     assert "wait expired and argument out of bounds" in text
+
+
+@pytest.mark.parametrize("n", [2**30 + 1, 2**31 - 1])
+def test_more_tokens_than_the_kernels_count(n):
+    """Their 32-bit token numbers would pass 2^31 in the last stride."""
+    assert _rotary(T=n) == _lib.FNX_EUNSUPPORTED
+    assert _layout(N=n) == _lib.FNX_EUNSUPPORTED
