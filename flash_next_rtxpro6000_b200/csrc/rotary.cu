@@ -10,8 +10,8 @@
 // A unit is 16 elements of a head: two 16-byte vectors that hold eight whole pairs in either
 // layout, so a unit needs nothing of its neighbours and q may be rotated in place.  A block is
 // D/16 units wide; its rows walk the token's heads, so a thread's cosines and sines stay in
-// registers over all the heads it turns.  Measured (B200, on the GPU): 2.2 us for one token of 16 + 2 heads
-// of 256, 21.8 us for 4,097 tokens of 32 + 8 heads of 128 (102 MB, 4.7 TB/s).
+// registers over all the heads it turns.  Measured (B200, calls in a graph): 2.3 us for one token of 16 + 2 heads
+// of 256 and for 16 of 32 + 8 heads of 128, 21.8 us for 4,097 tokens of 32 + 8 heads of 128 (102 MB, 4.7 TB/s).
 #include "fnx_common.cuh"
 #include "fnx_kernels.h"
 

@@ -29,7 +29,7 @@
 // Measured (B200): one row of 151,936 bf16 logits 10 us with a top-k of 50, 25 to 31 without top-k (of some
 // 57,000 cycles the histogram's pass takes 15,000 to 19,000, its exponentials and shared-memory adds in
 // equal parts, the gathering 9,000, the exchanges about 1,500 each); 16 such rows in fp32 28 to 32 us; 128
-// rows of 248,320 137 us.
+// rows of 248,320 138 us.  The form for many rows has 64 registers a thread and spills some 500 bytes of them.
 #include <cooperative_groups.h>
 
 #include <type_traits>

@@ -19,9 +19,9 @@
 // then weights may be larger than one, which costs nothing in floating point.  Every wait is bounded and records an error code; roles then fall
 // through to the end.
 //
-// Measured (B200): 24 ragged requests, D = 128 fp16, 357 MB: 103 us, 3.4 TB/s; 4 requests of 64 nodes
-// over 131,072 keys, 1.48 GB and 171 GFLOP: 397 us, 3.7 TB/s and 430 TFLOP/s.  Loading alone (the rings
-// emptied at once) takes 234 us at the latter.  What bounds it is the softmax warps' chain per tile:
+// Measured (B200, both launches, calls in a graph): 24 ragged requests, D = 128 fp16, 357 MB: 104 us, 3.4
+// TB/s; 4 requests of 64 nodes over 131,072 keys, 1.48 GB and 171 GFLOP: 400 to 430 us, 3.4 to 3.7 TB/s and
+// 400 to 430 TFLOP/s.  Loading alone (the rings emptied at once) takes 234 us at the latter.  What bounds it is the softmax warps' chain per tile:
 // about 1,800 cycles from scores to weights, of which the exponentials' unit is busy for 512 a row tile.
 // A second group on every other key tile of the same rows gained nothing (the rows' quarter of the SM
 // has one unit for both groups), nor did deeper rings.

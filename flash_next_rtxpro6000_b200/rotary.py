@@ -26,7 +26,13 @@ class RotaryScaling:
     ``linear``: every frequency divided by ``factor``.  ``ramp``: pairs that turn fewer than
     ``slow`` times over the original length are divided, those that turn more than ``fast``
     times are kept, with a linear ramp in the number of turns between; cosines and sines are
-    multiplied by ``attention`` (default 0.1 ln(factor) + 1)."""
+    multiplied by ``attention`` (default 0.1 ln(factor) + 1).
+
+    Checkpoints differ in the ramp: some ramp linearly in the pair's index, between the two indices
+    (often rounded to whole ones) at which a pair turns ``fast`` and ``slow`` times.  With the same two
+    numbers the pairs between then turn at other rates (by up to 40 % at 64 rotated elements, base 1e6,
+    factor 4).  For those make the fp32 table of cosines and sines with their own frequencies;
+    ``rotary_append`` takes any table."""
 
     factor: float
     kind: str = "ramp"

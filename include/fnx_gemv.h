@@ -502,8 +502,9 @@ int fnx_tree_layout(const int32_t* parents, const int32_t* node_offsets,
  * table entries past a request's last page are not read.
  *  q, out [nodes, q_heads, dim] with strides (elements) over nodes and heads; caches as in
  *  fnx_rotary_append, the type of q (FNX_T_BF16 or FNX_T_F16); dim 64, 128 or 256; rows and
- *  strides 16-byte aligned; scale positive and finite.  max_context: a bound on context_lens.  partials: scratch of
- *  fnx_tree_attention_workspace_floats fp32, not shared by calls that may overlap.
+ *  strides 16-byte aligned; scale positive and finite.  max_context: a bound on context_lens;
+ *  near the real lengths it is faster.  partials: scratch of fnx_tree_attention_workspace_floats fp32
+ *  (for the GPU that is current), not shared by calls that may overlap.
  * Lengths outside the bounds record FNX_DEVERR_LENGTHS, and the request's rows get 0 and -inf;
  * page numbers outside [0, num_pages) record FNX_DEVERR_PAGE and their keys count as zeros.
  * Rows of q ahead of node_offsets[0] and from node_offsets[batch] on get 0 and -inf (a captured call
