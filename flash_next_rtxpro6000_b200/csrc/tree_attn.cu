@@ -5,8 +5,8 @@
 // over the keys j < L of the request's context and the drafted tokens L + n whose bit n is set in node
 // i's mask; lse_i = log sum_j exp(scale q_i k_j).  A row that sees nothing gives 0 and -inf.  One pass
 // over the keys with a running maximum and sum; scores, weights' sums and outputs are held in fp32,
-// the weights are rounded to the cache's type for the second product (as wide as its other operand; fp16
-// weights relative to a reference that keeps them in its range, tree_attn.cuh).
+// the weights are rounded to the cache's type for the second product (as wide as its other operand, and
+// relative to a reference that keeps fp16 weights in its range: tree_attn.cuh).
 //
 // Bound: the cache's bytes, each read once for all G query heads and all nodes that share a kv head:
 // the G * T rows of a kv head are one matrix operand.  mma.sync.m16n8k16 with keys and values in

@@ -16,13 +16,14 @@
 // piece, so the row's maximum and sum need no shuffles), 4 warps that load keys and 4 that load values
 // (cp.async, any page size), one warp that issues the first product and one the second.  O is rescaled
 // only when a row's maximum has risen by more than 2^8 (or, with fp16, fallen far: tree_attn.cuh): until
-// then weights may be larger than one, which costs nothing in floating point.  Every wait is bounded and records an error code; roles then fall
-// through to the end.
+// then weights may be larger than one, which costs nothing in floating point.  Every wait is bounded and
+// records an error code; roles then fall through to the end.
 //
 // Measured (B200, both launches, calls in a graph): 24 ragged requests, D = 128 fp16, 357 MB: 104 us, 3.4
 // TB/s; 4 requests of 64 nodes over 131,072 keys, 1.48 GB and 171 GFLOP: 400 to 430 us, 3.4 to 3.7 TB/s and
-// 400 to 430 TFLOP/s.  Loading alone (the rings emptied at once) takes 234 us at the latter.  What bounds it is the softmax warps' chain per tile:
-// about 1,800 cycles from scores to weights, of which the exponentials' unit is busy for 512 a row tile.
+// 400 to 430 TFLOP/s.  Loading alone (the rings emptied at once) takes 234 us at the latter.  What bounds
+// it is the softmax warps' chain per tile: about 1,800 cycles from scores to weights, of which the
+// exponentials' unit is busy for 512 a row tile.
 // A second group on every other key tile of the same rows gained nothing (the rows' quarter of the SM
 // has one unit for both groups), nor did deeper rings.
 #include <type_traits>
@@ -35,6 +36,7 @@ namespace {
 
 constexpr int kTile = kKeyTile;
 constexpr int kBlockBytes = kTile * 128;  // 64 rows of a 64-element block
+// Bits by which a row's maximum may rise above its reference's, and a tile's fall below it (fp16), unnoticed.
 constexpr float kRise = 8.0f, kFall = 14.0f;
 template <typename T> constexpr float kHead = kNarrow<T> ? 7.0f : 0.0f;  // weights are at most 2^(kHead + kRise)
 
