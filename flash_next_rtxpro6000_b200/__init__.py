@@ -17,7 +17,12 @@ the hand-written CUDA library ``_fnx.so``):
   a paged cache, in one launch;
 * ``tree_layout``, ``tree_attention`` -- attention of drafted token trees over a paged cache
   (one node a request: decode);
-* ``sample_tokens`` -- temperature, top-k, top-p and min-p sampling from given random numbers;
+* ``rotary_append8``, ``tree_attention8`` -- the same two over a cache of 8 bits with a scale for each
+  block of tokens and head;
+* ``sample_tokens``, ``token_probs`` -- temperature, top-k, top-p and min-p sampling from given random
+  numbers, and the probabilities that it draws from;
+* ``verify_tokens`` -- verification of drafted trees against the target's probabilities;
+  ``compact_nodes`` -- the accepted nodes' keys and values moved behind the context;
 * ``nvfp4_dense`` -- the NVFP4 dense lm_head: load-time packing with an on-disk cache
   and the linear method serving it through the NVFP4 GEMV;
 * ``sharded`` -- vocab-sharded lm_head and expert-sharded MoE over torch.distributed;
@@ -66,7 +71,9 @@ from .errors import DeviceWaitError, check_device_errors  # noqa: F401
 from .router import covered, route_softmax_fast, router_gemv, router_topk  # noqa: F401
 from .draft_topk1 import draft_head_topk1, draft_topk1_postprocess  # noqa: F401
 from .rotary import RotaryScaling, rotary_append, rotary_table  # noqa: F401
-from .sampling import sample_tokens  # noqa: F401
+from .sampling import sample_tokens, token_probs  # noqa: F401
 from .tree_attention import tree_attention, tree_layout  # noqa: F401
+from .cache8 import rotary_append8, tree_attention8  # noqa: F401
+from .verification import compact_nodes, verify_tokens  # noqa: F401
 
 __version__ = "0.1.0"

@@ -37,8 +37,10 @@ DEVICE_ERRORS = {
     14: "LENGTHS: lengths that contradict each other or the bounds given",
     15: "PAGE: a page number outside the cache",
     16: "TREE: a parent that is not an earlier node",
+    17: "TOKEN: a drafted token outside the vocabulary",
+    18: "SCALE: a cache scale that no append writes",
 }
-ARGUMENT_ERRORS = (9, 11, 12, 13, 14, 15, 16)  # those that are no waits
+ARGUMENT_ERRORS = (9, 11, 12, 13, 14, 15, 16, 17, 18)  # those that are no waits
 
 EXPORTED = (
     "fnx_set_dense_path",
@@ -74,6 +76,11 @@ EXPORTED = (
     "fnx_tree_attention_workspace_floats",
     "fnx_tree_attention",
     "fnx_sample",
+    "fnx_token_probs",
+    "fnx_rotary_append8",
+    "fnx_tree_attention8",
+    "fnx_verify_tokens",
+    "fnx_compact_nodes",
     "fnx_last_error",
     "fnx_version",
 )
@@ -218,6 +225,20 @@ def _declare(lib):
         c_int64, c_int64, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_float, c_int, _P, _P,
         c_int, _P]
     lib.fnx_sample.argtypes = [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P]
+    lib.fnx_token_probs.argtypes = [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int64, c_int, _P]
+    lib.fnx_rotary_append8.argtypes = [
+        _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, _P, _P,
+        c_int64, c_int, _P, c_int64, c_int64, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, c_int64, c_int, c_int,
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, c_int, _P]
+    lib.fnx_tree_attention8.argtypes = [
+        _P, c_int64, c_int64, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, c_int64, c_int, c_int, _P, c_int64, c_int,
+        _P, _P, _P, _P, c_int64, c_int64, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_float, c_int, _P,
+        _P, c_int, _P]
+    lib.fnx_verify_tokens.argtypes = [_P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P,
+                                      _P, _P, _P, c_int, _P]
+    lib.fnx_compact_nodes.argtypes = [
+        _P, _I64P, c_int64, _P, _I64P, c_int64, _P, _I64P, c_int64, _P, _I64P, c_int64, c_int64, c_int, c_int, c_int,
+        c_int, c_int, c_int, _P, c_int64, c_int, _P, _P, c_int64, _P, c_int, c_int, _P, _P, c_int, _P]
     lib.fnx_last_error.restype = c_char_p
     lib.fnx_version.restype = c_char_p
     for name in EXPORTED:

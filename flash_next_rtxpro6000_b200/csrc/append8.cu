@@ -1,0 +1,320 @@
+// Rotary positions on queries and keys, with keys and values stored in an 8-bit paged cache (cache8.cuh).
+//
+// The rotation is rotary.cu's: (a cos - b sin, b cos + a sin) for the pairs of a head's first R elements, in fp32
+// with each product and sum rounded by itself.  Request b's new tokens go to places context_lens[b] + index.  For
+// every block of places and every head that gets new tokens, with amax their largest finite magnitude:
+//
+//   s' = smallest power of two >= amax / 448 (2^-40 at least), and >= the block's old scale if tokens of the context
+//        stay in the block;     new bytes = e4m3(y / s'),     old bytes = e4m3(value s / s')
+//
+// Bound: memory (each 16-bit element read once, a 16-bit query or an 8-bit key or value written once), or the launch
+// and its chain of loads (offsets, page, data) for a few tokens.  A CTA has one block of one request and as many
+// (key or value) heads as its 256 threads hold, a thread 16 elements of a token's head, or up to four times that: it
+// finds the block's largest element with one exchange and writes the block without reading anything twice.  The
+// queries go to CTAs of their own in the same launch.
+#include "cache8.cuh"
+
+namespace fnx {
+
+namespace {
+
+constexpr int kAT = 256;  // threads
+
+template <typename T> __device__ __forceinline__ float2 two(uint32_t w);
+template <> __device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <> __device__ __forceinline__ float2 two<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+__device__ __forceinline__ float one(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float one(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ uint32_t round_two(float a, float b);
+template <> __device__ __forceinline__ uint32_t round_two<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t round_two<__half>(float a, float b) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// 16 elements of a head: two runs of eight, which hold whole pairs where the sizes allow 16-byte vectors.
+struct Unit {
+  int o0, o1;
+};
+template <bool kVec>
+__device__ __forceinline__ Unit unit_of(const Append8Args& a, int u) {
+  const bool apart = kVec && 16 * u < a.R && !a.interleaved;
+  return apart ? Unit{8 * u, a.R / 2 + 8 * u} : Unit{16 * u, 16 * u + 8};
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void load_unit(const T* src, const Unit& un, float (&x)[16]) {
+  if (kVec) {
+    const uint4 v0 = *reinterpret_cast<const uint4*>(src + un.o0), v1 = *reinterpret_cast<const uint4*>(src + un.o1);
+    const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 y = two<T>(w[i]);
+      x[2 * i] = y.x, x[2 * i + 1] = y.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = one(src[un.o0 + i]);
+  }
+}
+
+__device__ __forceinline__ float turn_a(float a, float b, float c, float s) { return __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)); }
+__device__ __forceinline__ float turn_b(float a, float b, float c, float s) { return __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)); }
+
+// The unit's cosines and sines (kVec), eight of each.
+struct Turn {
+  float c[8], s[8];
+};
+__device__ __forceinline__ void load_turn(const float* row, int half, int u, Turn& t) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(row + 8 * u + i));
+    const float4 y = __ldg(reinterpret_cast<const float4*>(row + half + 8 * u + i));
+    t.c[i] = x.x, t.c[i + 1] = x.y, t.c[i + 2] = x.z, t.c[i + 3] = x.w;
+    t.s[i] = y.x, t.s[i + 1] = y.y, t.s[i + 2] = y.z, t.s[i + 3] = y.w;
+  }
+}
+__device__ __forceinline__ void turn_unit(bool interleaved, const Turn& t, float (&x)[16]) {
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {  // a pair's places in the unit
+    const float a = interleaved ? x[2 * i] : x[i], b = interleaved ? x[2 * i + 1] : x[8 + i];
+    const float ya = turn_a(a, b, t.c[i], t.s[i]), yb = turn_b(a, b, t.c[i], t.s[i]);
+    if (interleaved) y[2 * i] = ya, y[2 * i + 1] = yb;
+    else y[i] = ya, y[8 + i] = yb;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = y[i];
+}
+// Any sizes: 16 consecutive elements, each with its partner read by itself.
+template <typename T>
+__device__ __forceinline__ void turn_any(const Append8Args& a, const T* src, const float* row, int e0, float (&x)[16]) {
+  const int half = a.R / 2;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) {
+    const int e = e0 + i;
+    if (e >= a.R) break;
+    const int pair = a.interleaved ? e >> 1 : (e < half ? e : e - half);
+    const bool second = a.interleaved ? e & 1 : e >= half;
+    const int other = a.interleaved ? e ^ 1 : (second ? e - half : e + half);
+    const float c = __ldg(row + pair), s = __ldg(row + half + pair), mine = one(src[e]), its = one(src[other]);
+    const float y = second ? turn_b(its, mine, c, s) : turn_a(mine, its, c, s);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) x[k] = k == i ? y : x[k];
+  }
+}
+
+__device__ __forceinline__ const float* table_row(const Append8Args& a, int64_t t, bool report) {
+  int64_t pos = a.positions[t];
+  if (pos < 0 || pos >= a.P) {
+    if (report) record_error(a.err, ERR_POSITION);
+    pos = pos < 0 ? 0 : a.P - 1;
+  }
+  return a.table + pos * a.table_ld;
+}
+
+// The queries of the launch: a CTA takes tokens one after the other, a thread a unit of every `rows`-th head.
+template <typename T, bool kVec>
+__device__ __forceinline__ void queries(const Append8Args& a, int cta) {
+  const int wide = a.D / 16, rows = kAT / wide;
+  const int u = threadIdx.x % wide, r = threadIdx.x / wide;
+  const int part = cta % a.q_parts, first = cta / a.q_parts, step = a.q_ctas / a.q_parts;
+  const Unit un = unit_of<kVec>(a, u);
+  const bool turned = 16 * u < a.R;
+  for (int t = first; t < a.T; t += step) {
+    const float* row = table_row(a, t, part == 0 && threadIdx.x == 0);
+    Turn tn;
+    if (kVec && turned) load_turn(row, a.R / 2, u, tn);
+    for (int h0 = part * rows; h0 < a.Hq; h0 += a.q_parts * rows) {
+      const int h = h0 + r;
+      const bool live = h < a.Hq;
+      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
+      T* dst = reinterpret_cast<T*>(a.q_out) + (int64_t)t * a.o_st + (int64_t)h * a.o_sh;
+      float x[16];
+      if (live) {
+        load_unit<T, kVec>(src, un, x);
+        if (turned) {
+          if (kVec) turn_unit(a.interleaved, tn, x);
+          else turn_any(a, src, row, un.o0, x);
+        }
+      }
+      if (!kVec) __syncwarp();  // q may be turned in place, and a unit's partners are other lanes'
+      if (!live) continue;
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = round_two<T>(x[2 * i], x[2 * i + 1]);
+      if (kVec) {
+        *reinterpret_cast<uint4*>(dst + un.o0) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(dst + un.o1) = make_uint4(w[4], w[5], w[6], w[7]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint16_t bits = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+          reinterpret_cast<uint16_t*>(dst)[un.o0 + i] = bits;
+        }
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// Units of request b: numbers [off[b] / block + 2 b, off[b + 1] / block + 2 (b + 1)), at least as many as the blocks
+// that its tokens can touch wherever the context ends.  So a unit's request follows from the offsets alone.
+template <typename T, bool kVec, int kItems>
+__global__ void __launch_bounds__(kAT) append8_kernel(const __grid_constant__ Append8Args a) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  const int kv = a.kv_units * a.head_parts;
+  if ((int)blockIdx.x >= kv) {
+    queries<T, kVec>(a, blockIdx.x - kv);
+    pdl_trigger();
+    return;
+  }
+  const int unit = blockIdx.x / a.head_parts, part = blockIdx.x % a.head_parts;
+  int b = -1;
+  for (int b0 = 0; b0 < a.B; b0 += kAT) {
+    const int i = b0 + tid;
+    b += __syncthreads_count(i < a.B && a.node_offsets[i] / a.block + 2 * i <= unit);
+  }
+  __shared__ float amax_of[kAT / 32];
+  const int wide = a.D / 16;
+  const int per = kItems == 1 ? a.block * wide : kAT;  // threads of a head: a power of two, 64 at least
+  const int group = tid / per, at = tid % per;
+  const int head = part * (kAT / per) + group;  // keys' heads, then values'
+  const bool key = head < a.Hk;
+  const int h = key ? head : head - a.Hk;
+  const bool speaks = part == 0 && tid == 0;
+  if (b < 0) {  // ahead of the first request's units (offsets that start below 0)
+    pdl_trigger();
+    return;
+  }
+  const int n0 = a.node_offsets[b], n = a.node_offsets[b + 1] - n0, ctx = a.context_lens[b];
+  if (n0 < 0 || n < 0 || n > a.T - n0 || ctx < 0 || (int64_t)ctx + n > (int64_t)a.table_width * a.page_size) {
+    if (speaks) record_error(a.err, ERR_LENGTHS);
+    pdl_trigger();
+    return;
+  }
+  const int64_t j = ctx / a.block + unit - (n0 / a.block + 2 * b);  // block of the sequence
+  const int64_t start = j * a.block;
+  if (start >= (int64_t)ctx + n || n == 0) {
+    pdl_trigger();
+    return;
+  }
+  const int in_page = (int)(start % a.page_size);
+  const int page = a.page_table[(int64_t)b * a.pt_ld + start / a.page_size];
+  const bool there = page >= 0 && page < a.num_pages;
+  if (!there && speaks) record_error(a.err, ERR_PAGE);
+  const int kept = ctx > start ? (int)(ctx - start) : 0;  // places of the block in front of the first new one
+  const int64_t to_token = n0 + start - ctx;               // token at the block's first place
+  const int last = (int)min((int64_t)a.block, ctx + n - start);
+  const bool stores = there && head < 2 * a.Hk;
+  uint8_t* cache = reinterpret_cast<uint8_t*>(key ? a.k_cache : a.v_cache);
+  const int64_t* st = key ? a.kc_st : a.vc_st;
+  uint8_t* rows = cache + (int64_t)page * st[0] + (int64_t)in_page * st[1] + (int64_t)h * st[2];
+  float* scale_at = nullptr;
+  float old = 0.f;
+  if (stores) {
+    const int64_t* ss = key ? a.ks_st : a.vs_st;
+    scale_at = (key ? a.k_scale : a.v_scale) + (int64_t)page * ss[0] + (int64_t)(in_page / a.block) * ss[1] + (int64_t)h * ss[2];
+    if (kept > 0) old = *scale_at;
+  }
+  float x[kItems][16];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int r = (at + i * per) / wide, u = (at + i * per) % wide;
+    if (!stores || r < kept || r >= last) continue;
+    const int64_t t = to_token + r;
+    const T* src = reinterpret_cast<const T*>(key ? a.k : a.v) + t * (key ? a.k_st : a.v_st) + (int64_t)h * (key ? a.k_sh : a.v_sh);
+    const Unit un = unit_of<kVec>(a, u);
+    const bool turned = key && 16 * u < a.R;
+    load_unit<T, kVec>(src, un, x[i]);
+    if (turned) {
+      const float* row = table_row(a, t, h == 0 && u == 0);
+      if (kVec) {
+        Turn tn;
+        load_turn(row, a.R / 2, u, tn);
+        turn_unit(a.interleaved, tn, x[i]);
+      } else {
+        turn_any(a, src, row, un.o0, x[i]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float m = fabsf(x[i][e]);
+      amax = fmaxf(amax, m < INFINITY ? m : 0.f);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (lane == 0) amax_of[warp] = amax;
+  __syncthreads();
+  for (int w = group * per / 32; w < (group + 1) * per / 32; ++w) amax = fmaxf(amax, amax_of[w]);
+  float now = scale_for(amax);
+  float ratio = 1.f;
+  if (kept > 0) {
+    old = scale_or_least(old);
+    now = fmaxf(now, power_above(old));
+    ratio = old / now;
+  }
+  const float inv = 1.f / now;  // exact
+  if (stores) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int r = (at + i * per) / wide, u = (at + i * per) % wide;
+      if (r >= last) continue;
+      const Unit un = unit_of<kVec>(a, u);
+      uint2* d0 = reinterpret_cast<uint2*>(rows + (int64_t)r * st[1] + un.o0);
+      uint2* d1 = reinterpret_cast<uint2*>(rows + (int64_t)r * st[1] + un.o1);
+      if (r < kept) {
+        if (ratio == 1.f) continue;
+        uint2 y0 = *d0, y1 = *d1;
+        y0.x = e4m3_scaled(y0.x, ratio), y0.y = e4m3_scaled(y0.y, ratio);
+        y1.x = e4m3_scaled(y1.x, ratio), y1.y = e4m3_scaled(y1.y, ratio);
+        *d0 = y0, *d1 = y1;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[i][e] *= inv;
+        *d0 = make_uint2(e4m3_four(x[i]), e4m3_four(x[i] + 4));
+        *d1 = make_uint2(e4m3_four(x[i] + 8), e4m3_four(x[i] + 12));
+      }
+    }
+    if (at == 0) *scale_at = now;
+  }
+  pdl_trigger();
+}
+
+namespace {
+
+template <typename T, bool kVec>
+const void* append8_fn(int items) {
+  return items == 1 ? (const void*)append8_kernel<T, kVec, 1> : items == 2 ? (const void*)append8_kernel<T, kVec, 2>
+                                                                            : (const void*)append8_kernel<T, kVec, 4>;
+}
+
+}  // namespace
+
+int launch_append8(Append8Args a, cudaStream_t stream) {
+  const int units = a.block * (a.D / 16);  // 16-element units of a block and head: 64 to 1024
+  const int items = units <= kAT ? 1 : units / kAT, heads = units <= kAT ? kAT / units : 1;
+  a.kv_units = a.Hk ? a.T / a.block + 2 * a.B : 0;
+  a.head_parts = (2 * a.Hk + heads - 1) / heads;
+  // Few tokens: a token's query heads spread over CTAs; many: a CTA keeps its cosines and sines over them.
+  const int rows = kAT / (a.D / 16), spread = (a.Hq + rows - 1) / rows, want = 4 * num_sms();
+  a.q_parts = (want + a.T - 1) / a.T;
+  a.q_parts = a.q_parts < 1 ? 1 : a.q_parts > spread ? spread : a.q_parts;
+  const int tokens = a.T < 8192 ? a.T : 8192;
+  a.q_ctas = a.Hq ? tokens * a.q_parts : 0;
+  const int64_t grid = (int64_t)a.kv_units * a.head_parts + a.q_ctas;
+  const void* k = a.f16 ? (a.vectors ? append8_fn<__half, true>(items) : append8_fn<__half, false>(items))
+                        : (a.vectors ? append8_fn<__nv_bfloat16, true>(items) : append8_fn<__nv_bfloat16, false>(items));
+  return launch_with_pdl(k, a, (int)grid, kAT, 0, a.pdl, stream);
+}
+
+}  // namespace fnx

@@ -1387,16 +1387,17 @@ int fnx_tree_attention_workspace_floats(int64_t* floats) {
   return FNX_OK;
 }
 
-int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,
-                       const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
-                       int64_t num_pages, int page_size, const int32_t* page_table,
-                       int64_t table_ld, int table_width, const int32_t* context_lens,
-                       const int32_t* node_offsets, const uint64_t* tree_mask, void* out,
-                       int64_t o_sn, int64_t o_sh, float* lse, int batch, int nodes, int q_heads,
-                       int kv_heads, int dim, int max_nodes, int64_t max_context, float scale,
-                       int dtype, float* partials, int* error_flag, int pdl,
-                       fnx_stream_t stream) {
-  g_err.clear();
+namespace {
+
+// The checks of both tree attentions and their common arguments; none: there is nothing to do.
+int attn_shape_args(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,
+                    const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
+                    int64_t num_pages, int page_size, const int32_t* page_table, int64_t table_ld,
+                    int table_width, const int32_t* context_lens, const int32_t* node_offsets,
+                    const uint64_t* tree_mask, void* out, int64_t o_sn, int64_t o_sh, float* lse,
+                    int batch, int nodes, int q_heads, int kv_heads, int dim, int max_nodes,
+                    int64_t max_context, float scale, int dtype, float* partials, int* error_flag,
+                    int pdl, fnx::AttnArgs& a, bool& none) {
   if (!type16(dtype))
     return fail(FNX_EUNSUPPORTED, "tree attention: bf16 or fp16 only (dtype %d)", dtype);
   if (dim != 64 && dim != 128 && dim != 256)
@@ -1415,11 +1416,11 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
     return fail(FNX_EUNSUPPORTED, "tree attention: a GPU of %d SMs (at most %d)", fnx::num_sms(), fnx::kAttnMaxGrid);
   if (!(scale > 0.f) || scale > 3.0e38f)
     return fail(FNX_EINVAL, "tree attention: scale %g must be positive and finite", (double)scale);
-  if (nodes == 0) return FNX_OK;
+  none = nodes == 0;
+  if (none) return FNX_OK;
   if (batch < 1 || !q || !k_cache || !v_cache || !page_table || !context_lens || !node_offsets ||
       !out || !partials)
     return fail(FNX_EINVAL, "tree attention: null pointer");
-  fnx::AttnArgs a = {};
   if (!cache_strides(k_strides, a.kc_st) || !cache_strides(v_strides, a.vc_st))
     return fail(FNX_EINVAL, "tree attention: null cache strides");
   bool ok = aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16) &&
@@ -1453,47 +1454,342 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
   a.partials = partials;
   a.err = error_flag;
   a.pdl = pdl;
-  for (int b0 = 0; b0 < batch; b0 += fnx::kAttnMaxBatch) {  // requests of one launch
+  a.page_table = page_table;
+  a.context_lens = context_lens;
+  a.node_offsets = node_offsets;
+  return FNX_OK;
+}
+
+// The launches of a call, kAttnMaxBatch requests each.
+int attn_batches(fnx::AttnArgs& a, int batch, int (*launch)(const fnx::AttnArgs&, cudaStream_t), fnx_stream_t stream) {
+  const int *table = a.page_table, *lens = a.context_lens, *offsets = a.node_offsets;
+  for (int b0 = 0; b0 < batch; b0 += fnx::kAttnMaxBatch) {
     a.B = std::min(batch - b0, fnx::kAttnMaxBatch);
     a.head = b0 == 0;
     a.tail = b0 + a.B == batch;
-    a.page_table = page_table + (int64_t)b0 * table_ld;
-    a.context_lens = context_lens + b0;
-    a.node_offsets = node_offsets + b0;
-    if (launched([&] { return fnx::launch_tree_attn(a, static_cast<cudaStream_t>(stream)); }))
-      return cuda_fail("tree attention launch");
+    a.page_table = table + (int64_t)b0 * a.table_ld;
+    a.context_lens = lens + b0;
+    a.node_offsets = offsets + b0;
+    if (launched([&] { return launch(a, static_cast<cudaStream_t>(stream)); })) return cuda_fail("tree attention launch");
   }
   return FNX_OK;
 }
 
-int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const float* uniforms,
-               const float* temperature, const int32_t* top_k, const float* top_p,
-               const float* min_p, int64_t* tokens, float* probs, int pdl, fnx_stream_t stream) {
+}  // namespace
+
+int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,
+                       const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
+                       int64_t num_pages, int page_size, const int32_t* page_table,
+                       int64_t table_ld, int table_width, const int32_t* context_lens,
+                       const int32_t* node_offsets, const uint64_t* tree_mask, void* out,
+                       int64_t o_sn, int64_t o_sh, float* lse, int batch, int nodes, int q_heads,
+                       int kv_heads, int dim, int max_nodes, int64_t max_context, float scale,
+                       int dtype, float* partials, int* error_flag, int pdl,
+                       fnx_stream_t stream) {
   g_err.clear();
+  fnx::AttnArgs a = {};
+  bool none = false;
+  if (const int rc = attn_shape_args(q, q_sn, q_sh, k_cache, k_strides, v_cache, v_strides, num_pages, page_size,
+                                     page_table, table_ld, table_width, context_lens, node_offsets, tree_mask, out,
+                                     o_sn, o_sh, lse, batch, nodes, q_heads, kv_heads, dim, max_nodes, max_context,
+                                     scale, dtype, partials, error_flag, pdl, a, none))
+    return rc;
+  if (none) return FNX_OK;
+  return attn_batches(a, batch, fnx::launch_tree_attn, stream);
+}
+
+namespace {
+
+// What fnx_sample and fnx_token_probs have in common; FNX_OK with a.M == 0 where there is nothing to do.
+int sample_args(const char* what, const void* logits, int64_t ldl, int dtype, int M, int V,
+                const float* temperature, const int32_t* top_k, const float* top_p,
+                const float* min_p, int pdl, fnx::SampleArgs& a) {
   if (dtype != FNX_T_BF16 && dtype != FNX_T_F16 && dtype != FNX_T_F32)
-    return fail(FNX_EUNSUPPORTED, "sampling: bf16, fp16 or fp32 logits (dtype %d)", dtype);
+    return fail(FNX_EUNSUPPORTED, "%s: bf16, fp16 or fp32 logits (dtype %d)", what, dtype);
   if (M < 0 || V < 1 || ldl < V)
-    return fail(FNX_EINVAL, "sampling: bad logits shape M=%d V=%d ldl=%lld", M, V, (long long)ldl);
-  if (V > 1 << 21) return fail(FNX_EUNSUPPORTED, "sampling: V=%d (at most 2^21)", V);
-  if (M > 1 << 24) return fail(FNX_EUNSUPPORTED, "sampling: M=%d (at most 2^24)", M);
-  if (M == 0) return FNX_OK;
-  if (!logits || !uniforms || !tokens || !probs)
-    return fail(FNX_EINVAL, "sampling: null pointer");
-  fnx::SampleArgs a = {};
+    return fail(FNX_EINVAL, "%s: bad logits shape M=%d V=%d ldl=%lld", what, M, V, (long long)ldl);
+  if (V > 1 << 21) return fail(FNX_EUNSUPPORTED, "%s: V=%d (at most 2^21)", what, V);
+  if (M > 1 << 24) return fail(FNX_EUNSUPPORTED, "%s: M=%d (at most 2^24)", what, M);
   a.logits = logits;
   a.ldl = ldl;
   a.type = dtype;
   a.M = M;
   a.V = V;
-  a.uniforms = uniforms;
   a.temperature = temperature;
   a.top_k = top_k;
   a.top_p = top_p;
   a.min_p = min_p;
+  a.pdl = pdl;
+  return FNX_OK;
+}
+
+}  // namespace
+
+int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const float* uniforms,
+               const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, int64_t* tokens, float* probs, int pdl, fnx_stream_t stream) {
+  g_err.clear();
+  fnx::SampleArgs a = {};
+  if (const int rc = sample_args("sampling", logits, ldl, dtype, M, V, temperature, top_k, top_p, min_p, pdl, a)) return rc;
+  if (M == 0) return FNX_OK;
+  if (!logits || !uniforms || !tokens || !probs)
+    return fail(FNX_EINVAL, "sampling: null pointer");
+  a.uniforms = uniforms;
   a.tokens = tokens;
   a.probs = probs;
-  a.pdl = pdl;
   if (launched([&] { return fnx::launch_sample(a, static_cast<cudaStream_t>(stream)); })) return cuda_fail("sampling launch");
+  return FNX_OK;
+}
+
+int fnx_token_probs(const void* logits, int64_t ldl, int dtype, int M, int V,
+                    const float* temperature, const int32_t* top_k, const float* top_p,
+                    const float* min_p, float* probs, int64_t ldp, int pdl, fnx_stream_t stream) {
+  g_err.clear();
+  fnx::SampleArgs a = {};
+  if (const int rc = sample_args("token probabilities", logits, ldl, dtype, M, V, temperature, top_k, top_p, min_p, pdl, a)) return rc;
+  if (ldp < V) return fail(FNX_EINVAL, "token probabilities: rows of %d tokens %lld apart", V, (long long)ldp);
+  if (M == 0) return FNX_OK;
+  if (!logits || !probs) return fail(FNX_EINVAL, "token probabilities: null pointer");
+  a.all = probs;
+  a.ld_all = ldp;
+  if (launched([&] { return fnx::launch_token_probs(a, static_cast<cudaStream_t>(stream)); }))
+    return cuda_fail("token probabilities launch");
+  return FNX_OK;
+}
+
+namespace {
+
+// The shape of an 8-bit cache and its scales.
+int check_cache8(const char* what, int64_t num_pages, int page_size, int block, int dim) {
+  if (dim != 64 && dim != 128 && dim != 256)
+    return fail(FNX_EUNSUPPORTED, "%s: head size %d (64, 128 or 256)", what, dim);
+  if (block != 16 && block != 32 && block != 64)
+    return fail(FNX_EUNSUPPORTED, "%s: a scale for every %d tokens (16, 32 or 64)", what, block);
+  if (num_pages < 0 || page_size < 1 || page_size % block)
+    return fail(FNX_EINVAL, "%s: pages of %d tokens in blocks of %d", what, page_size, block);
+  return FNX_OK;
+}
+bool vec16(const int64_t (&st)[3]) { return st[0] % 16 == 0 && st[1] % 16 == 0 && st[2] % 16 == 0; }
+
+}  // namespace
+
+int fnx_rotary_append8(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                       int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out,
+                       int64_t o_st, int64_t o_sh, const int64_t* positions,
+                       const int32_t* context_lens, const int32_t* node_offsets,
+                       const int32_t* page_table, int64_t table_ld, int table_width,
+                       const float* table, int64_t rotary_ld, int64_t rotary_rows, void* k_cache,
+                       const int64_t* k_strides, void* v_cache, const int64_t* v_strides,
+                       float* k_scale, const int64_t* ks_strides, float* v_scale,
+                       const int64_t* vs_strides, int64_t num_pages, int page_size, int block,
+                       int batch, int tokens, int q_heads, int kv_heads, int dim, int rotated,
+                       int interleaved, int dtype, int* error_flag, int pdl, fnx_stream_t stream) {
+  g_err.clear();
+  if (!type16(dtype)) return fail(FNX_EUNSUPPORTED, "rotary: bf16 or fp16 only (dtype %d)", dtype);
+  if (const int rc = check_cache8("rotary", num_pages, page_size, block, dim)) return rc;
+  if (tokens < 0 || batch < 0 || q_heads < 0 || kv_heads < 1)
+    return fail(FNX_EINVAL, "rotary: bad shape tokens=%d batch=%d q_heads=%d kv_heads=%d", tokens, batch, q_heads, kv_heads);
+  if (rotated < 0 || rotated > dim || rotated % 2)
+    return fail(FNX_EINVAL, "rotary: rotated=%d must be even and at most dim=%d", rotated, dim);
+  if (table_width < 0 || rotary_rows < 1 || rotary_ld < rotated) return fail(FNX_EINVAL, "rotary: bad table shape");
+  if (tokens > 1 << 24) return fail(FNX_EUNSUPPORTED, "rotary: %d tokens (at most 2^24)", tokens);
+  if (batch > 1 << 16) return fail(FNX_EUNSUPPORTED, "rotary: %d requests (at most 2^16)", batch);
+  if (q_heads > 4096 || kv_heads > 1024) return fail(FNX_EUNSUPPORTED, "rotary: %d and %d heads", q_heads, kv_heads);
+  if (tokens == 0) return FNX_OK;
+  if (batch < 1 || (q_heads && (!q || !q_out)) || !k || !v || !k_cache || !v_cache || !k_scale || !v_scale || !positions ||
+      !context_lens || !node_offsets || !page_table || !table)
+    return fail(FNX_EINVAL, "rotary: null pointer");
+  fnx::Append8Args a = {};
+  if (!cache_strides(k_strides, a.kc_st) || !cache_strides(v_strides, a.vc_st) || !cache_strides(ks_strides, a.ks_st) ||
+      !cache_strides(vs_strides, a.vs_st))
+    return fail(FNX_EINVAL, "rotary: null cache strides");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !vec16(a.kc_st) || !vec16(a.vc_st))
+    return fail(FNX_EINVAL, "rotary: caches and their strides must be 16-byte aligned");
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_out = q_out;
+  a.q_st = q_st;
+  a.q_sh = q_sh;
+  a.k_st = k_st;
+  a.k_sh = k_sh;
+  a.v_st = v_st;
+  a.v_sh = v_sh;
+  a.o_st = o_st;
+  a.o_sh = o_sh;
+  a.positions = positions;
+  a.table = table;
+  a.table_ld = rotary_ld;
+  a.P = rotary_rows;
+  a.context_lens = context_lens;
+  a.node_offsets = node_offsets;
+  a.page_table = page_table;
+  a.pt_ld = table_ld;
+  a.num_pages = num_pages;
+  a.table_width = table_width;
+  a.page_size = page_size;
+  a.block = block;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.T = tokens;
+  a.B = batch;
+  a.Hq = q_heads;
+  a.Hk = kv_heads;
+  a.D = dim;
+  a.R = rotated;
+  a.interleaved = interleaved ? 1 : 0;
+  a.f16 = dtype == FNX_T_F16;
+  a.err = error_flag;
+  a.pdl = pdl;
+  bool ok = rotated % 16 == 0 && aligned(table, 16) && rotary_ld % 4 == 0 && aligned(q, 16) && aligned(k, 16) &&
+            aligned(v, 16) && aligned(q_out, 16);
+  for (int64_t st : {q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh}) ok = ok && vec8(st);
+  a.vectors = ok;
+  if (launched([&] { return fnx::launch_append8(a, static_cast<cudaStream_t>(stream)); })) return cuda_fail("rotary launch");
+  return FNX_OK;
+}
+
+int fnx_tree_attention8(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,
+                        const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
+                        const float* k_scale, const int64_t* ks_strides, const float* v_scale,
+                        const int64_t* vs_strides, int64_t num_pages, int page_size, int block,
+                        const int32_t* page_table, int64_t table_ld, int table_width,
+                        const int32_t* context_lens, const int32_t* node_offsets,
+                        const uint64_t* tree_mask, void* out, int64_t o_sn, int64_t o_sh,
+                        float* lse, int batch, int nodes, int q_heads, int kv_heads, int dim,
+                        int max_nodes, int64_t max_context, float scale, int dtype,
+                        float* partials, int* error_flag, int pdl, fnx_stream_t stream) {
+  g_err.clear();
+  fnx::Attn8Args a = {};
+  bool none = false;
+  if (const int rc = attn_shape_args(q, q_sn, q_sh, k_cache, k_strides, v_cache, v_strides, num_pages, page_size,
+                                     page_table, table_ld, table_width, context_lens, node_offsets, tree_mask, out,
+                                     o_sn, o_sh, lse, batch, nodes, q_heads, kv_heads, dim, max_nodes, max_context,
+                                     scale, dtype, partials, error_flag, pdl, a, none))
+    return rc;
+  if (const int rc = check_cache8("tree attention", num_pages, page_size, block, dim)) return rc;
+  if (none) return FNX_OK;
+  if (!k_scale || !v_scale) return fail(FNX_EINVAL, "tree attention: null pointer");
+  if (!cache_strides(ks_strides, a.ks_st) || !cache_strides(vs_strides, a.vs_st))
+    return fail(FNX_EINVAL, "tree attention: null cache strides");
+  if (!vec16(a.kc_st) || !vec16(a.vc_st))
+    return fail(FNX_EINVAL, "tree attention: rows and strides must be 16-byte aligned");
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.block = block;
+  return attn_batches(
+      a, batch,
+      [](const fnx::AttnArgs& x, cudaStream_t st) { return fnx::launch_tree_attn8(static_cast<const fnx::Attn8Args&>(x), st); },
+      stream);
+}
+
+int fnx_verify_tokens(const float* target, int64_t ldt, const float* draft, int64_t ldd,
+                      const int64_t* tokens, const int32_t* parents, const int32_t* node_offsets,
+                      const float* node_uniforms, const float* draw_uniforms, int batch, int nodes,
+                      int V, int max_nodes, int32_t* path, int32_t* accepted, int64_t* next,
+                      int* error_flag, int pdl, fnx_stream_t stream) {
+  g_err.clear();
+  if (batch < 0 || nodes < 0 || V < 1 || max_nodes < 1 || ldt < V || (draft && ldd < V))
+    return fail(FNX_EINVAL, "verification: bad shape batch=%d nodes=%d V=%d max_nodes=%d", batch, nodes, V, max_nodes);
+  if (max_nodes > 64) return fail(FNX_EUNSUPPORTED, "verification: %d nodes a request (at most 64)", max_nodes);
+  if (V > 1 << 21) return fail(FNX_EUNSUPPORTED, "verification: V=%d (at most 2^21)", V);
+  if (batch > 1 << 24) return fail(FNX_EUNSUPPORTED, "verification: %d requests (at most 2^24)", batch);
+  if (batch == 0) return FNX_OK;
+  if (!node_offsets || !draw_uniforms || !path || !accepted || !next ||
+      (nodes && (!target || !tokens || !parents || !node_uniforms)))
+    return fail(FNX_EINVAL, "verification: null pointer");
+  fnx::VerifyArgs a = {};
+  a.target = target;
+  a.draft = draft;
+  a.ldt = ldt;
+  a.ldd = ldd;
+  a.tokens = tokens;
+  a.parents = parents;
+  a.node_offsets = node_offsets;
+  a.node_uniforms = node_uniforms;
+  a.draw_uniforms = draw_uniforms;
+  a.path = path;
+  a.accepted = accepted;
+  a.next = next;
+  a.B = batch;
+  a.N = nodes;
+  a.V = V;
+  a.width = max_nodes;
+  a.err = error_flag;
+  a.pdl = pdl;
+  a.vectors = V % 4 == 0 && aligned(target, 16) && ldt % 4 == 0 && (!draft || (aligned(draft, 16) && ldd % 4 == 0));
+  if (launched([&] { return fnx::launch_verify(a, static_cast<cudaStream_t>(stream)); }))
+    return cuda_fail("verification launch");
+  return FNX_OK;
+}
+
+int fnx_compact_nodes(void* k_cache, const int64_t* k_strides, int64_t k_layer, void* v_cache,
+                      const int64_t* v_strides, int64_t v_layer, float* k_scale,
+                      const int64_t* ks_strides, int64_t ks_layer, float* v_scale,
+                      const int64_t* vs_strides, int64_t vs_layer, int64_t num_pages, int page_size,
+                      int block, int elem, int layers, int kv_heads, int dim,
+                      const int32_t* page_table, int64_t table_ld, int table_width,
+                      const int32_t* context_lens, const int32_t* path, int64_t path_ld,
+                      const int32_t* accepted, int batch, int width, int32_t* new_lens,
+                      int* error_flag, int pdl, fnx_stream_t stream) {
+  g_err.clear();
+  if (elem != 1 && elem != 2) return fail(FNX_EUNSUPPORTED, "compaction: elements of %d bytes (1 or 2)", elem);
+  if (elem == 1) {
+    if (const int rc = check_cache8("compaction", num_pages, page_size, block, dim)) return rc;
+  } else if (num_pages < 0 || page_size < 1 || dim < 1) {
+    return fail(FNX_EINVAL, "compaction: bad cache shape");
+  }
+  if (layers < 0 || kv_heads < 1 || table_width < 0 || batch < 0 || width < 0 || path_ld < width)
+    return fail(FNX_EINVAL, "compaction: bad shape layers=%d kv_heads=%d batch=%d width=%d", layers, kv_heads, batch, width);
+  if (width > 64) return fail(FNX_EUNSUPPORTED, "compaction: paths of %d nodes (at most 64)", width);
+  const int64_t bytes = (int64_t)kv_heads * dim * elem;
+  if (bytes > 1 << 20) return fail(FNX_EUNSUPPORTED, "compaction: %lld bytes a token (at most 2^20)", (long long)bytes);
+  if ((int64_t)batch * layers * 2 * ((bytes + 511) / 512) > 0x7FFFFFFF)
+    return fail(FNX_EUNSUPPORTED, "compaction: %d requests in %d layers", batch, layers);
+  if (batch == 0) return FNX_OK;
+  if (layers < 1) return fail(FNX_EINVAL, "compaction: no layers");
+  if (!k_cache || !v_cache || !page_table || !context_lens || (!path && width) || !accepted ||
+      (elem == 1 && (!k_scale || !v_scale)))
+    return fail(FNX_EINVAL, "compaction: null pointer");
+  fnx::CompactArgs a = {};
+  if (!cache_strides(k_strides, a.kc_st) || !cache_strides(v_strides, a.vc_st) ||
+      (elem == 1 && (!cache_strides(ks_strides, a.ks_st) || !cache_strides(vs_strides, a.vs_st))))
+    return fail(FNX_EINVAL, "compaction: null cache strides");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !vec16(a.kc_st) || !vec16(a.vc_st) || k_layer % 16 ||
+      v_layer % 16 || ((int64_t)dim * elem) % 16)
+    return fail(FNX_EINVAL, "compaction: heads, caches and strides must be 16-byte aligned");
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.k_layer = k_layer;
+  a.v_layer = v_layer;
+  if (elem == 1) {
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
+    a.ks_layer = ks_layer;
+    a.vs_layer = vs_layer;
+  }
+  a.page_table = page_table;
+  a.context_lens = context_lens;
+  a.path = path;
+  a.accepted = accepted;
+  a.pt_ld = table_ld;
+  a.path_ld = path_ld;
+  a.num_pages = num_pages;
+  a.new_lens = new_lens;
+  a.table_width = table_width;
+  a.page_size = page_size;
+  a.block = elem == 1 ? block : 1;
+  a.layers = layers;
+  a.B = batch;
+  a.Hk = kv_heads;
+  a.row_bytes = dim * elem;
+  a.width = width;
+  a.err = error_flag;
+  a.pdl = pdl;
+  if (launched([&] { return fnx::launch_compact(a, static_cast<cudaStream_t>(stream)); }))
+    return cuda_fail("compaction launch");
   return FNX_OK;
 }
 

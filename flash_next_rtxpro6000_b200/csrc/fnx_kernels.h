@@ -646,6 +646,72 @@ int64_t attn_workspace_floats();
 int launch_tree_attn(const AttnArgs& a, cudaStream_t stream);
 // The tensor-memory form; its grid and rows per item's slot are for the launch that joins the partials.
 int launch_tree_attn_tc(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows);
+// The launch that joins partial results of `rows` rows a slot that `grid` CTAs left.
+int launch_attn_join(const AttnArgs& a, cudaStream_t stream, int grid, int rows);
+
+// Over an 8-bit cache: strides in bytes, scales with their strides (elements) over pages, blocks and heads.
+struct Attn8Args : AttnArgs {
+  const float *k_scale, *v_scale;
+  int64_t ks_st[3], vs_st[3];
+  int block;
+};
+int launch_tree_attn8(const Attn8Args& a, cudaStream_t stream);
+int launch_tree_attn8_tc(const Attn8Args& a, cudaStream_t stream, int& grid, int& rows);
+
+struct Append8Args {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;  // strides over tokens and heads
+  const int64_t* positions;
+  const float* table;
+  int64_t table_ld, P;
+  const int *context_lens, *node_offsets, *page_table;
+  int64_t pt_ld, num_pages;
+  int table_width, page_size, block;
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  int64_t kc_st[3], vc_st[3];  // bytes, over pages, places and heads
+  int64_t ks_st[3], vs_st[3];  // elements, over pages, blocks and heads
+  int T, B, Hq, Hk, D, R;
+  int interleaved, f16;
+  int vectors;  // sizes and alignment allow 16-byte accesses
+  int* err;
+  int pdl;
+  int kv_units, head_parts, q_parts, q_ctas;  // set by the launch
+};
+int launch_append8(Append8Args a, cudaStream_t stream);
+
+struct CompactArgs {
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;      // null: a 16-bit cache
+  int64_t k_layer, v_layer, ks_layer, vs_layer;  // strides over layers
+  int64_t kc_st[3], vc_st[3];    // bytes, over pages, places and heads
+  int64_t ks_st[3], vs_st[3];    // elements, over pages, blocks and heads
+  const int *page_table, *context_lens, *path, *accepted;
+  int64_t pt_ld, path_ld, num_pages;
+  int* new_lens;
+  int table_width, page_size, block, layers, B, Hk, row_bytes;  // row_bytes: of a head
+  int width;  // of path
+  int* err;
+  int pdl;
+};
+int launch_compact(const CompactArgs& a, cudaStream_t stream);
+
+struct VerifyArgs {
+  const float *target, *draft;  // draft may be null
+  int64_t ldt, ldd;
+  const int64_t* tokens;
+  const int *parents, *node_offsets;
+  const float *node_uniforms, *draw_uniforms;
+  int *path, *accepted;
+  int64_t* next;
+  int B, N, V, width;
+  int* err;
+  int pdl;
+  int per;      // tokens of a CTA's slice, set by the launch
+  int vectors;  // rows are 16-byte aligned
+};
+int launch_verify(VerifyArgs a, cudaStream_t stream);
 
 enum LogitsType : int { LOGITS_BF16 = 0, LOGITS_F16 = 1, LOGITS_F32 = 2 };
 struct SampleArgs {
@@ -659,7 +725,10 @@ struct SampleArgs {
   int per;      // logits per CTA of a row's cluster
   int in_smem;  // they fit into its shared memory
   int pdl;
+  float* all;   // token_probs: the probabilities of all tokens, in rows ld_all apart
+  int64_t ld_all;
 };
 int launch_sample(SampleArgs a, cudaStream_t stream);
+int launch_token_probs(SampleArgs a, cudaStream_t stream);
 
 }  // namespace fnx

@@ -490,7 +490,10 @@ __device__ __forceinline__ Found answer(SampleSmem& s, const Scale& sc, const St
 }  // namespace
 
 // kMany: two CTAs on an SM, slices read from global memory (the L2 cache after the first time).
-template <typename T, bool kMany>
+// kAll: the probabilities of all tokens (token_probs).  The last token that is kept is the one that a random number of
+// 1 draws; once the first CTA has found it, every CTA writes its slice: a token's weight over that of all that are
+// kept where its key is not below the last one's, else 0.
+template <typename T, bool kMany, bool kAll>
 __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   SampleSmem& s = *reinterpret_cast<SampleSmem*>(smem);
@@ -503,7 +506,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   const int n = v0 >= a.V ? 0 : (a.V - v0 < a.per ? a.V - v0 : a.per);
   constexpr int kVec = 16 / sizeof(T);
   pdl_wait();
-  const float uniform = a.uniforms[row];
+  const float uniform = kAll ? 1.0f : a.uniforms[row];
   const float Tm = a.temperature ? a.temperature[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f,
               min_p = a.min_p ? a.min_p[row] : 0.0f;
   const int top_k = a.top_k ? a.top_k[row] : 0;
@@ -607,8 +610,27 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     low = fminf(low, o.low);
     floor = min(floor, o.floor);
   }
+  // Writes the slice's probabilities: f(logit, key) of each.
+  auto write = [&](auto&& f) {
+    float* out = a.all + (int64_t)row * a.ld_all + v0;
+    sweep([&](auto count, const float* x, int i0) {
+      float p[count];
+#pragma unroll
+      for (int q = 0; q < count; ++q) p[q] = f(x[q], v0 + i0 + q);
+      if (count > 1 && (reinterpret_cast<uintptr_t>(out + i0) & 15) == 0) {
+#pragma unroll
+        for (int q = 0; q + 3 < count; q += 4) *reinterpret_cast<float4*>(out + i0 + q) = make_float4(p[q], p[q + 1], p[q + 2], p[q + 3]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < count; ++q) out[i0 + q] = p[q];
+      }
+    });
+  };
   if (best == 0ull || !(Tm > 0.0f)) {  // nothing to draw from, or the most likely token
-    if (rank == 0 && tid == 0) {
+    if (kAll) {
+      const int only = best ? key_token(best) : -1;
+      write([&](float, int token) { return token == only ? 1.0f : 0.0f; });
+    } else if (rank == 0 && tid == 0) {
       a.tokens[row] = best ? key_token(best) : -1;
       a.probs[row] = best ? 1.0f : 0.0f;
     }
@@ -623,6 +645,48 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   sc.inv = sc.range > 0.0f ? (float)(kBins - 1) / sc.range : 0.0f;
   const bool use_p = top_p < 1.0f;
   sc.min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
+
+  // Writes the probabilities of the tokens from `last`'s key on, of which `kept` is the weight; 0 for the others.
+  auto write_kept = [&](u64 last, u64 kept) {
+    const float low = key_value(last);
+    const double inv = 1.0 / (double)kept;
+    write([&](float x, int token) {
+      if (!(x >= low) || (x == low && token > key_token(last))) return 0.0f;
+      return (float)((double)Scale::weight(sc.share(x)) * inv);
+    });
+  };
+  // Leaves the key of the last token kept, and their weight, where the cluster reads them (thread 0 of the first CTA).
+  auto last_key = [&](const Found& f) {
+    return make_key(logit(reinterpret_cast<const T*>(a.logits)[(int64_t)row * a.ldl + f.token]), (uint32_t)f.token);
+  };
+  if (kAll && top_k < 1 && !use_p) {  // all tokens, or those that min-p keeps: no order is needed
+    u64 kept = 0ull;
+    sweep([&](auto count, const float* x, int) {
+#pragma unroll
+      for (int q = 0; q < count; ++q) {
+        const float e = x[q] == sc.m || sc.m - x[q] <= sc.range ? sc.share(x[q]) : 0.0f;
+        if (e >= sc.min_p) kept += Scale::weight(e);
+      }
+    });
+    kept = warp_sum(kept);
+    if (lane == 0) s.red[warp] = kept;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kST / 32; ++w) kept += s.red[w];
+      s.mine.min_sum = kept;
+    }
+    cl.sync();
+    kept = 0ull;
+    for (int r = 0; r < C; ++r) kept += cl.map_shared_rank(&s, r)->mine.min_sum;
+    const double inv = 1.0 / (double)kept;
+    write([&](float x, int) {
+      const float e = x == sc.m || sc.m - x <= sc.range ? sc.share(x) : 0.0f;
+      return e >= sc.min_p ? (float)((double)Scale::weight(e) * inv) : 0.0f;
+    });
+    cl.sync();  // no CTA leaves while another reads its sum
+    pdl_trigger();
+    return;
+  }
 
   const double u = uniform > 0.0f ? (double)uniform : 0.0;  // NaN and negative numbers draw the most likely token
 
@@ -677,9 +741,15 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
           kept = want > 0.0 ? ask(WANT_SHARE, 0ull, want).sum : kOne;
         }
         if (sc.min_p > 0.0f) kept = by_share < kept ? by_share : kept;
-        draw(a, row, ask(WANT_SUM, target_of(u, kept), 0.0), kept);
+        const Found f = ask(WANT_SUM, target_of(u, kept), 0.0);
+        if (!kAll) draw(a, row, f, kept);
+        else if (tid == 0) s.ctl.key_lo = last_key(f), s.ctl.key_hi = kept;
       }
       cl.sync();  // the first CTA's count has been read by all before it leaves
+      if (kAll) {
+        write_kept(first.ctl.key_lo, first.ctl.key_hi);
+        cl.sync();
+      }
       pdl_trigger();
       return;
     }
@@ -952,25 +1022,26 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     kept = by_share < kept ? by_share : kept;
     const u64 target = target_of(u, kept);
     const int bt = bin_of(5, WANT_SUM, target, 0.0);
-    draw(a, row, held >= 0 ? from_list(bt, WANT_SUM, target, 0.0) : query(bt, WANT_SUM, target, 0.0), kept);
-    tell(Control{OP_DONE, 0, -1, 0, -1, 0ull, 0ull});
+    const Found f = held >= 0 ? from_list(bt, WANT_SUM, target, 0.0) : query(bt, WANT_SUM, target, 0.0);
+    if (!kAll) draw(a, row, f, kept);
+    tell(Control{OP_DONE, 0, -1, 0, -1, kAll && tid == 0 ? last_key(f) : 0ull, kAll ? kept : 0ull});
   }
+  if (kAll) write_kept(first.ctl.key_lo, first.ctl.key_hi);
   cl.sync();  // no CTA leaves while another reads its shared memory
   pdl_trigger();
 }
 
 namespace {
 
-template <bool kMany>
+template <bool kMany, bool kAll>
 const void* sample_fn(int type) {
-  if (type == LOGITS_F32) return (const void*)sample_kernel<float, kMany>;
-  if (type == LOGITS_F16) return (const void*)sample_kernel<__half, kMany>;
-  return (const void*)sample_kernel<__nv_bfloat16, kMany>;
+  if (type == LOGITS_F32) return (const void*)sample_kernel<float, kMany, kAll>;
+  if (type == LOGITS_F16) return (const void*)sample_kernel<__half, kMany, kAll>;
+  return (const void*)sample_kernel<__nv_bfloat16, kMany, kAll>;
 }
 
-}  // namespace
-
-int launch_sample(SampleArgs a, cudaStream_t stream) {
+template <bool kAll>
+int launch_rows(SampleArgs a, cudaStream_t stream) {
   const int size = a.type == LOGITS_F32 ? 4 : 2;
   // Rows for which clusters of 8 would not all run at once share the SMs two CTAs each, in clusters
   // of 4: 16 rows of 151,936 fp32 logits take 30 us in clusters of 8 and 50 in clusters of 4, 128
@@ -978,7 +1049,7 @@ int launch_sample(SampleArgs a, cudaStream_t stream) {
   // histogram's sums above 2^20.)
   const bool many = (int64_t)a.M * 8 > num_sms() && a.V <= 1 << 20;
   const int C = many ? 4 : 8;
-  const void* k = many ? sample_fn<true>(a.type) : sample_fn<false>(a.type);
+  const void* k = many ? sample_fn<true, kAll>(a.type) : sample_fn<false, kAll>(a.type);
   if (!prepare_kernel(k)) return 2;
   a.per = ((a.V + C - 1) / C + 15) / 16 * 16;
   const size_t fixed = (sizeof(SampleSmem) + 15) & ~(size_t)15;
@@ -1001,5 +1072,10 @@ int launch_sample(SampleArgs a, cudaStream_t stream) {
   void* params[1] = {&a};
   return cudaLaunchKernelExC(&cfg, k, params) == cudaSuccess ? 0 : 2;
 }
+
+}  // namespace
+
+int launch_sample(SampleArgs a, cudaStream_t stream) { return launch_rows<false>(a, stream); }
+int launch_token_probs(SampleArgs a, cudaStream_t stream) { return launch_rows<true>(a, stream); }
 
 }  // namespace fnx

@@ -535,20 +535,7 @@ int launch_form(const AttnArgs& a, cudaStream_t stream, int& grid, int& rows) {
 }
 
 template <typename T, int D>
-int launch_d(const AttnArgs& a, cudaStream_t stream) {
-  int grid = 0, rows = 0, rc;
-  const int most = a.max_nodes * a.group;
-  // The tensor-memory form needs some tiles a CTA to pay for its start-up and its row tiles of 128.  In
-  // key tiles an SM, times row tiles of 32: one token over 1,000 keys (0.2) 12.1 us here and 15.2 there,
-  // 4 requests of 16 nodes over 1,000 (7.4) 23.7 and 29.1, one token over 32k (7) 29.4 and 32.3, 8 nodes
-  // over 32k (14) 43.8 and 36.7, 16 nodes over 32k (28) 63.8 and 38.9, 16 requests of one token over 8k
-  // (111) 117 and 88.
-  const int64_t tiles = (int64_t)a.B * a.Hk * ((a.max_context + a.max_nodes + kKeyTile - 1) / kKeyTile);
-  if (tiles * ((most + 31) / 32) > 8 * num_sms()) rc = launch_tree_attn_tc(a, stream, grid, rows);
-  else if (most <= 16) rc = launch_form<T, D, 1, 4>(a, stream, grid, rows);
-  else if (most <= 32) rc = launch_form<T, D, 2, 4>(a, stream, grid, rows);
-  else rc = launch_form<T, D, 4, 2>(a, stream, grid, rows);
-  if (rc) return rc;
+int launch_join(const AttnArgs& a, cudaStream_t stream, int grid, int rows) {
   if (a.max_context + a.max_nodes <= kKeyTile) return 0;  // one key tile: no item is split
   cudaLaunchConfig_t cfg = {};
   const bool many = (int64_t)a.N * a.Hq >= 8 * num_sms();  // a row for each of eight warps an SM
@@ -566,6 +553,23 @@ int launch_d(const AttnArgs& a, cudaStream_t stream) {
   return cudaLaunchKernelExC(&cfg, k, params) == cudaSuccess ? 0 : 2;
 }
 
+template <typename T, int D>
+int launch_d(const AttnArgs& a, cudaStream_t stream) {
+  int grid = 0, rows = 0, rc;
+  const int most = a.max_nodes * a.group;
+  // The tensor-memory form needs some tiles a CTA to pay for its start-up and its row tiles of 128.  In
+  // key tiles an SM, times row tiles of 32: one token over 1,000 keys (0.2) 12.1 us here and 15.2 there,
+  // 4 requests of 16 nodes over 1,000 (7.4) 23.7 and 29.1, one token over 32k (7) 29.4 and 32.3, 8 nodes
+  // over 32k (14) 43.8 and 36.7, 16 nodes over 32k (28) 63.8 and 38.9, 16 requests of one token over 8k
+  // (111) 117 and 88.
+  const int64_t tiles = (int64_t)a.B * a.Hk * ((a.max_context + a.max_nodes + kKeyTile - 1) / kKeyTile);
+  if (tiles * ((most + 31) / 32) > 8 * num_sms()) rc = launch_tree_attn_tc(a, stream, grid, rows);
+  else if (most <= 16) rc = launch_form<T, D, 1, 4>(a, stream, grid, rows);
+  else if (most <= 32) rc = launch_form<T, D, 2, 4>(a, stream, grid, rows);
+  else rc = launch_form<T, D, 4, 2>(a, stream, grid, rows);
+  return rc ? rc : launch_join<T, D>(a, stream, grid, rows);
+}
+
 template <typename T>
 int launch_t(const AttnArgs& a, cudaStream_t stream) {
   if (a.D == 64) return launch_d<T, 64>(a, stream);
@@ -578,6 +582,12 @@ int launch_t(const AttnArgs& a, cudaStream_t stream) {
 int64_t attn_workspace_floats() {
   // the widest slots: 256 rows of 128, 128 rows of 256
   return 2ll * num_sms() * attn_slot_floats(256, 128);
+}
+
+int launch_attn_join(const AttnArgs& a, cudaStream_t stream, int grid, int rows) {
+  if (a.D == 64) return a.f16 ? launch_join<__half, 64>(a, stream, grid, rows) : launch_join<__nv_bfloat16, 64>(a, stream, grid, rows);
+  if (a.D == 128) return a.f16 ? launch_join<__half, 128>(a, stream, grid, rows) : launch_join<__nv_bfloat16, 128>(a, stream, grid, rows);
+  return a.f16 ? launch_join<__half, 256>(a, stream, grid, rows) : launch_join<__nv_bfloat16, 256>(a, stream, grid, rows);
 }
 
 int launch_tree_attn(const AttnArgs& a, cudaStream_t stream) {

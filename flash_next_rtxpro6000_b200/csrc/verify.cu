@@ -1,0 +1,328 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// A request's nodes form a tree: node 0 is its last token, row i of `target` the target's distribution p of the token
+// after node i, row i of `draft` the drafter's, q, that node i's children were drawn from.  The path starts at node 0.
+// At its end the children are asked in order, with r = p and S = 1 at first:
+//
+//   child with token x, random number u:   accepted  iff  u q(x) < r(x) / S    (it joins the path, and is its end)
+//   refused:                               r <- max(r / S - q, 0),  S <- sum r
+//
+// and without drafter probabilities (children chosen, not drawn: q is 1 at their token)
+//
+//   accepted  iff  u S < r(x);   refused:  S <- S - r(x),  r(x) <- 0.
+//
+// Then the next token is drawn from r by the request's own random number: the path's tokens and this one have the
+// target's distribution.  Values are held in 64-bit floating point with each operation rounded by itself, sums are of
+// whole numbers (trunc(2^52 r)), exact in any order: the split of a row changes nothing.  Where nothing is left (all
+// of r rounds to 0) r stays what it was.
+//
+// Bound: one read of the row at the path's end (of p, and of q where a child was refused there), since probabilities
+// of drafted tokens alone decide all else; for few requests, the chain of steps.  A cluster of CTAs has a request,
+// each a slice of the rows.  Every CTA walks the tree by itself, so the cluster only exchanges sums: one pass over
+// the slice for each refusal by q, whose sums also serve the final draw.  The token is found from the sums of CTAs,
+// then of warps, then by one more read of the 1/(8 x 16) of the row that holds it.
+#include <cooperative_groups.h>
+
+#include "fnx_common.cuh"
+#include "fnx_kernels.h"
+
+namespace fnx {
+
+namespace {
+
+namespace cg = cooperative_groups;
+using u64 = unsigned long long;
+
+constexpr int kVT = 512;             // threads
+constexpr int kVW = kVT / 32;        // warps
+constexpr int kNodes = 64;           // nodes of a request
+constexpr int kVCluster = 8;         // CTAs of a request
+constexpr int kTileV = 128;          // tokens of a warp's step: four a lane
+constexpr double kUnit = 4503599627370496.0;  // 2^52
+
+enum Step : int { STEP_PASS = 0, STEP_DRAW = 1 };
+
+struct VerifySmem {
+  int parent[kNodes];
+  int64_t token[kNodes];
+  double uniform[kNodes], p[kNodes], q[kNodes];  // of the node's token, in its parent's rows
+  double inv[kNodes];      // 1 / S of the refusals at the path's end
+  int refused[kNodes];     // their tokens (without drafter probabilities)
+  int path[kNodes];
+  u64 warp_sum[kVW];       // of the last pass
+  u64 total[2];            // this CTA's, of the last passes
+  u64 tile_sum[kTileV];    // of the warp's part that holds the token
+  // the walk
+  int i, current, length, rounds, kept_rounds, step;
+  bool summed;             // the last pass was over what is left now
+  double left;             // S
+};
+
+__device__ __forceinline__ double probability(float v) { return v > 0.f ? (double)fminf(v, 1.f) : 0.0; }
+__device__ __forceinline__ u64 whole(double r) { return (u64)__double2ull_rz(__dmul_rn(r, kUnit)); }
+
+__device__ __forceinline__ double residual(const double* inv, int rounds, double p, double q) {
+  for (int k = 0; k < rounds; ++k) p = fmax(__dsub_rn(__dmul_rn(p, inv[k]), q), 0.0);
+  return p;
+}
+
+__device__ __forceinline__ u64 warp_total(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Four tokens' probabilities, zeros past `end`.
+template <bool kVec>
+__device__ __forceinline__ float4 four(const float* row, int v, int end) {
+  if (kVec) return v < end ? __ldg(reinterpret_cast<const float4*>(row + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 x;
+  x.x = v < end ? __ldg(row + v) : 0.f;
+  x.y = v + 1 < end ? __ldg(row + v + 1) : 0.f;
+  x.z = v + 2 < end ? __ldg(row + v + 2) : 0.f;
+  x.w = v + 3 < end ? __ldg(row + v + 3) : 0.f;
+  return x;
+}
+
+}  // namespace
+
+template <bool kVec>
+__global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ VerifySmem s;
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank();
+  const int b = blockIdx.x / kVCluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  const int n0 = a.node_offsets[b], n = a.node_offsets[b + 1] - n0;
+  const bool bad = n0 < 0 || n < 0 || n > a.width || n > a.N - n0;
+  if (bad || n == 0) {  // the cluster's CTAs all leave here
+    if (rank == 0) {
+      if (tid < a.width) a.path[(int64_t)b * a.width + tid] = -1;
+      if (tid == 0) {
+        a.accepted[b] = 0;
+        a.next[b] = -1;
+        if (bad) record_error(a.err, ERR_LENGTHS);
+      }
+    }
+    pdl_trigger();
+    return;
+  }
+  if (tid < n) {
+    const int parent = tid ? a.parents[n0 + tid] : -1;
+    const int64_t x = a.tokens[n0 + tid];
+    const bool known = parent >= 0 && parent < tid, word = x >= 0 && x < a.V;
+    double p = 0.0, q = 0.0;
+    if (known && word) {
+      p = probability(a.target[(int64_t)(n0 + parent) * a.ldt + x]);
+      q = a.draft ? probability(a.draft[(int64_t)(n0 + parent) * a.ldd + x]) : 1.0;
+    }
+    if (rank == 0 && tid > 0) {
+      if (!known && parent != -1) record_error(a.err, ERR_TREE);
+      if (known && !word) record_error(a.err, ERR_TOKEN);
+    }
+    s.parent[tid] = known ? parent : -1;
+    s.token[tid] = word ? x : -1;
+    s.uniform[tid] = (double)a.node_uniforms[n0 + tid];
+    s.p[tid] = p;
+    s.q[tid] = q;
+  }
+  if (tid == 0) {
+    s.i = 1;
+    s.current = 0;
+    s.length = 1;
+    s.rounds = 0;
+    s.left = 1.0;
+    s.summed = false;
+    s.path[0] = 0;
+  }
+  __syncthreads();
+
+  const int v0 = rank * a.per + warp * (a.per / kVW);          // the warp's part of the row
+  const int v1 = min(a.V, v0 + a.per / kVW);
+  int phase = 0;
+  // Sums of what `rounds` refusals leave of the current row: the warps', the CTA's and the cluster's.
+  auto pass = [&](int rounds) {
+    const float* prow = a.target + (int64_t)(n0 + s.current) * a.ldt;
+    const float* qrow = a.draft ? a.draft + (int64_t)(n0 + s.current) * a.ldd : nullptr;
+    u64 sum = 0;
+    if (a.draft && rounds > 0) {
+#pragma unroll 4
+      for (int v = v0 + lane * 4; v < v1; v += kTileV) {
+        const float4 p = four<kVec>(prow, v, v1), q = four<kVec>(qrow, v, v1);
+        sum += whole(residual(s.inv, rounds, probability(p.x), probability(q.x)));
+        sum += whole(residual(s.inv, rounds, probability(p.y), probability(q.y)));
+        sum += whole(residual(s.inv, rounds, probability(p.z), probability(q.z)));
+        sum += whole(residual(s.inv, rounds, probability(p.w), probability(q.w)));
+      }
+    } else {
+#pragma unroll 4
+      for (int v = v0 + lane * 4; v < v1; v += kTileV) {
+        const float4 p = four<kVec>(prow, v, v1);
+        sum += whole(probability(p.x)) + whole(probability(p.y)) + whole(probability(p.z)) + whole(probability(p.w));
+      }
+      if (!a.draft && lane < rounds) {  // refused tokens' shares are taken out again
+        for (int k = lane; k < rounds; k += 32)
+          if (s.refused[k] >= v0 && s.refused[k] < v1) sum -= whole(probability(prow[s.refused[k]]));
+      }
+    }
+    sum = warp_total(sum);
+    __syncthreads();
+    if (lane == 0) s.warp_sum[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      u64 all = 0;
+      for (int w = 0; w < kVW; ++w) all += s.warp_sum[w];
+      s.total[phase] = all;
+    }
+    cl.sync();
+    u64 all = 0;
+#pragma unroll
+    for (int c = 0; c < kVCluster; ++c) all += cl.map_shared_rank(&s, c)->total[phase];
+    phase ^= 1;
+    return all;
+  };
+
+  for (;;) {
+    if (tid == 0) {
+      int step = STEP_DRAW;
+      for (; s.i < n; ++s.i) {
+        const int i = s.i;
+        if (s.parent[i] != s.current) continue;
+        bool accept;
+        if (a.draft) {
+          const double inv = __drcp_rn(s.left);
+          const double r = residual(s.inv, s.rounds, s.p[i], s.q[i]);
+          accept = __dmul_rn(s.uniform[i], s.q[i]) < __dmul_rn(r, inv);
+          if (!accept) {
+            s.inv[s.rounds] = inv;
+            step = STEP_PASS;
+          }
+        } else {
+          double r = s.p[i];
+          for (int k = 0; k < s.rounds; ++k)
+            if (s.refused[k] == (int)s.token[i]) r = 0.0;
+          accept = __dmul_rn(s.uniform[i], s.left) < r;
+          if (!accept && r > 0.0) {
+            s.left = fmax(__dsub_rn(s.left, r), 0.0);
+            s.refused[s.rounds++] = (int)s.token[i];
+          }
+        }
+        if (accept) {
+          s.path[s.length++] = i;
+          s.current = i;
+          s.rounds = 0;
+          s.left = 1.0;
+          s.summed = false;
+        }
+        if (step == STEP_PASS) break;
+      }
+      s.step = step;
+    }
+    __syncthreads();
+    if (s.step == STEP_DRAW) break;
+    const u64 all = pass(s.rounds + 1);
+    if (tid == 0) {
+      ++s.i;
+      s.summed = all > 0;
+      if (all > 0) {
+        ++s.rounds;
+        s.left = __dmul_rn(__ull2double_rn(all), 1.0 / kUnit);
+      }
+    }
+    __syncthreads();
+  }
+  // --- the draw
+  if (!s.summed) pass(s.rounds);
+  u64 before = 0, all = 0;
+  const u64 mine = s.total[phase ^ 1];
+  for (int c = 0; c < kVCluster; ++c) {
+    const u64 t = cl.map_shared_rank(&s, c)->total[phase ^ 1];
+    if (c < rank) before += t;
+    all += t;
+  }
+  if (rank == 0) {
+    if (tid < a.width) a.path[(int64_t)b * a.width + tid] = tid < s.length ? s.path[tid] : -1;
+    if (tid == 0) {
+      a.accepted[b] = s.length;
+      if (all == 0) a.next[b] = -1;
+    }
+  }
+  if (all > 0) {
+    const float given = a.draw_uniforms[b];
+    const double u = given > 0.f ? (double)given : 0.0;  // NaN and negative numbers draw the first token
+    const u64 reach = __double2ull_rz(__dmul_rn(u, __ull2double_rn(all)));
+    const u64 aim = reach < all - 1 ? reach : all - 1;
+    if (aim >= before && aim < before + mine) {  // the CTA has the token
+      int w = 0;
+      while (w < kVW - 1 && aim >= before + s.warp_sum[w]) before += s.warp_sum[w++];
+      const int p0 = rank * a.per + w * (a.per / kVW), p1 = min(a.V, p0 + a.per / kVW);
+      const float* prow = a.target + (int64_t)(n0 + s.current) * a.ldt;
+      const float* qrow = a.draft ? a.draft + (int64_t)(n0 + s.current) * a.ldd : nullptr;
+      const bool pairs = a.draft && s.rounds > 0;
+      auto weights = [&](int v, u64 (&x)[4]) {
+        const float4 p = four<kVec>(prow, v, p1);
+        const float4 q = pairs ? four<kVec>(qrow, v, p1) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float ps[4] = {p.x, p.y, p.z, p.w}, qs[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = whole(pairs ? residual(s.inv, s.rounds, probability(ps[e]), probability(qs[e])) : probability(ps[e]));
+          if (!a.draft)
+            for (int k = 0; k < s.rounds; ++k)
+              if (s.refused[k] == v + e) x[e] = 0;
+        }
+      };
+      const int tiles = (p1 - p0 + kTileV - 1) / kTileV;  // at most kTileV: 2^21 tokens over 8 x 16 x 128
+      for (int t = warp; t < tiles; t += kVW) {
+        u64 x[4];
+        weights(p0 + t * kTileV + lane * 4, x);
+        const u64 sum = warp_total(x[0] + x[1] + x[2] + x[3]);
+        if (lane == 0) s.tile_sum[t] = sum;
+      }
+      __syncthreads();  // of the CTA alone: the condition is the same for all of its threads
+      if (warp == 0) {
+        int t = 0;
+        while (t < tiles - 1 && aim >= before + s.tile_sum[t]) before += s.tile_sum[t++];
+        const int v = p0 + t * kTileV + lane * 4;
+        u64 x[4];
+        weights(v, x);
+        const u64 own = x[0] + x[1] + x[2] + x[3];
+        u64 sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += y;
+        }
+        u64 run = before + sum - own;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (aim >= run && aim < run + x[e]) a.next[b] = v + e;
+          run += x[e];
+        }
+      }
+    }
+  }
+  cl.sync();  // no CTA leaves while another reads its sums
+  pdl_trigger();
+}
+
+int launch_verify(VerifyArgs a, cudaStream_t stream) {
+  a.per = (a.V + kVCluster * kVW * kTileV - 1) / (kVCluster * kVW * kTileV) * (kVW * kTileV);
+  const void* k = a.vectors ? (const void*)verify_kernel<true> : (const void*)verify_kernel<false>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.B * kVCluster);
+  cfg.blockDim = dim3(kVT);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kVCluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.pdl ? 2 : 1;
+  void* params[1] = {&a};
+  return cudaLaunchKernelExC(&cfg, k, params) == cudaSuccess ? 0 : 2;
+}
+
+}  // namespace fnx

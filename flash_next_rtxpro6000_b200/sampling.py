@@ -2,8 +2,9 @@
 numbers (csrc/sample.cu).
 
 ``sample_tokens`` stands where the greedy argmax of ``w8a16_gemv`` or ``draft_topk1_postprocess``
-would: one token per row of logits, for every node of a verify pass in one launch.  No counterpart in
-the reference's operator modules.
+would: one token per row of logits, for every node of a verify pass in one launch.  ``token_probs`` gives
+the probabilities that it draws from, which ``verify_tokens`` takes.  No counterpart in the reference's
+operator modules.
 """
 
 from __future__ import annotations
@@ -38,3 +39,18 @@ def sample_tokens(
     numbers, so results are the same bit for bit from call to call."""
     return _lib.ops().sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p,
                                     PDL if pdl is None else pdl)
+
+
+def token_probs(
+    logits: torch.Tensor,
+    temperature: Optional[torch.Tensor] = None,
+    top_k: Optional[torch.Tensor] = None,
+    top_p: Optional[torch.Tensor] = None,
+    min_p: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    pdl: Optional[bool] = None,
+) -> torch.Tensor:
+    """fp32 [M, V] (in ``out``, which must not overlap logits): the probabilities from which ``sample_tokens``
+    draws with the same arguments -- each kept token's weight over that of all kept tokens, 0 for the others.
+    Temperature 0 gives 1 to the first token; a row without a logit above -inf is zeros."""
+    return _lib.ops().token_probs(logits, temperature, top_k, top_p, min_p, out, PDL if pdl is None else pdl)

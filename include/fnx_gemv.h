@@ -95,6 +95,8 @@ typedef void* fnx_stream_t;
 #define FNX_DEVERR_LENGTHS 14      /* lengths that contradict each other or the bounds */
 #define FNX_DEVERR_PAGE 15         /* a page number outside the cache                 */
 #define FNX_DEVERR_TREE 16         /* a parent that is not an earlier node            */
+#define FNX_DEVERR_TOKEN 17        /* a drafted token outside the vocabulary          */
+#define FNX_DEVERR_SCALE 18        /* a cache scale that no append writes             */
 
 /* Split-K and argmax scratch of the dense GEMVs.  Counters and keys must be zero when
  * first used; every launch leaves them zero again (self-resetting, graph-replay safe).
@@ -538,6 +540,106 @@ int fnx_tree_attention(const void* q, int64_t q_sn, int64_t q_sh, const void* k_
 int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const float* uniforms,
                const float* temperature, const int32_t* top_k, const float* top_p,
                const float* min_p, int64_t* tokens, float* probs, int pdl, fnx_stream_t stream);
+
+/*
+ * The probabilities that fnx_sample draws from: probs fp32 [M, V] (row stride ldp >= V), for each
+ * token its weight over that of all tokens that top-k, top-p and min-p keep, 0 for the others; a
+ * row at temperature <= 0 has a 1 at its first token, a row without a logit above -inf zeros.
+ */
+int fnx_token_probs(const void* logits, int64_t ldl, int dtype, int M, int V,
+                    const float* temperature, const int32_t* top_k, const float* top_p,
+                    const float* min_p, float* probs, int64_t ldp, int pdl, fnx_stream_t stream);
+
+/*
+ * The 8-bit paged cache: k_cache and v_cache [num_pages, page_size, kv_heads, dim] e4m3 bytes, strides
+ * (bytes) over pages, places and heads; k_scale and v_scale fp32 [num_pages, page_size / block,
+ * kv_heads], strides (elements) over pages, blocks and heads; an element is its byte's value times
+ * its block's scale.  block 16, 32 or 64, page_size a multiple of it; dim 64, 128 or 256; caches and
+ * their strides 16-byte aligned.
+ *
+ * fnx_rotary_append8: as fnx_rotary_append, with request b's tokens (rows node_offsets[b] ..
+ * node_offsets[b + 1] - 1, any number) stored at places context_lens[b] + index of its pages.  A
+ * block that gets tokens has the scale s' = the smallest power of two, 2^-40 at least, by which the
+ * largest finite magnitude of its new elements divided is at most 448, and not below the block's old
+ * scale where tokens of the context stay in it, which take the new scale too.  Elements are rounded
+ * to the nearest, infinite ones and NaN to NaN.  Rows of no request are rotated and not stored.
+ * Lengths that contradict each other or the table record FNX_DEVERR_LENGTHS, pages outside the cache
+ * FNX_DEVERR_PAGE: nothing is stored there.  No block may belong to two requests of a call.  At most
+ * 2^24 tokens and 2^16 requests.
+ */
+int fnx_rotary_append8(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                       int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out,
+                       int64_t o_st, int64_t o_sh, const int64_t* positions,
+                       const int32_t* context_lens, const int32_t* node_offsets,
+                       const int32_t* page_table, int64_t table_ld, int table_width,
+                       const float* table, int64_t rotary_ld, int64_t rotary_rows, void* k_cache,
+                       const int64_t* k_strides, void* v_cache, const int64_t* v_strides,
+                       float* k_scale, const int64_t* ks_strides, float* v_scale,
+                       const int64_t* vs_strides, int64_t num_pages, int page_size, int block,
+                       int batch, int tokens, int q_heads, int kv_heads, int dim, int rotated,
+                       int interleaved, int dtype, int* error_flag, int pdl, fnx_stream_t stream);
+
+/* fnx_tree_attention over an 8-bit cache.  Scales that fnx_rotary_append8 does not write (not in
+ * [2^-40, 2^120]; others need not be powers of two) record FNX_DEVERR_SCALE and count as 2^-40.  The
+ * scales of the values that a row sees should lie within a factor of 2^60 of each other. */
+int fnx_tree_attention8(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache,
+                        const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
+                        const float* k_scale, const int64_t* ks_strides, const float* v_scale,
+                        const int64_t* vs_strides, int64_t num_pages, int page_size, int block,
+                        const int32_t* page_table, int64_t table_ld, int table_width,
+                        const int32_t* context_lens, const int32_t* node_offsets,
+                        const uint64_t* tree_mask, void* out, int64_t o_sn, int64_t o_sh,
+                        float* lse, int batch, int nodes, int q_heads, int kv_heads, int dim,
+                        int max_nodes, int64_t max_context, float scale, int dtype,
+                        float* partials, int* error_flag, int pdl, fnx_stream_t stream);
+
+/*
+ * Verification of drafted trees.  Request b's nodes are rows node_offsets[b] .. node_offsets[b + 1]
+ * - 1 (at most max_nodes <= 64) of target (fp32 [nodes, V], row stride ldt): row i the target's
+ * distribution of the token after node i.  draft (row stride ldd; may be NULL): row i the
+ * distribution that node i's children were drawn from, independently of each other.  tokens int64
+ * [nodes], parents int32 [nodes] (as in fnx_tree_layout; node 0 is the request's last token and
+ * starts the path).  The children of the path's end are asked in order, with r = target's row and
+ * S = 1 at first: token x with node_uniforms u is accepted where u q(x) < r(x) / S, and becomes the
+ * path's end; else r = max(r / S - q, 0), S = sum r.  With draft NULL: accepted where u S < r(x),
+ * else S -= r(x), r(x) = 0.  Then next[b] is drawn from r, in the order of tokens, by
+ * draw_uniforms[b].  Sums are of whole numbers (2^52 r, truncated): results are the same bit for
+ * bit from call to call.  Probabilities count as within [0, 1], NaN as 0; where nothing is left r
+ * stays what it was.
+ *  path int32 [batch, max_nodes]: the accepted nodes' indices, node 0 first, then -1; accepted int32
+ *  [batch]: their number; next int64 [batch].  A request without nodes: 0 accepted, next -1; next is
+ *  -1 too where the row at the path's end is zeros.  rows of probabilities 2^21 wide at most.
+ * A parent that is not an earlier node records FNX_DEVERR_TREE (such nodes are not asked; -1 is no
+ * error), a token outside the vocabulary FNX_DEVERR_TOKEN (refused), lengths outside the bounds
+ * FNX_DEVERR_LENGTHS (as without nodes).
+ */
+int fnx_verify_tokens(const float* target, int64_t ldt, const float* draft, int64_t ldd,
+                      const int64_t* tokens, const int32_t* parents, const int32_t* node_offsets,
+                      const float* node_uniforms, const float* draw_uniforms, int batch, int nodes,
+                      int V, int max_nodes, int32_t* path, int32_t* accepted, int64_t* next,
+                      int* error_flag, int pdl, fnx_stream_t stream);
+
+/*
+ * The accepted nodes' keys and values moved behind their contexts: for d < accepted[b], what lies at
+ * place context_lens[b] + path[b][d] goes to place context_lens[b] + d, as if everything were read
+ * first, in `layers` caches (k_layer and v_layer bytes apart) of one page table.  path int32 [batch,
+ * width <= 64] rises from 0 on.  new_lens int32 [batch] (may be NULL): context_lens + accepted.
+ * elem 2: 16-bit caches as in fnx_rotary_append (strides in bytes; scales NULL).  elem 1: 8-bit
+ * caches (scales ks_layer and vs_layer elements apart): a block's scale becomes the largest of those
+ * of the tokens that come to it and, where tokens of the context stay in it, its own; elements whose
+ * scale changes are rounded again.  kv_heads * dim * elem at most 2^20; heads, caches and strides
+ * 16-byte aligned.  A path that does not rise, or reaches past the pages, records FNX_DEVERR_TREE or
+ * FNX_DEVERR_LENGTHS, a page outside the cache FNX_DEVERR_PAGE; the request is left as it was.
+ */
+int fnx_compact_nodes(void* k_cache, const int64_t* k_strides, int64_t k_layer, void* v_cache,
+                      const int64_t* v_strides, int64_t v_layer, float* k_scale,
+                      const int64_t* ks_strides, int64_t ks_layer, float* v_scale,
+                      const int64_t* vs_strides, int64_t vs_layer, int64_t num_pages, int page_size,
+                      int block, int elem, int layers, int kv_heads, int dim,
+                      const int32_t* page_table, int64_t table_ld, int table_width,
+                      const int32_t* context_lens, const int32_t* path, int64_t path_ld,
+                      const int32_t* accepted, int batch, int width, int32_t* new_lens,
+                      int* error_flag, int pdl, fnx_stream_t stream);
 
 /* Description of the last error of the calling thread ("" if none). */
 const char* fnx_last_error(void);
