@@ -25,27 +25,31 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int D, int MT, int WK>
+// MT row tiles of 16; WK warps share a row tile and a key tile; TG sets of these take key tiles in turn.
+template <int D, int MT, int WK, int TG>
 struct Attn8Cfg {
-  static constexpr int kThreads = 32 * MT * WK;
+  static constexpr int kThreads = 32 * MT * WK * TG;
   static constexpr int kRows = 16 * MT;
   static constexpr int kUnits = D / 16;             // 16-byte units of a key
   static constexpr int kTileBytes = kKeyTile * D;   // keys or values of one tile
-  static constexpr int kStages = D == 256 ? 4 : D == 128 ? 6 : 8;
+  static constexpr int kStages = (D == 256 ? 4 : D == 128 ? 8 : 12) / TG;  // of TG tiles
+  static constexpr int kParts = WK * TG;            // warps that share a row tile
+  static constexpr int kPass = kThreads / kUnits;   // rows that the block copies at a time
+  static_assert(kPass % kGroup == 0 || kPass == 8, "a thread's rows have one place in their groups, or two");
   static constexpr int kKeys = kKeyTile / WK;       // keys of a tile per warp
   static constexpr int kJoinRow = D + 4;            // floats; pads the rows apart
-  static_assert((WK - 1) * MT * 16 * (kJoinRow + 2) * 4 <= kStages * 2 * kTileBytes, "join area");
+  static_assert((kParts - 1) * MT * 16 * (kJoinRow + 2) * 4 <= kStages * TG * 2 * kTileBytes, "join area");
   static_assert(kKeys % kGroup == 0, "a warp has whole groups");
   struct Smem {
-    alignas(128) uint8_t ring[kStages][2][kTileBytes];
+    alignas(128) uint8_t ring[kStages][2][TG * kTileBytes];
     alignas(128) uint8_t q[kRows * D * 2];
-    float4 scales[kStages + 2][kKeyTile / kGroup];
-    int64_t place[2][2][kKeyTile];  // byte offsets of a tile's keys and values
+    float2 scales[kStages][TG * kKeyTile / kGroup];  // of the ring's groups: keys', values'
+    Place8 place[2][TG * kKeyTile / kGroup];         // of a stage's groups, which one page and one block hold each
     unsigned long long mask[kRows];
     long long before[kAttnMaxBatch + 1];
     long long scratch[32];
     float factor[kRows];  // of a row's scores
-    uint32_t odd[2];      // drafted tokens of a tile with NaN values
+    uint32_t odd[TG][2];  // drafted tokens of a tile with NaN values
   };
   // Places of 16-byte units in their rows, so that the eight lanes of one access meet eight different ones modulo
   // 128 bytes: two keys times four units of 16 for the scores, eight keys for the values.
@@ -55,16 +59,16 @@ struct Attn8Cfg {
 
 }  // namespace
 
-template <typename T, int D, int MT, int WK>
-__global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __grid_constant__ Attn8Args a) {
-  using Cfg = Attn8Cfg<D, MT, WK>;
+template <typename T, int D, int MT, int WK, int TG>
+__global__ void __launch_bounds__(32 * MT * WK * TG, 1) tree_attn8_kernel(const __grid_constant__ Attn8Args a) {
+  using Cfg = Attn8Cfg<D, MT, WK, TG>;
   constexpr int kRows = Cfg::kRows, kStages = Cfg::kStages, kKeys = Cfg::kKeys, kThreads = Cfg::kThreads;
-  constexpr int kUnits = Cfg::kUnits, kGroups = kKeys / kGroup, kSets = kStages + 2;
+  constexpr int kUnits = Cfg::kUnits, kGroups = kKeys / kGroup;
   constexpr bool kHold = D <= 128;  // the queries' operands stay in registers
   extern __shared__ __align__(128) uint8_t raw[];
   typename Cfg::Smem& s = *reinterpret_cast<typename Cfg::Smem*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wr = warp / WK, wk = warp % WK;
+  const int tg = warp / (MT * WK), wr = warp / WK % MT, wk = warp % WK;
   const uint8_t* kc = reinterpret_cast<const uint8_t*>(a.k_cache);
   const uint8_t* vc = reinterpret_cast<const uint8_t*>(a.v_cache);
   const float c2 = a.scale * 1.4426950408889634f;  // scores in base-2 units
@@ -90,33 +94,41 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
     const int t0 = (int)(w - item0), t1 = (int)(w1 - item0);
     const int len = rq.ctx + rq.nodes;
 
-    // places of tile t's keys, one thread each, into buffer t & 1, and its groups' scales
+    // A stage is TG tiles from t on.  Its groups' places, one thread each, go to buffer `which`.
+    constexpr int kStageGroups = TG * kKeyTile / kGroup;
     auto find = [&](int t) {
-      return tid < kKeyTile && t < t1 ? attn8_place(a, b, t * kKeyTile + tid, len, head) : Place8{-1, -1, -1, -1};
+      return tid < kStageGroups && t < t1 ? attn8_look(a, b, t * kKeyTile + tid * kGroup, len, head) : Look8{0, -1, 0};
     };
-    auto put = [&](int t, const Place8& p) {
-      if (tid < kKeyTile && t < t1) {
-        s.place[t & 1][0][tid] = p.k;
-        s.place[t & 1][1][tid] = p.v;
-        if (tid % kGroup == 0) s.scales[t % kSets][tid / kGroup] = group_scales(a, p);
-      }
+    auto put = [&](int which, const Look8& l) {
+      if (tid < kStageGroups) s.place[which][tid] = attn8_place(a, l);
     };
-    auto load = [&](int t) {
+    const int row = tid / kUnits, unit = tid % kUnits;
+    auto load = [&](int t, int stage) {
       if (t < t1) {
-        const int st = (t - t0) % kStages;
-#pragma unroll 4
-        for (int u = tid; u < kKeyTile * kUnits; u += kThreads) {
-          const int r = u / kUnits, c = u % kUnits;
-          const int64_t k = s.place[t & 1][0][r], v = s.place[t & 1][1][r];
-          cp16_or_zero(smem_u32(s.ring[st][0]) + r * D + (Cfg::key_unit(r, c) << 4), kc + (k < 0 ? 0 : k + c * 16), k >= 0);
-          cp16_or_zero(smem_u32(s.ring[st][1]) + r * D + (Cfg::value_unit(r, c) << 4), vc + (v < 0 ? 0 : v + c * 16), v >= 0);
+        const Place8* place = s.place[stage & 1];
+        const int st = stage % kStages, end_row = min(t1, t + TG) * kKeyTile;
+#pragma unroll
+        for (int j = 0; j < TG * kKeyTile / Cfg::kPass; ++j) {
+          const int r = j * Cfg::kPass + row;
+          const Place8& p = place[r / kGroup];
+          const int64_t k = p.k + (r % kGroup) * a.kc_st[1] + unit * 16, v = p.v + (r % kGroup) * a.vc_st[1] + unit * 16;
+          const bool there = p.k >= 0 && t * kKeyTile + r < min(len, end_row);
+          cp16_or_zero(smem_u32(s.ring[st][0]) + r * D + (Cfg::key_unit(r, unit) << 4), kc + (there ? k : 0), there);
+          cp16_or_zero(smem_u32(s.ring[st][1]) + r * D + (Cfg::value_unit(r, unit) << 4), vc + (there ? v : 0), there);
+        }
+        if (tid < 2 * kStageGroups) {
+          const int g = tid >> 1;
+          const int64_t at = tid & 1 ? place[g].vs : place[g].ks;
+          float* to = tid & 1 ? &s.scales[st][g].y : &s.scales[st][g].x;
+          if (at >= 0) cp_async4(to, (tid & 1 ? a.v_scale : a.k_scale) + at);
+          else *to = 1.f;
         }
       }
       cp_commit();
     };
 
     __syncthreads();  // the item before is done with shared memory
-    put(t0, find(t0));
+    put(0, find(t0));
     for (int r = warp; r < kRows; r += kThreads / 32) {  // a warp a row: two elements a lane and step
       constexpr int kSteps = D / 64;
       float2 x[kSteps];
@@ -147,8 +159,8 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
-      load(t0 + i);
-      put(t0 + i + 1, find(t0 + i + 1));
+      load(t0 + i * TG, i);
+      put((i + 1) & 1, find(t0 + (i + 1) * TG));
       __syncthreads();
     }
 
@@ -180,36 +192,46 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // reference, sum of weights
     float peak[2] = {-INFINITY, -INFINITY};                      // the highest reference so far
 
-    for (int t = t0; t < t1; ++t) {
+    Look8 ahead = find(t0 + kStages * TG);
+    for (int ts = t0, stage = 0; ts < t1; ts += TG, ++stage) {
       cp_wait<kStages - 2>();
       __syncthreads();
-      load(t + kStages - 1);
-      const Place8 ahead = find(t + kStages);
-      const int st = (t - t0) % kStages;
-      uint8_t* kt = s.ring[st][0];
-      uint8_t* vt = s.ring[st][1];
+      load(ts + (kStages - 1) * TG, stage + kStages - 1);
+      put((stage + kStages) & 1, ahead);
+      ahead = find(ts + (kStages + 1) * TG);  // a page number has an iteration to arrive
+      const int st = stage % kStages, t = ts + tg;
+      uint8_t* kt = s.ring[st][0] + tg * Cfg::kTileBytes;
+      uint8_t* vt = s.ring[st][1] + tg * Cfg::kTileBytes;
       const int pos0 = t * kKeyTile;
-      const bool tail = pos0 + kKeyTile > rq.ctx;  // drafted tokens, or places past the end
+      const bool tail = (ts + TG) * kKeyTile > rq.ctx;  // drafted tokens, or places past the end, in one of the tiles
       unsigned long long odd = 0ull;
       if (tail) {
         // A drafted token hidden from a row has weight 0 there, but 0 times NaN is NaN: such tokens' values are
         // taken out of the product and added row by row below.
-        if (tid < 2) s.odd[tid] = 0u;
+        if (tid < 2 * TG) s.odd[tid >> 1][tid & 1] = 0u;
         __syncthreads();
-        for (int u = tid; u < kKeyTile * kUnits; u += kThreads) {
+        uint8_t* all = s.ring[st][1];
+        const int rows = min(t1 - ts, TG) * kKeyTile;
+        for (int u = tid; u < rows * kUnits; u += kThreads) {
           const int r = u / kUnits;
-          if (pos0 + r < rq.ctx) continue;
-          const uint4 x = lds128(vt + u * 16);
-          if (has_nan(x.x) || has_nan(x.y) || has_nan(x.z) || has_nan(x.w)) atomicOr(&s.odd[r >> 5], 1u << (r & 31));
+          if (ts * kKeyTile + r < rq.ctx) continue;
+          const uint4 x = lds128(all + u * 16);
+          if (has_nan(x.x) || has_nan(x.y) || has_nan(x.z) || has_nan(x.w))
+            atomicOr(&s.odd[r / kKeyTile][(r >> 5) & 1], 1u << (r & 31));
         }
         __syncthreads();
-        odd = ((unsigned long long)s.odd[1] << 32) | s.odd[0];
-        if (odd) {
-          for (int u = tid; u < kKeyTile * kUnits; u += kThreads)
-            if (odd >> (u / kUnits) & 1) *reinterpret_cast<uint4*>(vt + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+        odd = ((unsigned long long)s.odd[tg][1] << 32) | s.odd[tg][0];
+        bool any = false;
+        for (int i = 0; i < TG; ++i) any |= (s.odd[i][0] | s.odd[i][1]) != 0u;
+        if (any) {
+          for (int u = tid; u < rows * kUnits; u += kThreads) {
+            const int r = u / kUnits;
+            if (s.odd[r / kKeyTile][(r >> 5) & 1] >> (r & 31) & 1) *reinterpret_cast<uint4*>(all + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
           __syncthreads();
         }
       }
+      if (TG > 1 && t >= t1) continue;  // the segment ends within the stage
 
       // scores of 16 rows x kKeys keys
       float sc[kKeys / 8][4];
@@ -235,7 +257,7 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
       }
       float4 gs[kGroups];
 #pragma unroll
-      for (int z = 0; z < kGroups; ++z) gs[z] = s.scales[t % kSets][wk * kGroups + z];
+      for (int z = 0; z < kGroups; ++z) gs[z] = group_factors(a, s.scales[st][tg * (kKeyTile / kGroup) + wk * kGroups + z]);
 #pragma unroll
       for (int i = 0; i < kKeys / 8; ++i) {
 #pragma unroll
@@ -334,7 +356,6 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
             for (int e = 0; e < 4; ++e) o[i][e & 1][2 * h + (e >> 1)] += p[h] * e4m3_value(vc[vo + i * 16 + q4 * 4 + e]);
         }
       }
-      put(t + kStages, ahead);
     }
     cp_wait<0>();
     __syncthreads();
@@ -346,11 +367,12 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
     }
-    if (WK > 1) {
+    const int part = tg * WK + wk;
+    {
       constexpr int kJ = Cfg::kJoinRow;
-      float* stat = join + (WK - 1) * MT * 16 * kJ;
-      if (wk > 0) {
-        const int slot = (wk - 1) * MT + wr;
+      float* stat = join + (Cfg::kParts - 1) * MT * 16 * kJ;
+      if (part > 0) {
+        const int slot = (part - 1) * MT + wr;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = g + 8 * h;
@@ -366,13 +388,13 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
         }
       }
       __syncthreads();
-      if (wk == 0) {
+      if (part == 0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = g + 8 * h;
           float mx = top[h];
 #pragma unroll
-          for (int x = 0; x < WK - 1; ++x) mx = fmaxf(mx, stat[((x * MT + wr) * 16 + r) * 2]);
+          for (int x = 0; x < Cfg::kParts - 1; ++x) mx = fmaxf(mx, stat[((x * MT + wr) * 16 + r) * 2]);
           const float ref = mx == -INFINITY ? 0.f : mx;
           float f = exp2_fast(top[h] - ref);
           sum[h] *= f;
@@ -381,7 +403,7 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
 #pragma unroll
             for (int e = 0; e < 2; ++e) o[i][e][2 * h] *= f, o[i][e][2 * h + 1] *= f;
 #pragma unroll
-          for (int x = 0; x < WK - 1; ++x) {
+          for (int x = 0; x < Cfg::kParts - 1; ++x) {
             const int slot = x * MT + wr;
             f = exp2_fast(stat[(slot * 16 + r) * 2] - ref);
             sum[h] += f * stat[(slot * 16 + r) * 2 + 1];
@@ -397,7 +419,7 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
         }
       }
     }
-    if (wk == 0) {
+    if (part == 0) {
       const bool all = w == item0 && w1 == item1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -432,10 +454,10 @@ __global__ void __launch_bounds__(32 * MT * WK, 1) tree_attn8_kernel(const __gri
 
 namespace {
 
-template <typename T, int D, int MT, int WK>
+template <typename T, int D, int MT, int WK, int TG>
 int launch_form8(const Attn8Args& a, cudaStream_t stream, int& grid, int& rows) {
-  using Cfg = Attn8Cfg<D, MT, WK>;
-  const void* k = (const void*)tree_attn8_kernel<T, D, MT, WK>;
+  using Cfg = Attn8Cfg<D, MT, WK, TG>;
+  const void* k = (const void*)tree_attn8_kernel<T, D, MT, WK, TG>;
   if (!prepare_kernel(k)) return 2;
   grid = num_sms();
   rows = Cfg::kRows;
@@ -446,9 +468,18 @@ template <typename T, int D>
 int launch_d8(const Attn8Args& a, cudaStream_t stream) {
   int grid = 0, rows = 0, rc;
   const int most = a.max_nodes * a.group;
-  if (most <= 16) rc = launch_form8<T, D, 1, 4>(a, stream, grid, rows);
-  else if (most <= 32) rc = launch_form8<T, D, 2, 4>(a, stream, grid, rows);
-  else rc = launch_form8<T, D, 4, 2>(a, stream, grid, rows);
+  // Key tiles of the launch.  Up to 16 rows a kv head (decoding, narrow trees) stay here, where a tile costs the fewest
+  // instructions, with more warps for the tiles where a CTA has several: one token over 1,000 keys 12.5 us with one set
+  // of warps and 13.7 with two, 16 requests of a token over up to 8,192 keys (66 tiles a CTA) 132 and 88 (three or four
+  // sets: 83 and 86; with heads of 64, 43, 37 and 36).  Only with tiles in plenty does the tensor-memory form draw level: 85
+  // and 101 us against 88 and 104 at 112 tiles an SM.  More rows go there from three tiles an SM times row tiles of 32
+  // on: at 1.8 17.7 us here and 19.5 there, at 3.5 30.3 and 25.7, at 7 30.6 and 27.8, at 28 66 and 39.
+  const int64_t tiles = (int64_t)a.B * a.Hk * ((a.max_context + a.max_nodes + kKeyTile - 1) / kKeyTile), sms = num_sms();
+  if (most <= 16 ? tiles > 100 * sms : tiles * ((most + 31) / 32) > 3 * sms) rc = launch_tree_attn8_tc(a, stream, grid, rows);
+  else if (most <= 16 && tiles <= sms) rc = launch_form8<T, D, 1, 4, 1>(a, stream, grid, rows);
+  else if (most <= 16) rc = launch_form8<T, D, 1, 4, D == 64 ? 3 : 2>(a, stream, grid, rows);
+  else if (most <= 32) rc = launch_form8<T, D, 2, 4, 1>(a, stream, grid, rows);
+  else rc = launch_form8<T, D, 4, 2, 1>(a, stream, grid, rows);
   return rc ? rc : launch_attn_join(a, stream, grid, rows);
 }
 

@@ -26,30 +26,47 @@ constexpr int kGroup = 16;  // keys with one scale
 struct Place8 {
   int64_t k, v, ks, vs;
 };
-__device__ __forceinline__ Place8 attn8_place(const Attn8Args& a, int b, int pos, int len, int head) {
+// In two steps, since the first waits for nothing: a warp that asks for a page number and tests it at once stands still
+// for an L2 access.
+struct Look8 {
+  int page, in, head;  // in -1: no such key
+};
+__device__ __forceinline__ Look8 attn8_look(const Attn8Args& a, int b, int pos, int len, int head) {
+  Look8 l{0, -1, head};
+  if (pos < len) {
+    const int p = pos / a.page_size;
+    l.in = pos - p * a.page_size;
+    l.page = __ldg(a.page_table + (int64_t)b * a.table_ld + p);
+  }
+  return l;
+}
+__device__ __forceinline__ Place8 attn8_place(const Attn8Args& a, const Look8& l) {
   Place8 r{-1, -1, -1, -1};
-  if (pos >= len) return r;
-  const int p = pos / a.page_size, in = pos - p * a.page_size;
-  const int page = a.page_table[(int64_t)b * a.table_ld + p];
-  if (page < 0 || page >= a.num_pages) {
+  if (l.in < 0) return r;
+  if (l.page < 0 || l.page >= a.num_pages) {
     record_error(a.err, ERR_PAGE);
     return r;
   }
-  const int blk = in / a.block;
-  r.k = (int64_t)page * a.kc_st[0] + (int64_t)in * a.kc_st[1] + (int64_t)head * a.kc_st[2];
-  r.v = (int64_t)page * a.vc_st[0] + (int64_t)in * a.vc_st[1] + (int64_t)head * a.vc_st[2];
-  r.ks = (int64_t)page * a.ks_st[0] + (int64_t)blk * a.ks_st[1] + (int64_t)head * a.ks_st[2];
-  r.vs = (int64_t)page * a.vs_st[0] + (int64_t)blk * a.vs_st[1] + (int64_t)head * a.vs_st[2];
+  const int blk = l.in / a.block;
+  r.k = (int64_t)l.page * a.kc_st[0] + (int64_t)l.in * a.kc_st[1] + (int64_t)l.head * a.kc_st[2];
+  r.v = (int64_t)l.page * a.vc_st[0] + (int64_t)l.in * a.vc_st[1] + (int64_t)l.head * a.vc_st[2];
+  r.ks = (int64_t)l.page * a.ks_st[0] + (int64_t)blk * a.ks_st[1] + (int64_t)l.head * a.ks_st[2];
+  r.vs = (int64_t)l.page * a.vs_st[0] + (int64_t)blk * a.vs_st[1] + (int64_t)l.head * a.vs_st[2];
   return r;
 }
+__device__ __forceinline__ Place8 attn8_place(const Attn8Args& a, int b, int pos, int len, int head) {
+  return attn8_place(a, attn8_look(a, b, pos, len, head));
+}
 
-// A group's (s_k, log2 s_v, 1 / s_v); ones where there are no keys.
+// What the softmax needs of a group's scales (s_k, s_v): s_k, log2 s_v, 1 / s_v.
+__device__ __forceinline__ float4 group_factors(const Attn8Args& a, float2 s) {
+  const float k = scale_or_least(s.x), v = scale_or_least(s.y);
+  if (!(k == s.x) || !(v == s.y)) record_error(a.err, ERR_SCALE);
+  return make_float4(k, __log2f(v), __fdividef(1.f, v), 0.f);
+}
+// Those of the key at p; ones where there is none.
 __device__ __forceinline__ float4 group_scales(const Attn8Args& a, const Place8& p) {
-  if (p.ks < 0) return make_float4(1.f, 0.f, 1.f, 0.f);
-  float ks = a.k_scale[p.ks], vs = a.v_scale[p.vs];
-  const float k = scale_or_least(ks), v = scale_or_least(vs);
-  if (!(k == ks) || !(v == vs)) record_error(a.err, ERR_SCALE);
-  return make_float4(k, log2f(v), 1.f / v, 0.f);
+  return group_factors(a, p.ks < 0 ? make_float2(1.f, 1.f) : make_float2(a.k_scale[p.ks], a.v_scale[p.vs]));
 }
 
 // Whether one of the four bytes is a NaN.

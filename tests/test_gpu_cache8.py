@@ -369,12 +369,21 @@ SHAPES = [
     ([9000], [64], 16, 4, 128, 256, 64, torch.bfloat16),
     ([20000, 7], [16, 2], 16, 2, 256, 64, 32, torch.bfloat16),
     ([12000, 2], [60, 3], 12, 4, 64, 64, 16, torch.float16),
+    ([20000], [1], 16, 2, 256, 64, 64, torch.bfloat16),
+    ([9000, 3001], [2, 1], 24, 4, 64, 64, 32, torch.float16),
+    ([6000, 129, 2500], [3, 1, 4], 32, 8, 128, 32, 16, torch.bfloat16),
 ]
 
 
 @pytest.mark.parametrize("args", SHAPES, ids=str)
 def test_attention(args):
     Attention(*args).check()
+
+
+@pytest.mark.parametrize("args", SHAPES, ids=str)
+def test_attention_bounds_far_from_the_lengths(args):
+    """Loose bounds take the tensor-memory form whatever the lengths are."""
+    Attention(*args, seed=1).check(max_context=10**7, max_nodes=64)
 
 
 @pytest.mark.parametrize("D,Hq,Hk", [(64, 8, 2), (128, 8, 2), (256, 8, 2)])
