@@ -34,6 +34,18 @@ int num_sms() {
   return cache[dev];
 }
 
+bool prepare_wide_cluster(const void* func) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({func, dev})) return true;
+  if (cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  done.insert({func, dev});
+  return true;
+}
+
 bool prepare_kernel(const void* func) {
   static std::mutex mu;
   static std::set<std::pair<const void*, int>> done;

@@ -575,6 +575,8 @@ int launch_dense_tc(const DenseArgs& d, int wt, int grid, size_t smem, float* pa
 int num_sms();
 // Raise a kernel's dynamic shared-memory limit once per device; false on failure.
 bool prepare_kernel(const void* func);
+// Allow a kernel clusters of 16 blocks, once per device; false on failure.
+bool prepare_wide_cluster(const void* func);
 
 // Launch `func(args)` with the programmatic-stream-serialization attribute when `pdl`.
 template <typename Args>

@@ -12,15 +12,19 @@
 //   accepted  iff  u S < r(x);   refused:  S <- S - r(x),  r(x) <- 0.
 //
 // Then the next token is drawn from r by the request's own random number: the path's tokens and this one have the
-// target's distribution.  Values are held in 64-bit floating point with each operation rounded by itself, sums are of
-// whole numbers (trunc(2^52 r)), exact in any order: the split of a row changes nothing.  Where nothing is left (all
-// of r rounds to 0) r stays what it was.
+// target's distribution.  r is held in 32 bits, as p and q are: r / S - q is p times a reciprocal in two 32-bit parts, by
+// two fused multiply-adds, so it is off by half a step of its own whatever cancels.  Sums are of whole numbers
+// (trunc(2^52 r), 64 bits), exact in any order: the split of a row changes nothing.  (In 64-bit floating point throughout
+// 32 trees of 16 nodes took 48 us against 25.)  S and the tests are in 64 bits.
+// Where nothing is left (all of r rounds to 0) r stays what it was.
 //
 // Bound: one read of the row at the path's end (of p, and of q where a child was refused there), since probabilities
 // of drafted tokens alone decide all else; for few requests, the chain of steps.  A cluster of CTAs has a request,
 // each a slice of the rows.  Every CTA walks the tree by itself, so the cluster only exchanges sums: one pass over
 // the slice for each refusal by q, whose sums also serve the final draw.  The token is found from the sums of CTAs,
-// then of warps, then by one more read of the 1/(8 x 16) of the row that holds it.
+// then of warps, then by one more read of the 1/(16 x 8) of the row that holds it.
+// Measured (B200): a chain of 6 nodes, vocabulary of 151,936, 8.5 us; 32 trees of 16 nodes 19.5 us, which is up to four
+// passes over the 1.2 MB of one request's two rows, on 16 of the 148 SMs (in clusters of 8 25 us, with 512 threads 26).
 #include <cooperative_groups.h>
 
 #include "fnx_common.cuh"
@@ -33,11 +37,12 @@ namespace {
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
-constexpr int kVT = 512;             // threads
+constexpr int kVT = 256;             // threads
 constexpr int kVW = kVT / 32;        // warps
 constexpr int kNodes = 64;           // nodes of a request
-constexpr int kVCluster = 8;         // CTAs of a request
+constexpr int kVCluster = 16;        // CTAs of a request
 constexpr int kTileV = 128;          // tokens of a warp's step: four a lane
+constexpr int kFlight = 5;           // steps whose loads are in flight together
 constexpr double kUnit = 4503599627370496.0;  // 2^52
 
 enum Step : int { STEP_PASS = 0, STEP_DRAW = 1 };
@@ -45,8 +50,8 @@ enum Step : int { STEP_PASS = 0, STEP_DRAW = 1 };
 struct VerifySmem {
   int parent[kNodes];
   int64_t token[kNodes];
-  double uniform[kNodes], p[kNodes], q[kNodes];  // of the node's token, in its parent's rows
-  double inv[kNodes];      // 1 / S of the refusals at the path's end
+  float uniform[kNodes], p[kNodes], q[kNodes];  // of the node's token, in its parent's rows
+  float2 inv[kNodes];      // 1 / S of the refusals at the path's end, in two parts
   int refused[kNodes];     // their tokens (without drafter probabilities)
   int path[kNodes];
   u64 warp_sum[kVW];       // of the last pass
@@ -58,12 +63,26 @@ struct VerifySmem {
   double left;             // S
 };
 
-__device__ __forceinline__ double probability(float v) { return v > 0.f ? (double)fminf(v, 1.f) : 0.0; }
-__device__ __forceinline__ u64 whole(double r) { return (u64)__double2ull_rz(__dmul_rn(r, kUnit)); }
-
-__device__ __forceinline__ double residual(const double* inv, int rounds, double p, double q) {
-  for (int k = 0; k < rounds; ++k) p = fmax(__dsub_rn(__dmul_rn(p, inv[k]), q), 0.0);
-  return p;
+__device__ __forceinline__ float probability(float v) { return __saturatef(v); }  // NaN counts as 0
+// trunc(2^52 r) for r in [0, 2): the significand at 2^55 and up, shifted down.
+__device__ __forceinline__ u64 whole(float r) {
+  const uint32_t bits = __float_as_uint(r);
+  const u64 m = (u64)((bits & 0x007FFFFFu) | 0x00800000u) << 32;
+  return m >> min(127 + 23 - 52 + 32 - (int)(bits >> 23), 63);
+}
+__device__ __forceinline__ float2 reciprocal(double s) {
+  const double r = 1.0 / s;
+  const float hi = (float)r;
+  return make_float2(hi, (float)(r - (double)hi));
+}
+// What `rounds` refusals leave of n tokens' p.
+template <int N>
+__device__ __forceinline__ void residual(const float2* inv, int rounds, float (&p)[N], const float (&q)[N]) {
+  for (int k = 0; k < rounds; ++k) {
+    const float2 by = inv[k];
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = fmaxf(fmaf(p[e], by.y, fmaf(p[e], by.x, -q[e])), 0.f);
+  }
 }
 
 __device__ __forceinline__ u64 warp_total(u64 v) {
@@ -111,10 +130,10 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
     const int parent = tid ? a.parents[n0 + tid] : -1;
     const int64_t x = a.tokens[n0 + tid];
     const bool known = parent >= 0 && parent < tid, word = x >= 0 && x < a.V;
-    double p = 0.0, q = 0.0;
+    float p = 0.f, q = 0.f;
     if (known && word) {
       p = probability(a.target[(int64_t)(n0 + parent) * a.ldt + x]);
-      q = a.draft ? probability(a.draft[(int64_t)(n0 + parent) * a.ldd + x]) : 1.0;
+      q = a.draft ? probability(a.draft[(int64_t)(n0 + parent) * a.ldd + x]) : 1.f;
     }
     if (rank == 0 && tid > 0) {
       if (!known && parent != -1) record_error(a.err, ERR_TREE);
@@ -122,7 +141,7 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
     }
     s.parent[tid] = known ? parent : -1;
     s.token[tid] = word ? x : -1;
-    s.uniform[tid] = (double)a.node_uniforms[n0 + tid];
+    s.uniform[tid] = a.node_uniforms[n0 + tid];
     s.p[tid] = p;
     s.q[tid] = q;
   }
@@ -146,19 +165,28 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
     const float* qrow = a.draft ? a.draft + (int64_t)(n0 + s.current) * a.ldd : nullptr;
     u64 sum = 0;
     if (a.draft && rounds > 0) {
-#pragma unroll 4
-      for (int v = v0 + lane * 4; v < v1; v += kTileV) {
-        const float4 p = four<kVec>(prow, v, v1), q = four<kVec>(qrow, v, v1);
-        sum += whole(residual(s.inv, rounds, probability(p.x), probability(q.x)));
-        sum += whole(residual(s.inv, rounds, probability(p.y), probability(q.y)));
-        sum += whole(residual(s.inv, rounds, probability(p.z), probability(q.z)));
-        sum += whole(residual(s.inv, rounds, probability(p.w), probability(q.w)));
+      for (int v = v0 + lane * 4; v < v1; v += kFlight * kTileV) {
+        float p[4 * kFlight], q[4 * kFlight];
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+          const float4 x = four<kVec>(prow, v + f * kTileV, v1), y = four<kVec>(qrow, v + f * kTileV, v1);
+          p[4 * f] = x.x, p[4 * f + 1] = x.y, p[4 * f + 2] = x.z, p[4 * f + 3] = x.w;
+          q[4 * f] = y.x, q[4 * f + 1] = y.y, q[4 * f + 2] = y.z, q[4 * f + 3] = y.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4 * kFlight; ++e) p[e] = probability(p[e]), q[e] = probability(q[e]);
+        residual(s.inv, rounds, p, q);
+#pragma unroll
+        for (int e = 0; e < 4 * kFlight; ++e) sum += whole(p[e]);
       }
     } else {
-#pragma unroll 4
-      for (int v = v0 + lane * 4; v < v1; v += kTileV) {
-        const float4 p = four<kVec>(prow, v, v1);
-        sum += whole(probability(p.x)) + whole(probability(p.y)) + whole(probability(p.z)) + whole(probability(p.w));
+      for (int v = v0 + lane * 4; v < v1; v += kFlight * kTileV) {
+        float4 p[kFlight];
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) p[f] = four<kVec>(prow, v + f * kTileV, v1);
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f)
+          sum += whole(probability(p[f].x)) + whole(probability(p[f].y)) + whole(probability(p[f].z)) + whole(probability(p[f].w));
       }
       if (!a.draft && lane < rounds) {  // refused tokens' shares are taken out again
         for (int k = lane; k < rounds; k += 32)
@@ -190,20 +218,21 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
         if (s.parent[i] != s.current) continue;
         bool accept;
         if (a.draft) {
-          const double inv = __drcp_rn(s.left);
-          const double r = residual(s.inv, s.rounds, s.p[i], s.q[i]);
-          accept = __dmul_rn(s.uniform[i], s.q[i]) < __dmul_rn(r, inv);
+          float r[1] = {s.p[i]};
+          const float q[1] = {s.q[i]};
+          residual(s.inv, s.rounds, r, q);
+          accept = (double)s.uniform[i] * (double)s.q[i] * s.left < (double)r[0];
           if (!accept) {
-            s.inv[s.rounds] = inv;
+            s.inv[s.rounds] = reciprocal(s.left);
             step = STEP_PASS;
           }
         } else {
-          double r = s.p[i];
+          double r = (double)s.p[i];
           for (int k = 0; k < s.rounds; ++k)
             if (s.refused[k] == (int)s.token[i]) r = 0.0;
-          accept = __dmul_rn(s.uniform[i], s.left) < r;
+          accept = (double)s.uniform[i] * s.left < r;
           if (!accept && r > 0.0) {
-            s.left = fmax(__dsub_rn(s.left, r), 0.0);
+            s.left = fmax(s.left - r, 0.0);
             s.refused[s.rounds++] = (int)s.token[i];
           }
         }
@@ -226,7 +255,7 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
       s.summed = all > 0;
       if (all > 0) {
         ++s.rounds;
-        s.left = __dmul_rn(__ull2double_rn(all), 1.0 / kUnit);
+        s.left = (double)all * (1.0 / kUnit);
       }
     }
     __syncthreads();
@@ -240,6 +269,7 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
     if (c < rank) before += t;
     all += t;
   }
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // the others' sums have been read
   if (rank == 0) {
     if (tid < a.width) a.path[(int64_t)b * a.width + tid] = tid < s.length ? s.path[tid] : -1;
     if (tid == 0) {
@@ -262,10 +292,12 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
       auto weights = [&](int v, u64 (&x)[4]) {
         const float4 p = four<kVec>(prow, v, p1);
         const float4 q = pairs ? four<kVec>(qrow, v, p1) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float ps[4] = {p.x, p.y, p.z, p.w}, qs[4] = {q.x, q.y, q.z, q.w};
+        float ps[4] = {probability(p.x), probability(p.y), probability(p.z), probability(p.w)};
+        const float qs[4] = {probability(q.x), probability(q.y), probability(q.z), probability(q.w)};
+        if (pairs) residual(s.inv, s.rounds, ps, qs);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = whole(pairs ? residual(s.inv, s.rounds, probability(ps[e]), probability(qs[e])) : probability(ps[e]));
+          x[e] = whole(ps[e]);
           if (!a.draft)
             for (int k = 0; k < s.rounds; ++k)
               if (s.refused[k] == v + e) x[e] = 0;
@@ -301,13 +333,15 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
       }
     }
   }
-  cl.sync();  // no CTA leaves while another reads its sums
+  // no CTA leaves while another reads its sums
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   pdl_trigger();
 }
 
 int launch_verify(VerifyArgs a, cudaStream_t stream) {
   a.per = (a.V + kVCluster * kVW * kTileV - 1) / (kVCluster * kVW * kTileV) * (kVW * kTileV);
   const void* k = a.vectors ? (const void*)verify_kernel<true> : (const void*)verify_kernel<false>;
+  if (!prepare_wide_cluster(k)) return 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.B * kVCluster);
   cfg.blockDim = dim3(kVT);

@@ -603,7 +603,7 @@ int fnx_tree_attention8(const void* q, int64_t q_sn, int64_t q_sh, const void* k
  * S = 1 at first: token x with node_uniforms u is accepted where u q(x) < r(x) / S, and becomes the
  * path's end; else r = max(r / S - q, 0), S = sum r.  With draft NULL: accepted where u S < r(x),
  * else S -= r(x), r(x) = 0.  Then next[b] is drawn from r, in the order of tokens, by
- * draw_uniforms[b].  Sums are of whole numbers (2^52 r, truncated): results are the same bit for
+ * draw_uniforms[b].  Sums are of whole numbers (2^52 r, truncated), r in 32 bits: results are the same bit for
  * bit from call to call.  Probabilities count as within [0, 1], NaN as 0; where nothing is left r
  * stays what it was.
  *  path int32 [batch, max_nodes]: the accepted nodes' indices, node 0 first, then -1; accepted int32

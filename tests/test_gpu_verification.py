@@ -4,8 +4,10 @@ token_probs: against the definition in 64 bits.  The weights come from fp32 expo
 at 2^-24 moves a weight by less than 28 * 2^-23 + 2^-22 < 2^-18, as for sample_tokens), so probabilities are within
 2^-17, relatively, or 2^-40 (a weight's last bit) of those that some top-p within that share of the given one gives.
 
-verify_tokens: against a walk in 64-bit numbers.  Sums of whole numbers lose less than V 2^-52 of a distribution; a
-comparison or a draw that lies within 2^-28 of its border may fall either way, and no other.
+verify_tokens: against a walk in 64-bit numbers.  An element of what refusals leave is rounded to 32 bits in each
+(2^-24 of it, carried through 1 / S of the later ones, S at least 2^-4 in these cases and one after another at most
+twice below 2^-1), and sums of whole numbers lose less than V 2^-52: a comparison or a draw that lies within NEAR_CHOICE =
+2^-18 of its border may fall either way, and no other.
 
 compact_nodes: exact, but for elements of an 8-bit cache that take another scale: within 2^-10 of it where they fall below
 2^-6 of it, exact above (powers of two)."""
@@ -20,6 +22,7 @@ from tests.test_gpu_sampling import NEAR
 pytestmark = pytest.mark.gpu
 
 E4M3 = torch.float8_e4m3fn
+NEAR_CHOICE = 2.0**-18
 
 
 def _fx():
@@ -204,7 +207,7 @@ class Drafts:
             if self.counts[b] == 0:
                 assert got == [] and int(tokens[b]) == -1
                 continue
-            found = [self.walk(b, e) for e in (0.0, 2.0**-28, -(2.0**-28))]
+            found = [self.walk(b, e) for e in (0.0, NEAR_CHOICE, -NEAR_CHOICE)]
             fit = [r for p, r in found if p == got]
             assert fit, (b, got, [p for p, _ in found])
             t = int(tokens[b])
@@ -216,7 +219,7 @@ class Drafts:
                 cum = np.cumsum(r)
                 aim = float(np.clip(self.w[b], 0, 1)) * cum[-1]
                 lo = cum[t - 1] if t > 0 else 0.0
-                right.append(t >= 0 and r[t] > 0 and lo - 2.0**-28 * cum[-1] <= aim <= cum[t] + 2.0**-28 * cum[-1])
+                right.append(t >= 0 and r[t] > 0 and lo - NEAR_CHOICE * cum[-1] <= aim <= cum[t] + NEAR_CHOICE * cum[-1])
             assert any(right), (b, t)
         return path, accepted, tokens
 
