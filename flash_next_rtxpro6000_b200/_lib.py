@@ -225,7 +225,7 @@ def _declare(lib):
         c_int64, c_int64, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_float, c_int, _P, _P,
         c_int, _P]
     lib.fnx_sample.argtypes = [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P]
-    lib.fnx_token_probs.argtypes = [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int64, c_int, _P]
+    lib.fnx_token_probs.argtypes = [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int64, _P, c_int, _P]
     lib.fnx_rotary_append8.argtypes = [
         _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, _P, _P,
         c_int64, c_int, _P, c_int64, c_int64, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, c_int64, c_int, c_int,

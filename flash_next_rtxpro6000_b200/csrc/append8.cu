@@ -11,7 +11,9 @@
 // and its chain of loads (offsets, page, data) for a few tokens.  A CTA has one block of one request and as many
 // (key or value) heads as its 256 threads hold, a thread 16 elements of a token's head, or up to four times that: it
 // finds the block's largest element with one exchange and writes the block without reading anything twice.  The
-// queries go to CTAs of their own in the same launch.
+// queries go to CTAs of their own in the same launch.  Measured (B200, calls in a graph): 3.1 us for 8 tokens of 16 + 2
+// heads of 256, 25.8 us for 4,097 tokens of 32 + 8 heads of 128 (93 MB, 3.6 TB/s): the queries alone take 14, keys and
+// values alone 15 before infinities were looked for once a thread, and both wait for instructions more than for memory.
 #include "cache8.cuh"
 
 namespace fnx {
@@ -47,49 +49,57 @@ __device__ __forceinline__ Unit unit_of(const Append8Args& a, int u) {
   return apart ? Unit{8 * u, a.R / 2 + 8 * u} : Unit{16 * u, 16 * u + 8};
 }
 
+// The unit as it lies in memory: elements stay 16 bits until they are used, which leaves registers for more loads.
+struct Raw {
+  uint32_t w[8];
+};
 template <typename T, bool kVec>
-__device__ __forceinline__ void load_unit(const T* src, const Unit& un, float (&x)[16]) {
+__device__ __forceinline__ Raw load_raw(const T* src, const Unit& un) {
+  Raw r;
   if (kVec) {
     const uint4 v0 = *reinterpret_cast<const uint4*>(src + un.o0), v1 = *reinterpret_cast<const uint4*>(src + un.o1);
-    const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 y = two<T>(w[i]);
-      x[2 * i] = y.x, x[2 * i + 1] = y.y;
-    }
+    r.w[0] = v0.x, r.w[1] = v0.y, r.w[2] = v0.z, r.w[3] = v0.w;
+    r.w[4] = v1.x, r.w[5] = v1.y, r.w[6] = v1.z, r.w[7] = v1.w;
   } else {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(src) + un.o0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = one(src[un.o0 + i]);
+    for (int i = 0; i < 8; ++i) r.w[i] = e[2 * i] | ((uint32_t)e[2 * i + 1] << 16);
   }
+  return r;
 }
 
 __device__ __forceinline__ float turn_a(float a, float b, float c, float s) { return __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)); }
 __device__ __forceinline__ float turn_b(float a, float b, float c, float s) { return __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)); }
 
-// The unit's cosines and sines (kVec), eight of each.
-struct Turn {
-  float c[8], s[8];
-};
-__device__ __forceinline__ void load_turn(const float* row, int half, int u, Turn& t) {
+// The unit's elements in 32 bits, turned by row's cosines and sines where `turned`.
+template <typename T>
+__device__ __forceinline__ void values(const Append8Args& a, const Raw& r, const float* row, int u, bool turned, float (&x)[16]) {
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    const float4 x = __ldg(reinterpret_cast<const float4*>(row + 8 * u + i));
-    const float4 y = __ldg(reinterpret_cast<const float4*>(row + half + 8 * u + i));
-    t.c[i] = x.x, t.c[i + 1] = x.y, t.c[i + 2] = x.z, t.c[i + 3] = x.w;
-    t.s[i] = y.x, t.s[i + 1] = y.y, t.s[i + 2] = y.z, t.s[i + 3] = y.w;
+  for (int i = 0; i < 8; ++i) {
+    const float2 y = two<T>(r.w[i]);
+    x[2 * i] = y.x, x[2 * i + 1] = y.y;
   }
-}
-__device__ __forceinline__ void turn_unit(bool interleaved, const Turn& t, float (&x)[16]) {
-  float y[16];
+  if (!turned) return;
+  const int half = a.R / 2;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {  // a pair's places in the unit
-    const float a = interleaved ? x[2 * i] : x[i], b = interleaved ? x[2 * i + 1] : x[8 + i];
-    const float ya = turn_a(a, b, t.c[i], t.s[i]), yb = turn_b(a, b, t.c[i], t.s[i]);
-    if (interleaved) y[2 * i] = ya, y[2 * i + 1] = yb;
-    else y[i] = ya, y[8 + i] = yb;
+  for (int z = 0; z < 2; ++z) {  // four pairs at a time
+    const float4 c4 = __ldg(reinterpret_cast<const float4*>(row + 8 * u + 4 * z));
+    const float4 s4 = __ldg(reinterpret_cast<const float4*>(row + half + 8 * u + 4 * z));
+    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 4 * z + e;
+      if (a.interleaved) {
+        const float p = x[2 * i], q = x[2 * i + 1];
+        x[2 * i] = turn_a(p, q, c[e], s[e]);
+        x[2 * i + 1] = turn_b(p, q, c[e], s[e]);
+      } else {
+        const float p = x[i], q = x[8 + i];
+        x[i] = turn_a(p, q, c[e], s[e]);
+        x[8 + i] = turn_b(p, q, c[e], s[e]);
+      }
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = y[i];
 }
 // Any sizes: 16 consecutive elements, each with its partner read by itself.
 template <typename T>
@@ -127,21 +137,19 @@ __device__ __forceinline__ void queries(const Append8Args& a, int cta) {
   const Unit un = unit_of<kVec>(a, u);
   const bool turned = 16 * u < a.R;
   for (int t = first; t < a.T; t += step) {
-    const float* row = table_row(a, t, part == 0 && threadIdx.x == 0);
-    Turn tn;
-    if (kVec && turned) load_turn(row, a.R / 2, u, tn);
+    const float* row = nullptr;
     for (int h0 = part * rows; h0 < a.Hq; h0 += a.q_parts * rows) {
       const int h = h0 + r;
       const bool live = h < a.Hq;
       const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
       T* dst = reinterpret_cast<T*>(a.q_out) + (int64_t)t * a.o_st + (int64_t)h * a.o_sh;
+      Raw raw;
+      if (live) raw = load_raw<T, kVec>(src, un);  // ahead of the position, which the table waits for
+      if (!row) row = table_row(a, t, part == 0 && threadIdx.x == 0);
       float x[16];
       if (live) {
-        load_unit<T, kVec>(src, un, x);
-        if (turned) {
-          if (kVec) turn_unit(a.interleaved, tn, x);
-          else turn_any(a, src, row, un.o0, x);
-        }
+        values<T>(a, raw, row, u, kVec && turned, x);
+        if (!kVec && turned) turn_any(a, src, row, un.o0, x);
       }
       if (!kVec) __syncwarp();  // q may be turned in place, and a unit's partners are other lanes'
       if (!live) continue;
@@ -166,6 +174,7 @@ __device__ __forceinline__ void queries(const Append8Args& a, int cta) {
 
 // Units of request b: numbers [off[b] / block + 2 b, off[b + 1] / block + 2 (b + 1)), at least as many as the blocks
 // that its tokens can touch wherever the context ends.  So a unit's request follows from the offsets alone.
+// kItems: 16-element units of a thread, in one block and head.
 template <typename T, bool kVec, int kItems>
 __global__ void __launch_bounds__(kAT) append8_kernel(const __grid_constant__ Append8Args a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -176,21 +185,18 @@ __global__ void __launch_bounds__(kAT) append8_kernel(const __grid_constant__ Ap
     pdl_trigger();
     return;
   }
-  const int unit = blockIdx.x / a.head_parts, part = blockIdx.x % a.head_parts;
+  const int unit = blockIdx.x / a.head_parts, part = blockIdx.x - unit * a.head_parts;
+  const int block_shift = 31 - __clz(a.block), wide_shift = 27 - __clz(a.D);  // blocks of 16 to 64, heads of 64 to 256
   int b = -1;
   for (int b0 = 0; b0 < a.B; b0 += kAT) {
     const int i = b0 + tid;
-    b += __syncthreads_count(i < a.B && a.node_offsets[i] / a.block + 2 * i <= unit);
+    b += __syncthreads_count(i < a.B && (a.node_offsets[i] >> block_shift) + 2 * i <= unit);
   }
-  __shared__ float amax_of[kAT / 32];
-  const int wide = a.D / 16;
-  const int per = kItems == 1 ? a.block * wide : kAT;  // threads of a head: a power of two, 64 at least
-  const int group = tid / per, at = tid % per;
-  const int head = part * (kAT / per) + group;  // keys' heads, then values'
-  const bool key = head < a.Hk;
-  const int h = key ? head : head - a.Hk;
+  __shared__ uint32_t amax_of[kAT / 32];
+  const int per_shift = kItems == 1 ? block_shift + wide_shift : 8;  // threads of a head: 64 at least
+  const int group = tid >> per_shift, at = tid & ((1 << per_shift) - 1), groups = kAT >> per_shift;
   const bool speaks = part == 0 && tid == 0;
-  if (b < 0) {  // ahead of the first request's units (offsets that start below 0)
+  if (b < 0) {  // ahead of the first request's units
     pdl_trigger();
     return;
   }
@@ -200,76 +206,86 @@ __global__ void __launch_bounds__(kAT) append8_kernel(const __grid_constant__ Ap
     pdl_trigger();
     return;
   }
-  const int64_t j = ctx / a.block + unit - (n0 / a.block + 2 * b);  // block of the sequence
-  const int64_t start = j * a.block;
-  if (start >= (int64_t)ctx + n || n == 0) {
+  const int blk = (ctx >> block_shift) + unit - ((n0 >> block_shift) + 2 * b);  // block of the sequence
+  const uint32_t start = (uint32_t)blk << block_shift, end = (uint32_t)ctx + n;
+  if (start >= end || n == 0) {
     pdl_trigger();
     return;
   }
-  const int in_page = (int)(start % a.page_size);
-  const int page = a.page_table[(int64_t)b * a.pt_ld + start / a.page_size];
+  const int kept = (uint32_t)ctx > start ? (int)(ctx - start) : 0;  // places of the block in front of the first new one
+  const int64_t to_token = (int64_t)n0 + start - ctx;               // token at the block's first place
+  const int last = (int)min((uint32_t)a.block, end - start);
+  const uint32_t number = start / (uint32_t)a.page_size;
+  const int in_page = (int)(start - number * (uint32_t)a.page_size);
+  const int page = a.page_table[(int64_t)b * a.pt_ld + number];
+  const int head = part * groups + group;  // keys' heads, then values'
+  const bool key = head < a.Hk, mine = head < 2 * a.Hk;
+  const int h = key ? head : head - a.Hk;
+  const int u = at & ((1 << wide_shift) - 1);  // the same for all of the thread's units
+  const Unit un = unit_of<kVec>(a, u);
+  const bool turned = key && 16 * u < a.R;
+  auto row_of = [&](int i) { return (at + (i << per_shift)) >> wide_shift; };
+  auto fresh = [&](int i) { return mine && row_of(i) >= kept && row_of(i) < last; };
+  auto source = [&](int i) {
+    return reinterpret_cast<const T*>(key ? a.k : a.v) + (to_token + row_of(i)) * (key ? a.k_st : a.v_st) +
+           (int64_t)h * (key ? a.k_sh : a.v_sh);
+  };
+  Raw raw[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i)
+    if (fresh(i)) raw[i] = load_raw<T, kVec>(source(i), un);  // ahead of the positions, which the table waits for
+  float x[kItems][16];
+  uint32_t amax = 0u;  // bits of the largest magnitude, infinities and NaN among them
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    if (!fresh(i)) continue;
+    const float* row = turned ? table_row(a, to_token + row_of(i), h == 0 && u == 0) : nullptr;
+    values<T>(a, raw[i], row, u, kVec && turned, x[i]);
+    if (!kVec && turned) turn_any(a, source(i), row, un.o0, x[i]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
+  }
+  const bool odd = amax >= 0x7F800000u;  // rare: an element is not finite
+  if (odd) {
+    amax = 0u;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t m = fresh(i) ? __float_as_uint(x[i][e]) & 0x7FFFFFFFu : 0u;
+        amax = max(amax, m < 0x7F800000u ? m : 0u);
+        if (m >= 0x7F800000u) x[i][e] = NAN;
+      }
+  }
+  amax = __reduce_max_sync(0xffffffffu, amax);
+  if (lane == 0) amax_of[warp] = amax;
   const bool there = page >= 0 && page < a.num_pages;
   if (!there && speaks) record_error(a.err, ERR_PAGE);
-  const int kept = ctx > start ? (int)(ctx - start) : 0;  // places of the block in front of the first new one
-  const int64_t to_token = n0 + start - ctx;               // token at the block's first place
-  const int last = (int)min((int64_t)a.block, ctx + n - start);
-  const bool stores = there && head < 2 * a.Hk;
-  uint8_t* cache = reinterpret_cast<uint8_t*>(key ? a.k_cache : a.v_cache);
-  const int64_t* st = key ? a.kc_st : a.vc_st;
-  uint8_t* rows = cache + (int64_t)page * st[0] + (int64_t)in_page * st[1] + (int64_t)h * st[2];
+  const bool stores = there && mine;
   float* scale_at = nullptr;
   float old = 0.f;
   if (stores) {
     const int64_t* ss = key ? a.ks_st : a.vs_st;
-    scale_at = (key ? a.k_scale : a.v_scale) + (int64_t)page * ss[0] + (int64_t)(in_page / a.block) * ss[1] + (int64_t)h * ss[2];
+    scale_at = (key ? a.k_scale : a.v_scale) + (int64_t)page * ss[0] + (int64_t)(in_page >> block_shift) * ss[1] + (int64_t)h * ss[2];
     if (kept > 0) old = *scale_at;
   }
-  float x[kItems][16];
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const int r = (at + i * per) / wide, u = (at + i * per) % wide;
-    if (!stores || r < kept || r >= last) continue;
-    const int64_t t = to_token + r;
-    const T* src = reinterpret_cast<const T*>(key ? a.k : a.v) + t * (key ? a.k_st : a.v_st) + (int64_t)h * (key ? a.k_sh : a.v_sh);
-    const Unit un = unit_of<kVec>(a, u);
-    const bool turned = key && 16 * u < a.R;
-    load_unit<T, kVec>(src, un, x[i]);
-    if (turned) {
-      const float* row = table_row(a, t, h == 0 && u == 0);
-      if (kVec) {
-        Turn tn;
-        load_turn(row, a.R / 2, u, tn);
-        turn_unit(a.interleaved, tn, x[i]);
-      } else {
-        turn_any(a, src, row, un.o0, x[i]);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float m = fabsf(x[i][e]);
-      amax = fmaxf(amax, m < INFINITY ? m : 0.f);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if (lane == 0) amax_of[warp] = amax;
   __syncthreads();
-  for (int w = group * per / 32; w < (group + 1) * per / 32; ++w) amax = fmaxf(amax, amax_of[w]);
-  float now = scale_for(amax);
-  float ratio = 1.f;
-  if (kept > 0) {
-    old = scale_or_least(old);
-    now = fmaxf(now, power_above(old));
-    ratio = old / now;
-  }
-  const float inv = 1.f / now;  // exact
+  for (int w = group << (per_shift - 5); w < (group + 1) << (per_shift - 5); ++w) amax = max(amax, amax_of[w]);
   if (stores) {
+    const int64_t* st = key ? a.kc_st : a.vc_st;
+    uint8_t* rows = reinterpret_cast<uint8_t*>(key ? a.k_cache : a.v_cache) + (int64_t)page * st[0] + (int64_t)in_page * st[1] +
+                    (int64_t)h * st[2];
+    float now = scale_for(__uint_as_float(amax)), ratio = 1.f;
+    if (kept > 0) {
+      old = scale_or_least(old);
+      now = fmaxf(now, power_above(old));
+      ratio = old / now;
+    }
+    const float inv = 1.f / now;  // exact
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const int r = (at + i * per) / wide, u = (at + i * per) % wide;
+      const int r = row_of(i);
       if (r >= last) continue;
-      const Unit un = unit_of<kVec>(a, u);
       uint2* d0 = reinterpret_cast<uint2*>(rows + (int64_t)r * st[1] + un.o0);
       uint2* d1 = reinterpret_cast<uint2*>(rows + (int64_t)r * st[1] + un.o1);
       if (r < kept) {
@@ -311,10 +327,9 @@ int launch_append8(Append8Args a, cudaStream_t stream) {
   a.q_parts = a.q_parts < 1 ? 1 : a.q_parts > spread ? spread : a.q_parts;
   const int tokens = a.T < 8192 ? a.T : 8192;
   a.q_ctas = a.Hq ? tokens * a.q_parts : 0;
-  const int64_t grid = (int64_t)a.kv_units * a.head_parts + a.q_ctas;
   const void* k = a.f16 ? (a.vectors ? append8_fn<__half, true>(items) : append8_fn<__half, false>(items))
                         : (a.vectors ? append8_fn<__nv_bfloat16, true>(items) : append8_fn<__nv_bfloat16, false>(items));
-  return launch_with_pdl(k, a, (int)grid, kAT, 0, a.pdl, stream);
+  return launch_with_pdl(k, a, a.kv_units * a.head_parts + a.q_ctas, kAT, 0, a.pdl, stream);
 }
 
 }  // namespace fnx

@@ -398,11 +398,12 @@ PyObject* token_probs(PyObject* const* a) {
     Unlocked others;
     if (!to) made = at::empty({M, V}, x.options().dtype(at::kFloat));
     const at::Tensor& out = to ? *to : made;
+    const at::Tensor rows = at::empty({M, FNX_TOKEN_PROBS_SCRATCH / 8}, x.options().dtype(at::kLong));
     check(fnx_token_probs(x.data_ptr(), M > 1 ? x.stride(0) : std::max(x.stride(0), V),
                           st == at::kFloat ? FNX_T_F32 : st == at::kHalf ? FNX_T_F16 : FNX_T_BF16, small(M, "rows"),
                           small(V, "vocab"), static_cast<const float*>(p[0]), static_cast<const int32_t*>(p[1]),
                           static_cast<const float*>(p[2]), static_cast<const float*>(p[3]), ptr<float>(out),
-                          M > 1 ? out.stride(0) : std::max(out.stride(0), V), pdl, stream),
+                          M > 1 ? out.stride(0) : std::max(out.stride(0), V), rows.data_ptr(), pdl, stream),
           "token_probs");
   }
   return result(a[5], std::move(made));

@@ -32,11 +32,9 @@ __device__ __forceinline__ float power_above(float s) {
   return __uint_as_float((bits + 0x007FFFFFu) & 0xFF800000u);
 }
 
-// Two values rounded to e4m3 (to the nearest, ties to even), the first in the low byte.  Infinities become NaN.
+// Two values rounded to e4m3 (to the nearest, ties to even; NaN stays NaN), the first in the low byte.
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
   uint16_t r;
-  a = fabsf(a) == INFINITY ? NAN : a;
-  b = fabsf(b) == INFINITY ? NAN : b;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
   return r;
 }

@@ -1555,13 +1555,17 @@ int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const f
 
 int fnx_token_probs(const void* logits, int64_t ldl, int dtype, int M, int V,
                     const float* temperature, const int32_t* top_k, const float* top_p,
-                    const float* min_p, float* probs, int64_t ldp, int pdl, fnx_stream_t stream) {
+                    const float* min_p, float* probs, int64_t ldp, void* scratch, int pdl,
+                    fnx_stream_t stream) {
+  static_assert(sizeof(fnx::KeptTokens) == FNX_TOKEN_PROBS_SCRATCH, "scratch of a row");
   g_err.clear();
   fnx::SampleArgs a = {};
   if (const int rc = sample_args("token probabilities", logits, ldl, dtype, M, V, temperature, top_k, top_p, min_p, pdl, a)) return rc;
   if (ldp < V) return fail(FNX_EINVAL, "token probabilities: rows of %d tokens %lld apart", V, (long long)ldp);
   if (M == 0) return FNX_OK;
-  if (!logits || !probs) return fail(FNX_EINVAL, "token probabilities: null pointer");
+  if (!logits || !probs || !scratch) return fail(FNX_EINVAL, "token probabilities: null pointer");
+  if (!aligned(scratch, 8)) return fail(FNX_EINVAL, "token probabilities: misaligned scratch");
+  a.rows = static_cast<fnx::KeptTokens*>(scratch);
   a.all = probs;
   a.ld_all = ldp;
   if (launched([&] { return fnx::launch_token_probs(a, static_cast<cudaStream_t>(stream)); }))

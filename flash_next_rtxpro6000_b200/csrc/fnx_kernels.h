@@ -715,6 +715,17 @@ struct VerifyArgs {
 };
 int launch_verify(VerifyArgs a, cudaStream_t stream);
 
+// What token_probs knows of a row before it writes: which tokens are kept, and their weight.
+enum Kept : int {
+  KEPT_PREFIX = 0,  // those above the logit `low`, and at it up to token `last`
+  KEPT_ONE = 1,     // token `last` (-1: none)
+};
+struct KeptTokens {
+  float m, T, low;
+  int what, last;
+  unsigned long long kept;
+};
+
 enum LogitsType : int { LOGITS_BF16 = 0, LOGITS_F16 = 1, LOGITS_F32 = 2 };
 struct SampleArgs {
   const void* logits;
@@ -729,6 +740,7 @@ struct SampleArgs {
   int pdl;
   float* all;   // token_probs: the probabilities of all tokens, in rows ld_all apart
   int64_t ld_all;
+  KeptTokens* rows;  // scratch, one a row
 };
 int launch_sample(SampleArgs a, cudaStream_t stream);
 int launch_token_probs(SampleArgs a, cudaStream_t stream);

@@ -545,10 +545,13 @@ int fnx_sample(const void* logits, int64_t ldl, int dtype, int M, int V, const f
  * The probabilities that fnx_sample draws from: probs fp32 [M, V] (row stride ldp >= V), for each
  * token its weight over that of all tokens that top-k, top-p and min-p keep, 0 for the others; a
  * row at temperature <= 0 has a 1 at its first token, a row without a logit above -inf zeros.
+ * scratch: FNX_TOKEN_PROBS_SCRATCH bytes a row, 8-byte aligned, not shared by calls that may overlap.
  */
+#define FNX_TOKEN_PROBS_SCRATCH 32
 int fnx_token_probs(const void* logits, int64_t ldl, int dtype, int M, int V,
                     const float* temperature, const int32_t* top_k, const float* top_p,
-                    const float* min_p, float* probs, int64_t ldp, int pdl, fnx_stream_t stream);
+                    const float* min_p, float* probs, int64_t ldp, void* scratch, int pdl,
+                    fnx_stream_t stream);
 
 /*
  * The 8-bit paged cache: k_cache and v_cache [num_pages, page_size, kv_heads, dim] e4m3 bytes, strides

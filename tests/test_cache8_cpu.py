@@ -62,13 +62,14 @@ def test_tree_attention8(kw, code):
 
 def _probs(**kw):
     return _call("fnx_token_probs", dict(logits=16, ldl=100, dtype=2, M=2, V=100, t=None, k=None, p=None, mp=None,
-                                         probs=16, ldp=100, pdl=0, stream=None), kw)
+                                         probs=16, ldp=100, scratch=16, pdl=0, stream=None), kw)
 
 
 @pytest.mark.parametrize("kw,code", [
     (dict(M=0), _lib.FNX_OK), (dict(dtype=3), _lib.FNX_EUNSUPPORTED), (dict(V=0), _lib.FNX_EINVAL),
     (dict(ldl=99), _lib.FNX_EINVAL), (dict(ldp=99), _lib.FNX_EINVAL), (dict(V=2**22, ldl=2**23, ldp=2**23), _lib.FNX_EUNSUPPORTED),
-    (dict(logits=None), _lib.FNX_EINVAL), (dict(probs=None), _lib.FNX_EINVAL),
+    (dict(logits=None), _lib.FNX_EINVAL), (dict(probs=None), _lib.FNX_EINVAL), (dict(scratch=None), _lib.FNX_EINVAL),
+    (dict(scratch=12), _lib.FNX_EINVAL),
 ])
 def test_token_probs(kw, code):
     assert _probs(**kw) == code
