@@ -206,9 +206,9 @@ __global__ void __launch_bounds__(kAT) append8_kernel(const __grid_constant__ Ap
     pdl_trigger();
     return;
   }
-  const int blk = (ctx >> block_shift) + unit - ((n0 >> block_shift) + 2 * b);  // block of the sequence
-  const uint32_t start = (uint32_t)blk << block_shift, end = (uint32_t)ctx + n;
-  if (start >= end || n == 0) {
+  const int ahead = unit - ((n0 >> block_shift) + 2 * b);  // blocks of the request in front of this one
+  const uint32_t start = (uint32_t)((ctx >> block_shift) + ahead) << block_shift, end = (uint32_t)ctx + n;
+  if (ahead < 0 || start >= end || n == 0) {
     pdl_trigger();
     return;
   }

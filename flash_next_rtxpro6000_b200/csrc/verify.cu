@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
     }
     s.parent[tid] = known ? parent : -1;
     s.token[tid] = word ? x : -1;
-    s.uniform[tid] = a.node_uniforms[n0 + tid];
+    s.uniform[tid] = fmaxf(a.node_uniforms[n0 + tid], 0.f);  // NaN and negative numbers count as 0
     s.p[tid] = p;
     s.q[tid] = q;
   }
