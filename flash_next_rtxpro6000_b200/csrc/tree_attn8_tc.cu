@@ -53,6 +53,7 @@ struct Tc8 {
     // keys reach the chunk that a tile's had kK tiles before, the softmax of the tile kScales before has ended.
     float4 scales[kScales][kTile / kGroup];
     float2 stat[kAlt ? 128 : 1];  // the second set's references and sums
+    float factor[kQInTmem ? 128 : 1];  // of the rows' scores
     long long before[kAttnMaxBatch + 1];
     unsigned long long kfull[kK], kempty[kK], vfull[kV], vempty[kV];
     unsigned long long sfull[RT][2], pfull[RT][2], odone[RT][2], qfull[RT];
@@ -425,11 +426,86 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
       const bool mine = r < sg.live;
       const bool busy = r0 + quad * 32 < sg.live;  // the warp has a live row
       const int node = mine ? (sg.row0 + r) / a.group : 0;
-      const int hq = sg.head * a.group + (sg.row0 + r) % a.group;
+      const int hq = sg.head * a.group + sg.row0 + r - node * a.group;  // where the row is live
       const int64_t qn = sg.rq.n0 + node;
       const unsigned long long mask = mine ? attn_mask(a, sg.rq, node) : 0ull;
       float factor = a.scale * 1.4426950408889634f;  // of the row's scores, in base-2 units
-      {
+      if (Cfg::kQInTmem) {
+        // Into tensor memory, a row a lane, by way of the warp's part of s.q: 64 elements at a time, eight lanes a row,
+        // so that loads are whole lines (one 16-node tree over 32,768 keys 39 -> 36 us).  First each row's largest
+        // element, then its elements times its power of two.
+        const int64_t my = mine ? qn * a.q_sn + (int64_t)hq * a.q_sh : -1;
+        const T* q = reinterpret_cast<const T*>(a.q) + (lane & 7) * 8;
+        const T* from[8];
+        float top[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int64_t at = __shfl_sync(0xffffffffu, my, 4 * k + (lane >> 3));
+          from[k] = at < 0 ? nullptr : q + at;
+          top[k] = 0.f;
+        }
+        auto eight = [&](int k, int c) {
+          return from[k] ? *reinterpret_cast<const uint4*>(from[k] + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        constexpr int kHold = D / 64 < 2 ? 1 : 2;  // 128 elements of a row at a time
+        uint4 held[kHold][8];
+#pragma unroll 1
+        for (int c0 = 0; c0 < D / 64; c0 += kHold) {
+#pragma unroll
+          for (int c = 0; c < kHold; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) held[c][k] = eight(k, c0 + c);
+#pragma unroll
+          for (int c = 0; c < kHold; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t w[4] = {held[c][k].x, held[c][k].y, held[c][k].z, held[c][k].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 y = query_two<T>(w[e]);
+                top[k] = max_three(top[k], fabsf(y.x), fabsf(y.y));
+              }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+          const int e2 = row_exponent(top[k]);
+          if ((lane & 7) == 0) s.factor[quad * 32 + 4 * k + (lane >> 3)] = factor * pow2f(-e2);
+          top[k] = pow2f(e2);
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint8_t* to = s.q[0] + quad * 32 * 128;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint4 x = eight(k, c);
+            const int y = 4 * k + (lane >> 3);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 v = query_two<T>(w[e]);
+              z[e] = round_pair<H>(v.x * top[k], v.y * top[k]);
+            }
+            *reinterpret_cast<uint4*>(to + y * 128 + (((lane & 7) ^ (y & 7)) << 4)) = make_uint4(z[0], z[1], z[2], z[3]);
+          }
+          __syncwarp();
+          uint32_t z[32];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint4 x = lds128(to + lane * 128 + ((e ^ (lane & 7)) << 4));
+            z[4 * e] = x.x, z[4 * e + 1] = x.y, z[4 * e + 2] = x.z, z[4 * e + 3] = x.w;
+          }
+          st32(tm + lanes + Cfg::kQCol + 32 * c, z);
+          __syncwarp();
+        }
+        wait_st();
+        fence_before();
+        __syncwarp();
+        factor = s.factor[row];
+      } else {
         const T* q = reinterpret_cast<const T*>(a.q) + qn * a.q_sn + (int64_t)hq * a.q_sh;
         uint8_t* to = s.q[kAlt ? 0 : rt] + row * 128;
         float amax = 0.f;
@@ -457,19 +533,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
             y[e] = round_pair<H>(z.x * up, z.y * up);
           }
         };
-        if (kAlt && rt == 1) {  // the other set stores them
-        } else if (Cfg::kQInTmem) {
-#pragma unroll 1
-          for (int c = 0; c < D / 8; c += 8) {
-            uint32_t y[32];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) eight(c + e, y + 4 * e);
-            __syncwarp();
-            st32(tm + lanes + Cfg::kQCol + 4 * c, y);
-          }
-          wait_st();
-          fence_before();
-        } else {
+        if (!(kAlt && rt == 1)) {  // the other set stores them
 #pragma unroll 8
           for (int c = 0; c < D / 8; ++c) {
             uint32_t y[4];
@@ -478,6 +542,8 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
                 make_uint4(y[0], y[1], y[2], y[3]);
           }
         }
+      }
+      {
         if (tid == 0) s.odd[seg % 3] = 0ull;  // the next segment's
         fence_proxy_async_smem();
         __syncwarp();
@@ -698,7 +764,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
       }
       if (busy) {
         const uint32_t oa = tm + lanes + r0 / 128 * D;
-        const bool all = sg.first && sg.last, dense = sg.live - r0 - quad * 32 > 8;
+        const bool all = sg.first && sg.last;
         const float inv = all ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
         T* out = reinterpret_cast<T*>(a.out) + qn * a.o_sn + (int64_t)hq * a.o_sh;
         float* slot = a.partials + (2ll * blockIdx.x + (sg.first ? 1 : 0)) * attn_slot_floats(kRows, D);
@@ -729,12 +795,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
               *reinterpret_cast<uint4*>(out + c + e) = y;
             }
           }
-          if (mine && !all && !dense) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(slot + (int64_t)r * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-          if (!all && dense) {
+          if (!all) {
             // A row a thread would touch 32 lines a store: the warp's 32 rows x 32 columns go through the
             // queries' place of its rows (they have been used), and out four whole lines a store.
             uint8_t* turn = s.q[kAlt ? 0 : rt] + quad * 32 * 128;
