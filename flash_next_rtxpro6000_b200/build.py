@@ -29,7 +29,8 @@ OBJ_DIR = PKG / "_build"
 SOURCES = ["fnx_api.cu", "dense_gemv.cu", "dense_gemv_slice.cu", "dense_gemv_norm.cu", "dense_tc.cu",
            "moe_gemv.cu",
            "moe_fused.cu", "moe_lean.cu", "nvfp4_codec.cu", "router.cu", "topk1.cu",
-           "rotary.cu", "tree_attn.cu", "tree_attn_tc.cu", "sample.cu", "token_probs.cu",
+           "rotary.cu", "tree_attn.cu", "tree_attn_tc.cu", "sample.cu", "sample_many.cu",
+           "token_probs.cu", "token_probs_many.cu",
            "append8.cu", "tree_attn8.cu", "tree_attn8_tc.cu", "verify.cu", "compact.cu"]
 BINDING = "binding.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -26,10 +26,14 @@
 //     both values' intervals are sent at once.  An interval with more tokens than the list holds
 //     (many ties, or one token far from the others) is split again by order key and token index
 //     until it fits.
-// Measured (B200): one row of 151,936 bf16 logits 10 us with a top-k of 50, 25 to 31 without top-k (of some
+// Measured (B200): one row of 151,936 bf16 logits 10 us with a top-k of 50, 22 to 37 without top-k (of some
 // 57,000 cycles the histogram's pass takes 15,000 to 19,000, its exponentials and shared-memory adds in
-// equal parts, the gathering 9,000, the exchanges about 1,500 each); 16 such rows in fp32 28 to 32 us; 128
-// rows of 248,320 138 us.  The form for many rows has 64 registers a thread and spills some 500 bytes of them.
+// equal parts, the gathering 9,000, the exchanges about 1,500 each); 16 such rows in fp32 19 and 42 to 50 us; 128
+// rows of 248,320 52 and 142 to 158 us (175 to 234 with a division and a 64-bit shift a logit in place of quotient()
+// and add_share()).  Two other ways were measured: a list of the likely tokens, made while all weights are added up, in
+// place of the histogram (31 and 92 us where it decides, 65 and 240 where it does not and the histogram follows), and a
+// histogram of counts, then exact sums around the interval that it points at (44 to 52, 128 to 240 us).  The form for
+// many rows has 64 registers a thread and spills some 500 bytes of them.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -42,6 +46,10 @@
 namespace fnx {
 
 namespace {
+
+// Lambdas are inlined by force.  Where the compiler left one out (the third kernel of a unit, say), all that it captures went
+// to local memory: 16 rows of 151,936 logits without top-k took 77 us instead of 56.
+#define FNX_INLINE __attribute__((always_inline))
 
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
@@ -149,6 +157,20 @@ struct Scale {
     const u64 m = (bits & 0x007FFFFFu) | 0x00800000u;
     return up >= 0 ? m << up : m >> min(-up, 63);
   }
+  // (x - m) / T for tokens with weight, something without for others; `by` is T's reciprocal in two parts.  a by.x + a by.y
+  // is the quotient but for one unit in its last place at most and its remainder is exact, so one more step gives the
+  // correctly rounded quotient (Markstein's theorem; by.x is the correctly rounded reciprocal).  Where `plain`: finite m
+  // and T in [2^-60, 2^60]; quotients so small that the remainder is not exact have an exponential of 1 all the same.
+  __device__ __forceinline__ bool plain() const { return m < INFINITY && T >= 0x1p-60f && T <= 0x1p60f; }
+  __device__ __forceinline__ float2 reciprocal() const {
+    const float y = __frcp_rn(T);
+    return make_float2(y, fmaf(-y, T, 1.0f) * y);
+  }
+  __device__ __forceinline__ float quotient(float x, float2 by) const {
+    const float a = fmaxf(x - m, -kReach * T);  // of NaN, too
+    const float q = fmaf(a, by.x, a * by.y);
+    return fmaf(fmaf(-q, T, a), by.x, q);
+  }
   // the interval of x, or -1 for a token without weight (NaN and -inf among them)
   __device__ __forceinline__ int bin(float x) const {
     const float d = x == m ? 0.0f : m - x;
@@ -215,6 +237,15 @@ __device__ __forceinline__ void add_sum(uint32_t w0_of_bin, u64 w) {
   add_shared(w0_of_bin, w0);
   add_shared(w0_of_bin + kBins * 4, w1);
   add_shared(w0_of_bin + kBins * 8, w2);
+}
+// The same of trunc(2^40 e): adding 2^(23 - k), rounded towards 0, leaves the whole number of 2^-k in a float's lowest bits.
+__device__ __forceinline__ void add_share(uint32_t w0_of_bin, float e) {
+  const float h = __fadd_rz(e, 0x1p11f), a = e - (h - 0x1p11f);     // 2^-12
+  const float i = __fadd_rz(a, 0x1p-3f), b = a - (i - 0x1p-3f);     // 2^-26
+  const float l = __fadd_rz(b, 0x1p-17f);                          // 2^-40
+  add_shared(w0_of_bin, __float_as_uint(l) - 0x37000000u);
+  add_shared(w0_of_bin + kBins * 4, __float_as_uint(i) - 0x3E000000u);
+  add_shared(w0_of_bin + kBins * 8, __float_as_uint(h) - 0x45000000u);
 }
 __device__ __forceinline__ u64 sum_of(const Bins& h, int b) {
   return h.w0[b] + ((u64)h.w1[b] << 14) + ((u64)h.w2[b] << 28);
@@ -521,7 +552,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
 
   // Calls f(number of logits, their values, place of the first) for the thread's logits of the
   // slice, a 16-byte vector at a time where the alignment allows; places rise within a thread.
-  auto sweep = [&](auto&& f) {
+  auto sweep = [&](auto&& f) FNX_INLINE {
     if (tid < head) {
       const float x[1] = {logit(xs[tid])};
       f(std::integral_constant<int, 1>{}, x, tid);
@@ -553,7 +584,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
 
   float top = -INFINITY, low = INFINITY;
   int top_at = -1;
-  auto look = [&](float x, int i) {
+  auto look = [&](float x, int i) FNX_INLINE {
     if (x > top) top = x, top_at = i;  // strictly: the first of equal logits stays
     low = fminf(low, x > -INFINITY ? x : low);
   };
@@ -612,14 +643,14 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     floor = min(floor, o.floor);
   }
   // Thread 0 of the first CTA leaves the row's kept tokens for the launch that writes the probabilities.
-  auto leave = [&](int what, const Scale& sc, int last, u64 kept) {
+  auto leave = [&](int what, const Scale& sc, int last, u64 kept) FNX_INLINE {
     if (rank != 0 || tid != 0) return;
     KeptTokens k;
     k.what = what;
     k.m = sc.m;
     k.T = sc.T;
     k.last = last;
-    k.low = what == KEPT_PREFIX ? logit(reinterpret_cast<const T*>(a.logits)[(int64_t)row * a.ldl + last]) : 0.0f;
+    k.low = what != KEPT_PREFIX ? 0.0f : last < 0 ? -INFINITY : logit(reinterpret_cast<const T*>(a.logits)[(int64_t)row * a.ldl + last]);
     k.kept = kept;
     a.rows[row] = k;
   };
@@ -645,11 +676,11 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   const double u = uniform > 0.0f ? (double)uniform : 0.0;  // NaN and negative numbers draw the most likely token
 
   // A found token goes to the CTA's own finds, and these to the first CTA's list in one piece.
-  auto find = [&](u64 key) {
+  auto find = [&](u64 key) FNX_INLINE {
     const uint32_t at = next_shared(finds0);
     if (at < (uint32_t)kCap) s.mine_found[at] = key;
   };
-  auto send = [&]() {
+  auto send = [&]() FNX_INLINE {
     __syncthreads();
     const uint32_t m = s.finds;
     if (tid == 0) s.place = atomicAdd(&first.listed, m);
@@ -663,7 +694,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   // --- (2) the tokens that reach the floor
   if (quick) {
     const float least = order_value(floor > kLowest ? floor : kLowest);
-    sweep([&](auto count, const float* x, int i0) {
+    sweep([&](auto count, const float* x, int i0) FNX_INLINE {
       float most = x[0];
 #pragma unroll
       for (int q = 1; q < count; ++q) most = fmaxf(most, x[q]);
@@ -685,7 +716,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
         Ranked r;
         if (few) r = rank_list(s, sc, held, by_share);
         else by_share = measure(s, sc, st, held);
-        auto ask = [&](int what, u64 value, double share) {
+        auto ask = [&](int what, u64 value, double share) FNX_INLINE {
           return few ? answer(s, r, held, 0, 0, what, value, share) : answer(s, sc, st, held, 0, 0, what, value, share);
         };
         // the list holds at least top_k tokens, or all there are
@@ -705,35 +736,75 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     }
   }
 
+  // --- all tokens are kept: their sum is the answer, no histogram is needed (16 rows 48 -> 22 us, 128 rows 230 -> 120,
+  // with the probabilities' launch)
+  if (kAll && top_k <= 0 && !use_p && !(sc.min_p > 0.0f) && sc.plain()) {
+    const float2 by = sc.reciprocal();
+    // whole numbers of 2^-17, and the rest (as in add_share); a thread has fewer than 2^15 tokens
+    uint32_t high = 0u;
+    u64 all = 0ull;
+    sweep([&](auto count, const float* x, int) FNX_INLINE {
+      uint32_t rest = 0u;
+#pragma unroll
+      for (int q = 0; q < count; ++q) {
+        const float e = expf(sc.quotient(x[q], by));
+        const float h = __fadd_rz(e, 64.0f), l = __fadd_rz(e - (h - 64.0f), 0x1p-17f);
+        high += __float_as_uint(h) - 0x42800000u;
+        rest += __float_as_uint(l) - 0x37000000u;
+      }
+      all += rest;
+    });
+    all = warp_sum(all + ((u64)high << 23));
+    if (lane == 0) s.red[warp] = all;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kST / 32; ++w) all += s.red[w];
+      s.mine.min_sum = all;
+    }
+    cl.sync();
+    if (rank == 0) {
+      all = 0ull;
+      for (int r = 0; r < C; ++r) all += cl.map_shared_rank(&s, r)->mine.min_sum;
+      leave(KEPT_PREFIX, sc, -1, all);
+    }
+    cl.sync();  // no CTA leaves while another reads its shared memory
+    pdl_trigger();
+    return;
+  }
+
   // --- (3) histogram, with counts where there is a top-k
   const bool counts = top_k > 0;
   {
     for (int b = tid; b < kBins; b += kST) s.h.count[b] = s.h.w0[b] = s.h.w1[b] = s.h.w2[b] = 0u;
     __syncthreads();
     u64 min_sum = 0ull;
-    // Weights of a whole vector first, so that their chains overlap; T = 1 needs no division.
-    auto fill = [&](auto unit) {
-      sweep([&](auto count, const float* x, int) {
+    // Weights of a whole vector first, so that their chains overlap.
+    const float2 by = sc.reciprocal();
+    auto fill = [&](auto plain) FNX_INLINE {
+      sweep([&](auto count, const float* x, int) FNX_INLINE {
         float e[count];
 #pragma unroll
         for (int q = 0; q < count; ++q) {
+          if (plain) {
+            e[q] = expf(sc.quotient(x[q], by));
+            continue;
+          }
           float d = x[q] - sc.m;
           const bool none = !(-d <= sc.range);  // NaN and -inf among them
           if (none || x[q] == sc.m) d = 0.0f;  // the division is slow where it meets an infinity
-          e[q] = expf(unit ? d : d / sc.T);
+          e[q] = expf(d / sc.T);
           if (none && x[q] != sc.m) e[q] = 0.0f;
         }
 #pragma unroll
         for (int q = 0; q < count; ++q) {
-          const int b = sc.bin(x[q]);
+          const int b = sc.bin(x[q]);  // -1: the weight is 0
           if (counts) add_shared(count0 + b * 4, b >= 0 ? 1u : 0u);
-          const u64 w = Scale::weight(e[q]);
-          add_sum(sum0 + b * 4, w);
-          if (sc.min_p > 0.0f && e[q] >= sc.min_p) min_sum += w;
+          add_share(sum0 + b * 4, e[q]);
+          if (sc.min_p > 0.0f && e[q] >= sc.min_p) min_sum += Scale::weight(e[q]);
         }
       });
     };
-    if (sc.T == 1.0f) fill(std::true_type{});
+    if (sc.plain()) fill(std::true_type{});
     else fill(std::false_type{});
     min_sum = warp_sum(min_sum);
     if (lane == 0) s.red[warp] = min_sum;
@@ -792,7 +863,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     __syncthreads();
   }
   // The interval in which the value is reached; each question has a place of its own for the answer.
-  auto bin_of = [&](int place, int want, u64 value, double share) {
+  auto bin_of = [&](int place, int want, u64 value, double share) FNX_INLINE {
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
       if (reached(want, own_count[q + 1], own_sum[q + 1], value, share) &&
@@ -809,8 +880,8 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   }
 
   // Calls f(key, logit) for the slice's tokens that the first CTA asks for.
-  auto asked = [&](const Control& c, auto&& f) {
-    sweep([&](auto count, const float* x, int i0) {
+  auto asked = [&](const Control& c, auto&& f) FNX_INLINE {
+    sweep([&](auto count, const float* x, int i0) FNX_INLINE {
 #pragma unroll
       for (int q = 0; q < count; ++q) {
         const int b = sc.bin(x[q]);
@@ -822,8 +893,8 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   };
 
   // Sends them to its list.
-  auto gather = [&](const Control& c) {
-    asked(c, [&](u64 key, float) { find(key); });
+  auto gather = [&](const Control& c) FNX_INLINE {
+    asked(c, [&](u64 key, float) FNX_INLINE { find(key); });
     send();
     cl.sync();
   };
@@ -832,9 +903,9 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   // first CTA.
   u64 klo = 0ull, khi = 0ull;
   int shift = 0;
-  auto split = [&](const Control& c) {
+  auto split = [&](const Control& c) FNX_INLINE {
     klo = ~0ull, khi = 0ull;
-    asked(c, [&](u64 key, float) {
+    asked(c, [&](u64 key, float) FNX_INLINE {
       klo = key < klo ? key : klo;
       khi = key > khi ? key : khi;
     });
@@ -852,7 +923,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     }
     shift = 0;
     while (((khi - klo) >> shift) >= (u64)kSub) ++shift;
-    asked(c, [&](u64 key, float x) {
+    asked(c, [&](u64 key, float x) FNX_INLINE {
       const int at = (int)((khi - key) >> shift);
       add_shared(count0 + at * 4, 1u);
       add_sum(sum0 + at * 4, Scale::weight(sc.share(x)));
@@ -901,7 +972,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
       cl.sync();
     }
   } else {
-    auto tell = [&](const Control& c) {
+    auto tell = [&](const Control& c) FNX_INLINE {
       __syncthreads();
       if (tid == 0) {
         s.ctl = c;
@@ -910,7 +981,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
       cl.sync();
     };
     // The token of interval b at which the value is reached; the list is loaded.
-    auto query = [&](int b, int want, u64 value, double share) -> Found {
+    auto query = [&](int b, int want, u64 value, double share) FNX_INLINE -> Found {
       c = Control{OP_GATHER, b, b, 0, -1, 0ull, ~0ull};
       u64 base_count = s.count[b], base_sum = s.sum[b];
       for (;;) {
@@ -954,7 +1025,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     u64 unused;
     if (few) r = rank_list(s, sc, held, unused);
     int measured = -1;
-    auto from_list = [&](int b, int what, u64 value, double share) {
+    auto from_list = [&](int b, int what, u64 value, double share) FNX_INLINE {
       if (few) {  // weight ahead of the list's tokens: that of an interval after the others is not in it
         u64 base = s.sum[c.bin_lo];
         if (b > c.bin_hi) base += s.sum[b] - s.sum[c.bin_hi + 1];
@@ -990,6 +1061,16 @@ const void* sample_fn(int type) {
   return (const void*)sample_kernel<__nv_bfloat16, kMany, kAll>;
 }
 
+}  // namespace
+
+// Each form is a unit of compilation: one takes the compiler a minute and a half.
+const void* sample_fn_one(int type);
+const void* sample_fn_many(int type);
+const void* probs_fn_one(int type);
+const void* probs_fn_many(int type);
+
+namespace {
+
 template <bool kAll>
 int launch_rows(SampleArgs a, cudaStream_t stream) {
   const int size = a.type == LOGITS_F32 ? 4 : 2;
@@ -999,7 +1080,7 @@ int launch_rows(SampleArgs a, cudaStream_t stream) {
   // histogram's sums above 2^20.)
   const bool many = (int64_t)a.M * 8 > num_sms() && a.V <= 1 << 20;
   const int C = many ? 4 : 8;
-  const void* k = many ? sample_fn<true, kAll>(a.type) : sample_fn<false, kAll>(a.type);
+  const void* k = kAll ? (many ? probs_fn_many(a.type) : probs_fn_one(a.type)) : many ? sample_fn_many(a.type) : sample_fn_one(a.type);
   if (!prepare_kernel(k)) return 2;
   a.per = ((a.V + C - 1) / C + 15) / 16 * 16;
   const size_t fixed = (sizeof(SampleSmem) + 15) & ~(size_t)15;

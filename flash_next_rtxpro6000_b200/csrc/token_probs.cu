@@ -78,6 +78,8 @@ const void* probs_fn(bool vec) {
 
 }  // namespace
 
+const void* probs_fn_one(int type) { return sample_fn<false, true>(type); }
+
 int launch_token_probs(SampleArgs a, cudaStream_t stream) {
   if (const int rc = launch_rows<true>(a, stream)) return rc;
   const int size = a.type == LOGITS_F32 ? 4 : 2, per = 16 / size;
