@@ -101,6 +101,22 @@ def test_probs_ties_and_rows_of_nothing():
     assert int((got[0] > 0).sum()) == 1500 and float(got[0, 1499]) > 0
 
 
+@pytest.mark.parametrize("M", [3, 40])  # few rows, many
+@pytest.mark.parametrize("T", [2.0**-70, 2.0**-60, 0.001, 0.9999999, 7.3, 2.0**60, 2.0**70])
+def test_probs_at_temperatures_of_any_size(M, T):
+    """Logits of the temperature's size, unfiltered and not; some infinite, some NaN."""
+    g, d = torch.Generator().manual_seed(M), dev()
+    x = torch.randn(M, 20011, generator=g) * 3 * T
+    x[torch.rand(M, 20011, generator=g) < 0.05] = -float("inf")
+    x[0, 7] = float("inf")
+    x[1, 70:90] = float("nan")
+    x[2, 5:] = -float("inf")
+    x, t = x.to(d), torch.full((M,), T, device=d)
+    _check_probs(x, t)
+    _check_probs(x, t, p=torch.full((M,), 0.9, device=d))
+    _check_probs(x, t, mp=torch.full((M,), 0.05, device=d))
+
+
 @pytest.mark.parametrize("M", [3, 40])
 def test_probs_are_what_sampling_draws_from(M):
     fx, d = _fx(), dev()
