@@ -11,12 +11,15 @@
 //
 //   accepted  iff  u S < r(x);   refused:  S <- S - r(x),  r(x) <- 0.
 //
+// A refusal that would leave nothing leaves r and S as they are.  With drafter probabilities the refusal's own sum tells.
+// Without, a row is not summed before the draw, so it is found there, when the refused tokens turn out to be all that the
+// row has: the walk goes back to the refusal that took the last one and goes on from there with that token alone.
+//
 // Then the next token is drawn from r by the request's own random number: the path's tokens and this one have the
 // target's distribution.  r is held in 32 bits, as p and q are: r / S - q is p times a reciprocal in two 32-bit parts, by
 // two fused multiply-adds, so it is off by half a step of its own whatever cancels.  Sums are of whole numbers
 // (trunc(2^52 r), 64 bits), exact in any order: the split of a row changes nothing.  (In 64-bit floating point throughout
 // 32 trees of 16 nodes took 48 us against 25.)  S and the tests are in 64 bits.
-// Where nothing is left (all of r rounds to 0) r stays what it was.
 //
 // Bound: one read of the row at the path's end (of p, and of q where a child was refused there), since probabilities
 // of drafted tokens alone decide all else; for few requests, the chain of steps.  A cluster of CTAs has a request,
@@ -52,13 +55,16 @@ struct VerifySmem {
   int64_t token[kNodes];
   float uniform[kNodes], p[kNodes], q[kNodes];  // of the node's token, in its parent's rows
   float2 inv[kNodes];      // 1 / S of the refusals at the path's end, in two parts
-  int refused[kNodes];     // their tokens (without drafter probabilities)
+  int refused[kNodes];     // their tokens (without drafter probabilities) ...
+  int refused_node[kNodes];     // ... and nodes, and S before
+  double left_before[kNodes];
   int path[kNodes];
   u64 warp_sum[kVW];       // of the last pass
   u64 total[2];            // this CTA's, of the last passes
   u64 tile_sum[kTileV];    // of the warp's part that holds the token
   // the walk
   int i, current, length, rounds, kept_rounds, step;
+  int sole;                // the only token left, or -1: its refusals change nothing (without drafter probabilities)
   bool summed;             // the last pass was over what is left now
   double left;             // S
 };
@@ -106,7 +112,7 @@ __device__ __forceinline__ float4 four(const float* row, int v, int end) {
 }  // namespace
 
 template <bool kVec>
-__global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ VerifySmem s;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank();
@@ -151,6 +157,7 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
     s.length = 1;
     s.rounds = 0;
     s.left = 1.0;
+    s.sole = -1;
     s.summed = false;
     s.path[0] = 0;
   }
@@ -231,8 +238,10 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
           for (int k = 0; k < s.rounds; ++k)
             if (s.refused[k] == (int)s.token[i]) r = 0.0;
           accept = (double)s.uniform[i] * s.left < r;
-          if (!accept && r > 0.0) {
+          if (!accept && r > 0.0 && (int)s.token[i] != s.sole) {
+            s.left_before[s.rounds] = s.left;
             s.left = fmax(s.left - r, 0.0);
+            s.refused_node[s.rounds] = i;
             s.refused[s.rounds++] = (int)s.token[i];
           }
         }
@@ -241,6 +250,7 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
           s.current = i;
           s.rounds = 0;
           s.left = 1.0;
+          s.sole = -1;
           s.summed = false;
         }
         if (step == STEP_PASS) break;
@@ -248,20 +258,35 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
       s.step = step;
     }
     __syncthreads();
-    if (s.step == STEP_DRAW) break;
-    const u64 all = pass(s.rounds + 1);
-    if (tid == 0) {
-      ++s.i;
-      s.summed = all > 0;
-      if (all > 0) {
-        ++s.rounds;
-        s.left = (double)all * (1.0 / kUnit);
+    const bool refusal = s.step == STEP_PASS;
+    if (!refusal && s.summed) break;
+    const u64 all = pass(s.rounds + (refusal ? 1 : 0));
+    if (!refusal) {
+      if (all > 0 || a.draft) break;
+      // the last refusal that took something; those behind it took tokens below 2^-52
+      int k = s.rounds - 1;
+      while (k >= 0 && whole(s.p[s.refused_node[k]]) == 0) --k;
+      if (k < 0) break;  // the row is zeros
+      __syncthreads();   // all have read what the next lines change
+      if (tid == 0) {
+        s.sole = s.refused[k];
+        s.left = s.left_before[k];
+        s.i = s.refused_node[k] + 1;
+        s.rounds = k;
       }
+    } else {
+      if (tid == 0) {
+        ++s.i;
+        s.summed = all > 0;
+        if (all > 0) {
+          ++s.rounds;
+          s.left = (double)all * (1.0 / kUnit);
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
   // --- the draw
-  if (!s.summed) pass(s.rounds);
   u64 before = 0, all = 0;
   const u64 mine = s.total[phase ^ 1];
   for (int c = 0; c < kVCluster; ++c) {

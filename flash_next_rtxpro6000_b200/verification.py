@@ -45,14 +45,15 @@ def verify_tokens(
     From the path's end on, its children are asked in order: with r = p (the target's row) and S = 1 at
     first, token x is accepted where u q(x) < r(x) / S, and its node becomes the path's end; otherwise r
     becomes max(r / S - q, 0) and S its sum (without draft_probs: accepted where u S < r(x), otherwise x
-    leaves r and S).  The next token is drawn from r, in the order of tokens, by draw_uniforms.  So the
-    accepted tokens and the next one have the target's distribution whatever the drafter's is.
-    ``path`` has the accepted nodes' indices, node 0 first, then -1.  Sums are of whole numbers: results
-    are the same bit for bit from call to call.
+    leaves r and S).  A refusal that would leave nothing leaves r and S as they are.  The next token is drawn
+    from r, in the order of tokens, by draw_uniforms.  So the accepted tokens and the next one have the
+    target's distribution whatever the drafter's is.  ``path`` has the accepted nodes' indices, node 0 first,
+    then -1.  Sums are of whole numbers: results are the same bit for bit from call to call.
 
-    A request without nodes accepts 0 and gives -1, as one whose row is all zeros gives -1.  Parents that
-    are not earlier nodes (those nodes are never asked), tokens outside the vocabulary (refused) and lengths
-    outside the bounds (as without nodes) are reported by ``check_device_errors``."""
+    A request without nodes accepts 0 and gives -1; one whose row at the path's end is zeros (nothing of 2^-52
+    or more) gives -1.  Parents that are not earlier nodes (those nodes are never asked), tokens outside the
+    vocabulary (refused) and lengths outside the bounds (as without nodes) are reported by
+    ``check_device_errors``."""
     return _lib.ops().verify_tokens(target_probs, draft_probs, tokens, parents, node_offsets, node_uniforms,
                                     draw_uniforms, max_nodes, _flag(target_probs), PDL if pdl is None else pdl)
 

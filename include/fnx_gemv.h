@@ -605,13 +605,14 @@ int fnx_tree_attention8(const void* q, int64_t q_sn, int64_t q_sh, const void* k
  * starts the path).  The children of the path's end are asked in order, with r = target's row and
  * S = 1 at first: token x with node_uniforms u is accepted where u q(x) < r(x) / S, and becomes the
  * path's end; else r = max(r / S - q, 0), S = sum r.  With draft NULL: accepted where u S < r(x),
- * else S -= r(x), r(x) = 0.  Then next[b] is drawn from r, in the order of tokens, by
- * draw_uniforms[b].  Sums are of whole numbers (2^52 r, truncated), r in 32 bits: results are the same bit for
- * bit from call to call.  Probabilities count as within [0, 1], NaN as 0, and random numbers below 0
- * and NaN as 0; where nothing is left r stays what it was.
+ * else S -= r(x), r(x) = 0.  A refusal that would leave nothing leaves r and S as they are.  Then
+ * next[b] is drawn from r, in the order of tokens, by draw_uniforms[b].  Sums are of whole numbers
+ * (2^52 r, truncated), r in 32 bits: results are the same bit for bit from call to call.
+ * Probabilities count as within [0, 1], NaN as 0, and random numbers below 0 and NaN as 0.
  *  path int32 [batch, max_nodes]: the accepted nodes' indices, node 0 first, then -1; accepted int32
  *  [batch]: their number; next int64 [batch].  A request without nodes: 0 accepted, next -1; next is
- *  -1 too where the row at the path's end is zeros.  rows of probabilities 2^21 wide at most.
+ *  -1 too where the row at the path's end is zeros (nothing of 2^-52 or more).  rows of probabilities
+ *  2^21 wide at most.
  * A parent that is not an earlier node records FNX_DEVERR_TREE (such nodes are not asked; -1 is no
  * error), a token outside the vocabulary FNX_DEVERR_TOKEN (refused), lengths outside the bounds
  * FNX_DEVERR_LENGTHS (as without nodes).

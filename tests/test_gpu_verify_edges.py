@@ -1,0 +1,117 @@
+"""verify_tokens on the GPU where its rules meet their ends, against walks in exact arithmetic.
+
+Siblings that cover a row: probabilities are multiples of 2^-25 and random numbers of 2^-24, so u S and S - r take less
+than 53 bits and every comparison of the kernel is exact, as its sums are: paths and tokens are compared for equality."""
+
+from fractions import Fraction
+
+import numpy as np
+import pytest
+import torch
+
+from tests.gpu_util import dev
+
+pytestmark = pytest.mark.gpu
+
+
+def _fx():
+    import flash_next_rtxpro6000_b200 as fx
+
+    return fx
+
+
+def _call(p, q, tokens, parents, offsets, u, w, max_nodes):
+    d = dev()
+    to = lambda x, t: torch.as_tensor(np.asarray(x), dtype=t).to(d)  # noqa: E731
+    args = (to(p, torch.float32), None if q is None else to(q, torch.float32), to(tokens, torch.int64),
+            to(parents, torch.int32), to(offsets, torch.int32), to(u, torch.float32), to(w, torch.float32))
+    out = _fx().verify_tokens(*args, max_nodes=max_nodes)
+    again = _fx().verify_tokens(*args, max_nodes=max_nodes)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+    return [x.tolist() for x in out]
+
+
+def _exact_walk(p, tokens, parents, u, w):
+    """(path, next token) of one request without drafter probabilities; p {token: Fraction} of each node."""
+    path, r, s = [0], dict(p[0]), Fraction(1)
+    for i in range(1, len(tokens)):
+        if parents[i] != path[-1]:
+            continue
+        x = tokens[i]
+        if Fraction(float(u[i])) * s < r.get(x, 0):
+            path.append(i)
+            r, s = dict(p[i]), Fraction(1)
+        elif sum(v for t, v in r.items() if t != x) > 0:  # else nothing would be left: r stays
+            s = max(s - r.get(x, 0), Fraction(0))
+            r[x] = Fraction(0)
+    total = sum(r.values())
+    if total == 0:
+        return path, -1
+    aim, run = min(Fraction(float(w)) * total, total - Fraction(1, 2**52)), Fraction(0)
+    for t in sorted(r):
+        run += r[t]
+        if aim < run:
+            return path, t
+
+
+def test_siblings_that_cover_a_row_leave_it_a_token():
+    """Two tokens share a row whose sum is 1 - 2^-25; both are drafted, and both refused."""
+    p = np.zeros((3, 40), np.float32)
+    p[:, 7], p[:, 30] = 0.5, 0.5 - 2.0**-25
+    u = [0.0, 1 - 2.0**-24, 1 - 2.0**-24]
+    path, accepted, tokens = _call(p, None, [1, 7, 30], [-1, 0, 0], [0, 3], u, [0.25], 3)
+    assert (path, accepted, tokens) == ([[0, -1, -1]], [1], [30])
+    # what stays is asked again by the same token's next sibling: 1 / 4 of 1 / 2 is below it
+    p = np.concatenate([p, p[:1]])
+    path, accepted, tokens = _call(p, None, [1, 7, 30, 30], [-1, 0, 0, 0], [0, 4], u + [0.25], [0.0], 4)
+    assert (path, accepted, tokens) == ([[0, 3, -1, -1]], [2], [7])
+    # a row with one token and less than 1 in all
+    p = np.zeros((3, 40), np.float32)
+    p[:, 39] = 0.25
+    path, accepted, tokens = _call(p, None, [1, 39, 5], [-1, 0, 0], [0, 3], [0.0, 0.5, 0.5], [0.5], 3)
+    assert (path, accepted, tokens) == ([[0, -1, -1]], [1], [39])
+    _fx().check_device_errors()
+
+
+@pytest.mark.parametrize("V", [2, 3, 50, 4097, 151936])
+def test_siblings_over_the_support_of_rows(V):
+    """Every token that has probability drafted in some order, some twice, by random numbers near 1 for the most part; rows
+    that sum to 1, to 1 - 2^-25 and to less."""
+    rng = np.random.default_rng(V)
+    p, tokens, parents, u, offsets, want = [], [], [], [], [0], []
+    w = rng.integers(0, 2**24, 60) * 2.0**-24
+    for b in range(60):
+        n = int(rng.integers(2, 9))
+        rows = []
+        for _ in range(n):
+            k = min(int(rng.integers(1, 5)), V)
+            cut = np.sort(rng.choice(2**25 - 1, k - 1, replace=False) + 1)
+            share = np.diff(np.concatenate([[0], cut, [2**25]]))
+            kind = rng.integers(0, 3)
+            share = share // 4 if kind == 1 and share.min() >= 4 else share
+            share[-1] -= 1 if kind == 2 and share[-1] > 1 else 0
+            share = np.array([s if s < 2**24 else s // 2 * 2 for s in share])  # 24 bits
+            at = rng.choice(min(V, 300), k, replace=False) * max(V // 300, 1)
+            rows.append({int(t): Fraction(int(s), 2**25) for t, s in zip(at, share)})
+        par = [-1] + [int(rng.integers(0, 2)) if i > 1 and rng.random() < 0.3 else 0 for i in range(1, n)]
+        tok, seen = [0], {}
+        for i in range(1, n):  # the parent's support in turn
+            support = sorted(rows[par[i]])
+            tok.append(support[seen.get(par[i], 0) % len(support)])
+            seen[par[i]] = seen.get(par[i], 0) + 1
+        uu = np.where(rng.random(n) < 0.85, 2**24 - 1 - rng.integers(0, 2, n), rng.integers(0, 2**24, n)) * 2.0**-24
+        want.append(_exact_walk(rows, tok, par, uu, w[b]))
+        for row in rows:
+            x = np.zeros(V, np.float32)
+            for t, s in row.items():
+                x[t] = float(s)
+            p.append(x)
+        tokens += tok
+        parents += par
+        u += uu.tolist()
+        offsets.append(offsets[-1] + n)
+    path, accepted, drawn = _call(np.stack(p), None, tokens, parents, offsets, u, w, 8)
+    for b, (right, token) in enumerate(want):
+        assert [x for x in path[b] if x >= 0] == right and accepted[b] == len(right) and drawn[b] == token, b
+    assert min(drawn) >= 0
+    _fx().check_device_errors()
