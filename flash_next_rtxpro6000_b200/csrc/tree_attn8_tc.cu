@@ -35,7 +35,12 @@ struct Tc8 {
   static constexpr int kK = D == 256 ? 2 : D == 128 ? (RT == 2 && !kAlt ? 2 : 3) : 5;  // chunks of the rings
   static constexpr int kV = D == 256 ? 2 : D == 128 ? (RT == 2 && !kAlt ? 3 : 4) : 5;
   static constexpr int kRows = kAlt ? 128 : 128 * RT;
-  static constexpr int kScales = kK + (kAlt ? 4 : 2);
+  // Scales of tiles: those of tile i are written when the scores of tile i - kK have been computed, which is when its keys
+  // get their chunk.  Scores wait for the output product of the same set's tile two before, and these products go tile by
+  // tile, so while a set reads the scales of tile a, scores get no further than a + 1 where there is one set, and a + 3
+  // where two take turns.  With two row tiles it is a + 2: where a is the second row tile's last and the next segment has
+  // one row tile only, its scores wait for the first one's products alone, and a's has been issued.
+  static constexpr int kScales = kK + (kAlt ? 4 : RT == 2 ? 3 : 2);
   static constexpr int kAhead = D == 256 ? 2 : D == 128 ? 4 : 6;  // 8-bit tiles in flight
   static constexpr bool kQInTmem = D == 256;
   static constexpr int kLoad = 4 * RT, kIssue = kLoad + 8;  // first loading, first issuing warp
@@ -49,8 +54,6 @@ struct Tc8 {
     uint8_t v[kV][kChunk];
     uint4 raw[2][kAhead][kTile * D / 16];  // keys and values as they lie in the cache, by lane
     float2 raw_scales[kAhead][4];
-    // A tile's scores follow its keys, and are computed two tiles (of a set's own) ahead of its weights at most: when
-    // keys reach the chunk that a tile's had kK tiles before, the softmax of the tile kScales before has ended.
     float4 scales[kScales][kTile / kGroup];
     float2 stat[kAlt ? 128 : 1];  // the second set's references and sums
     float factor[kQInTmem ? 128 : 1];  // of the rows' scores
