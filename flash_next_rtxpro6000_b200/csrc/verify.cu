@@ -16,10 +16,10 @@
 // row has: the walk goes back to the refusal that took the last one and goes on from there with that token alone.
 //
 // Then the next token is drawn from r by the request's own random number: the path's tokens and this one have the
-// target's distribution.  r is held in 32 bits, as p and q are: r / S - q is p times a reciprocal in two 32-bit parts, by
-// two fused multiply-adds, so it is off by half a step of its own whatever cancels.  Sums are of whole numbers
-// (trunc(2^52 r), 64 bits), exact in any order: the split of a row changes nothing.  (In 64-bit floating point throughout
-// 32 trees of 16 nodes took 48 us against 25.)  S and the tests are in 64 bits.
+// target's distribution.  r, S and the tests are in 64-bit floating point, r / S - q in one rounding but for that of 1 / S:
+// what cancels in one refusal keeps the bits that the next ones need.  (In 32 bits choices within some 2^-23 of their
+// borders fell either way.)  Sums are of whole numbers (trunc(2^52 r), 64 bits), exact in any order: the split of a row
+// changes nothing.
 //
 // Bound: one read of the row at the path's end (of p, and of q where a child was refused there), since probabilities
 // of drafted tokens alone decide all else; for few requests, the chain of steps.  A cluster of CTAs has a request,
@@ -54,40 +54,43 @@ struct VerifySmem {
   int parent[kNodes];
   int64_t token[kNodes];
   float uniform[kNodes], p[kNodes], q[kNodes];  // of the node's token, in its parent's rows
-  float2 inv[kNodes];      // 1 / S of the refusals at the path's end, in two parts
+  double inv[kNodes];      // 1 / S of the refusals at the path's end
   int refused[kNodes];     // their tokens (without drafter probabilities) ...
-  int refused_node[kNodes];     // ... and nodes, and S before
+  int refused_node[kNodes];  // ... and nodes, and S before
   double left_before[kNodes];
   int path[kNodes];
   u64 warp_sum[kVW];       // of the last pass
   u64 total[2];            // this CTA's, of the last passes
   u64 tile_sum[kTileV];    // of the warp's part that holds the token
   // the walk
-  int i, current, length, rounds, kept_rounds, step;
+  int i, current, length, rounds, step;
   int sole;                // the only token left, or -1: its refusals change nothing (without drafter probabilities)
   bool summed;             // the last pass was over what is left now
   double left;             // S
 };
 
 __device__ __forceinline__ float probability(float v) { return __saturatef(v); }  // NaN counts as 0
-// trunc(2^52 r) for r in [0, 2): the significand at 2^55 and up, shifted down.
-__device__ __forceinline__ u64 whole(float r) {
-  const uint32_t bits = __float_as_uint(r);
-  const u64 m = (u64)((bits & 0x007FFFFFu) | 0x00800000u) << 32;
-  return m >> min(127 + 23 - 52 + 32 - (int)(bits >> 23), 63);
+// A float in [0, 1] as a double by its bits, since conversions have a quarter of the arithmetic's rate: half of a pair's are
+// made this way.  Those below 2^-126, 0 among them, become some 2^-127: enough for a q, which is taken away, and for sums.
+__device__ __forceinline__ double widen_bits(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return __hiloint2double((int)((b >> 3) + 0x38000000u), (int)(b << 29));
 }
-__device__ __forceinline__ float2 reciprocal(double s) {
-  const double r = 1.0 / s;
-  const float hi = (float)r;
-  return make_float2(hi, (float)(r - (double)hi));
-}
-// What `rounds` refusals leave of n tokens' p.
+// trunc(2^52 r) for r in [0, 1]: the lowest bits of 1 + r, rounded towards 0.
+__device__ __forceinline__ u64 whole(double r) { return (u64)(__double_as_longlong(__dadd_rz(r, 1.0)) - 0x3FF0000000000000ll); }
+__device__ __forceinline__ u64 part(float v) { return whole(widen_bits(probability(v))); }
+// What `rounds` refusals leave of n tokens' r; negative numbers become 0 by their sign bit.
 template <int N>
-__device__ __forceinline__ void residual(const float2* inv, int rounds, float (&p)[N], const float (&q)[N]) {
+__device__ __forceinline__ void residual(const double* inv, int rounds, double (&r)[N], const double (&q)[N]) {
+#pragma unroll 1
   for (int k = 0; k < rounds; ++k) {
-    const float2 by = inv[k];
+    const double by = inv[k];
 #pragma unroll
-    for (int e = 0; e < N; ++e) p[e] = fmaxf(fmaf(p[e], by.y, fmaf(p[e], by.x, -q[e])), 0.f);
+    for (int e = 0; e < N; ++e) {
+      const double x = __fma_rn(r[e], by, -q[e]);
+      const int hi = __double2hiint(x), keep = ~(hi >> 31);
+      r[e] = __hiloint2double(hi & keep, __double2loint(x) & keep);
+    }
   }
 }
 
@@ -111,6 +114,8 @@ __device__ __forceinline__ float4 four(const float* row, int v, int end) {
 
 }  // namespace
 
+// Four blocks an SM, at 64 registers and some 40 bytes of spills: 32 clusters of 16 run at once then (without drafter
+// probabilities 16.0 us against 17.5 with three, with them 37.8 against 37.4 where most children are refused).
 template <bool kVec>
 __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ VerifySmem s;
@@ -181,10 +186,14 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
           q[4 * f] = y.x, q[4 * f + 1] = y.y, q[4 * f + 2] = y.z, q[4 * f + 3] = y.w;
         }
 #pragma unroll
-        for (int e = 0; e < 4 * kFlight; ++e) p[e] = probability(p[e]), q[e] = probability(q[e]);
-        residual(s.inv, rounds, p, q);
+        for (int f = 0; f < kFlight; ++f) {
+          double r[4], y[4];
 #pragma unroll
-        for (int e = 0; e < 4 * kFlight; ++e) sum += whole(p[e]);
+          for (int e = 0; e < 4; ++e) r[e] = (double)probability(p[4 * f + e]), y[e] = widen_bits(probability(q[4 * f + e]));
+          residual(s.inv, rounds, r, y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum += whole(r[e]);
+        }
       }
     } else {
       for (int v = v0 + lane * 4; v < v1; v += kFlight * kTileV) {
@@ -193,11 +202,11 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
         for (int f = 0; f < kFlight; ++f) p[f] = four<kVec>(prow, v + f * kTileV, v1);
 #pragma unroll
         for (int f = 0; f < kFlight; ++f)
-          sum += whole(probability(p[f].x)) + whole(probability(p[f].y)) + whole(probability(p[f].z)) + whole(probability(p[f].w));
+          sum += part(p[f].x) + part(p[f].y) + part(p[f].z) + part(p[f].w);
       }
       if (!a.draft && lane < rounds) {  // refused tokens' shares are taken out again
         for (int k = lane; k < rounds; k += 32)
-          if (s.refused[k] >= v0 && s.refused[k] < v1) sum -= whole(probability(prow[s.refused[k]]));
+          if (s.refused[k] >= v0 && s.refused[k] < v1) sum -= part(prow[s.refused[k]]);
       }
     }
     sum = warp_total(sum);
@@ -218,54 +227,55 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
   };
 
   for (;;) {
-    if (tid == 0) {
-      int step = STEP_DRAW;
-      for (; s.i < n; ++s.i) {
-        const int i = s.i;
-        if (s.parent[i] != s.current) continue;
+    if (tid == 0) {  // the state in registers: a node costs no more than its loads
+      int step = STEP_DRAW, i = s.i, current = s.current, length = s.length, rounds = s.rounds, sole = s.sole;
+      double left = s.left;
+      bool summed = s.summed;
+      for (; i < n; ++i) {
+        if (s.parent[i] != current) continue;
+        const int x = (int)s.token[i];
         bool accept;
         if (a.draft) {
-          float r[1] = {s.p[i]};
-          const float q[1] = {s.q[i]};
-          residual(s.inv, s.rounds, r, q);
-          accept = (double)s.uniform[i] * (double)s.q[i] * s.left < (double)r[0];
+          double r[1] = {(double)s.p[i]};
+          const double q[1] = {(double)s.q[i]};
+          residual(s.inv, rounds, r, q);
+          accept = (double)s.uniform[i] * q[0] * left < r[0];
           if (!accept) {
-            s.inv[s.rounds] = reciprocal(s.left);
+            s.inv[rounds] = 1.0 / left;
             step = STEP_PASS;
           }
         } else {
           double r = (double)s.p[i];
-          for (int k = 0; k < s.rounds; ++k)
-            if (s.refused[k] == (int)s.token[i]) r = 0.0;
-          accept = (double)s.uniform[i] * s.left < r;
-          if (!accept && r > 0.0 && (int)s.token[i] != s.sole) {
-            s.left_before[s.rounds] = s.left;
-            s.left = fmax(s.left - r, 0.0);
-            s.refused_node[s.rounds] = i;
-            s.refused[s.rounds++] = (int)s.token[i];
+          for (int k = 0; k < rounds; ++k)
+            if (s.refused[k] == x) r = 0.0;
+          accept = (double)s.uniform[i] * left < r;
+          if (!accept && r > 0.0 && x != sole) {
+            s.left_before[rounds] = left;
+            s.refused_node[rounds] = i;
+            s.refused[rounds++] = x;
+            left = fmax(left - r, 0.0);
           }
         }
         if (accept) {
-          s.path[s.length++] = i;
-          s.current = i;
-          s.rounds = 0;
-          s.left = 1.0;
-          s.sole = -1;
-          s.summed = false;
+          s.path[length++] = i;
+          current = i;
+          rounds = 0;
+          left = 1.0;
+          sole = -1;
+          summed = false;
         }
         if (step == STEP_PASS) break;
       }
-      s.step = step;
+      s.step = step, s.i = i, s.current = current, s.length = length, s.rounds = rounds, s.sole = sole;
+      s.left = left;
+      s.summed = summed;
     }
     __syncthreads();
-    const bool refusal = s.step == STEP_PASS;
-    if (!refusal && s.summed) break;
-    const u64 all = pass(s.rounds + (refusal ? 1 : 0));
-    if (!refusal) {
-      if (all > 0 || a.draft) break;
+    if (s.step == STEP_DRAW) {
+      if (s.summed || pass(s.rounds) > 0 || a.draft) break;
       // the last refusal that took something; those behind it took tokens below 2^-52
       int k = s.rounds - 1;
-      while (k >= 0 && whole(s.p[s.refused_node[k]]) == 0) --k;
+      while (k >= 0 && part(s.p[s.refused_node[k]]) == 0) --k;
       if (k < 0) break;  // the row is zeros
       __syncthreads();   // all have read what the next lines change
       if (tid == 0) {
@@ -274,17 +284,18 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
         s.i = s.refused_node[k] + 1;
         s.rounds = k;
       }
-    } else {
-      if (tid == 0) {
-        ++s.i;
-        s.summed = all > 0;
-        if (all > 0) {
-          ++s.rounds;
-          s.left = (double)all * (1.0 / kUnit);
-        }
-      }
-      __syncthreads();
+      continue;
     }
+    const u64 all = pass(s.rounds + 1);
+    if (tid == 0) {
+      ++s.i;
+      s.summed = all > 0;
+      if (all > 0) {
+        ++s.rounds;
+        s.left = (double)all * (1.0 / kUnit);
+      }
+    }
+    __syncthreads();
   }
   // --- the draw
   u64 before = 0, all = 0;
@@ -317,12 +328,14 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
       auto weights = [&](int v, u64 (&x)[4]) {
         const float4 p = four<kVec>(prow, v, p1);
         const float4 q = pairs ? four<kVec>(qrow, v, p1) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float ps[4] = {probability(p.x), probability(p.y), probability(p.z), probability(p.w)};
-        const float qs[4] = {probability(q.x), probability(q.y), probability(q.z), probability(q.w)};
-        if (pairs) residual(s.inv, s.rounds, ps, qs);
+        const float ps[4] = {p.x, p.y, p.z, p.w}, qs[4] = {q.x, q.y, q.z, q.w};
+        double r[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = (double)probability(ps[e]), y[e] = widen_bits(probability(qs[e]));
+        if (pairs) residual(s.inv, s.rounds, r, y);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = whole(ps[e]);
+          x[e] = whole(r[e]);
           if (!a.draft)
             for (int k = 0; k < s.rounds; ++k)
               if (s.refused[k] == v + e) x[e] = 0;

@@ -607,7 +607,7 @@ int fnx_tree_attention8(const void* q, int64_t q_sn, int64_t q_sh, const void* k
  * path's end; else r = max(r / S - q, 0), S = sum r.  With draft NULL: accepted where u S < r(x),
  * else S -= r(x), r(x) = 0.  A refusal that would leave nothing leaves r and S as they are.  Then
  * next[b] is drawn from r, in the order of tokens, by draw_uniforms[b].  Sums are of whole numbers
- * (2^52 r, truncated), r in 32 bits: results are the same bit for bit from call to call.
+ * (2^52 r, truncated), r in 64 bits: results are the same bit for bit from call to call.
  * Probabilities count as within [0, 1], NaN as 0, and random numbers below 0 and NaN as 0.
  *  path int32 [batch, max_nodes]: the accepted nodes' indices, node 0 first, then -1; accepted int32
  *  [batch]: their number; next int64 [batch].  A request without nodes: 0 accepted, next -1; next is

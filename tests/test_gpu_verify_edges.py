@@ -115,3 +115,62 @@ def test_siblings_over_the_support_of_rows(V):
         assert [x for x in path[b] if x >= 0] == right and accepted[b] == len(right) and drawn[b] == token, b
     assert min(drawn) >= 0
     _fx().check_device_errors()
+
+
+# A refusal's residual in 64 bits: each element is rounded at 2^-53 of r / S, and S, a sum of V truncations, is off by
+# V 2^-52 of 1 at most.  Relative to an r(x) that is at least 2^-8 of the r(x) / S it came from (children with less are not
+# drafted here) and S of 2^-4 at least, ten refusals at V = 700 stay below 10 * 2^8 * (2^-53 + 700 * 2^-52 * 2^4) < 2^-26:
+# random numbers 2^-25.5 above a refusal's border, or as far below an acceptance's, decide as the formula does.
+MARGIN = 2.0**-25.5
+
+
+def _bordering(p, q, rng, refusals):
+    """Tokens and random numbers of one node's children: `refusals` that are just refused, then one that is just accepted;
+    and what is left of the row."""
+    tokens, u, r, s = [], [], p.astype(np.longdouble), np.longdouble(1)
+    p, q = p.astype(np.longdouble), q.astype(np.longdouble)
+    for k in range(refusals + 1):
+        share = r / s
+        last = k == refusals
+        # borders r(x) / (S q(x)) inside (0, 1), without much cancellation in what made r(x)
+        border = np.where(q > 0, share / np.maximum(q, np.longdouble(1e-30)), 0)
+        fit = np.flatnonzero((border > 2.0**-8) & (border < 0.99) & (share > 2.0**-8 * p))
+        x = int(rng.choice(fit))
+        at = np.float32(border[x])
+        if last:
+            while np.longdouble(at) * q[x] >= share[x] * (1 - np.longdouble(MARGIN)):
+                at = np.nextafter(at, np.float32(0))
+        else:
+            while np.longdouble(at) * q[x] < share[x] * (1 + np.longdouble(MARGIN)):
+                at = np.nextafter(at, np.float32(1))
+            r = np.maximum(share - q, 0)
+            s = r.sum()
+            assert s > 2.0**-4
+        tokens.append(x)
+        u.append(float(at))
+    return tokens, u
+
+
+def test_residuals_keep_the_bits_that_choices_need():
+    """Up to ten refusals one after the other at random numbers that are the next or next but one above their borders, then
+    one acceptance as near below its border."""
+    rng = np.random.default_rng(21)
+    B, V = 200, 700
+    soft = lambda z: (np.exp(z) / np.exp(z).sum(1, keepdims=True)).astype(np.float32)  # noqa: E731
+    x = rng.standard_normal((B, V)) * 2
+    p, q = soft(x), soft(x + rng.standard_normal((B, V)) * 1.5)
+    rows, draft, tokens, parents, u, offsets, want = [], [], [], [], [], [0], []
+    for b in range(B):
+        k = int(rng.integers(0, 11))
+        t, v = _bordering(p[b], q[b], rng, k)
+        tokens += [0] + t
+        u += [0.0] + v
+        parents += [-1] + [0] * (k + 1)
+        rows += [p[b]] * (k + 2)
+        draft += [q[b]] * (k + 2)
+        offsets.append(offsets[-1] + k + 2)
+        want.append([0, k + 1] + [-1] * 10)
+    path, accepted, _ = _call(np.stack(rows), np.stack(draft), tokens, parents, offsets, u, np.full(B, 0.5), 12)
+    wrong = [b for b in range(B) if path[b] != want[b]]
+    assert not wrong, (len(wrong), wrong[:5], [path[b] for b in wrong[:5]])
+    _fx().check_device_errors()
