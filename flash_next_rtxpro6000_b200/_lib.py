@@ -39,8 +39,9 @@ DEVICE_ERRORS = {
     16: "TREE: a parent that is not an earlier node",
     17: "TOKEN: a drafted token outside the vocabulary",
     18: "SCALE: a cache scale that no append writes",
+    19: "PROBS: a row of probabilities that sums to 64 or more",
 }
-ARGUMENT_ERRORS = (9, 11, 12, 13, 14, 15, 16, 17, 18)  # those that are no waits
+ARGUMENT_ERRORS = (9, 11, 12, 13, 14, 15, 16, 17, 18, 19)  # those that are no waits
 
 EXPORTED = (
     "fnx_set_dense_path",

@@ -574,7 +574,7 @@ enum ErrCode : int { ERR_NONE = 0, ERR_WAIT_FULL = 1, ERR_WAIT_EMPTY = 2, ERR_WA
                      ERR_WAIT_RFREE = 4, ERR_DRAIN = 5, ERR_WAIT_X = 6, ERR_WAIT_PEER = 7,
                      ERR_PEER_DESYNC = 8, ERR_ROUTES = 9, ERR_WAIT_EXPERT = 10,
                      ERR_RING = 11, ERR_POSITION = 12, ERR_SLOT = 13, ERR_LENGTHS = 14,
-                     ERR_PAGE = 15, ERR_TREE = 16, ERR_TOKEN = 17, ERR_SCALE = 18 };
+                     ERR_PAGE = 15, ERR_TREE = 16, ERR_TOKEN = 17, ERR_SCALE = 18, ERR_PROBS = 19 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);

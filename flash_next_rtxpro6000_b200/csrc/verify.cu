@@ -19,7 +19,8 @@
 // target's distribution.  r, S and the tests are in 64-bit floating point, r / S - q in one rounding but for that of 1 / S:
 // what cancels in one refusal keeps the bits that the next ones need.  (In 32 bits choices within some 2^-23 of their
 // borders fell either way.)  Sums are of whole numbers (trunc(2^52 r), 64 bits), exact in any order: the split of a row
-// changes nothing.
+// changes nothing.  64 bits hold 4,096 in that unit, and a row that is no distribution could sum to more, so sums are
+// capped on their way (by 128 a thread, warp and CTA) and one of 64 or more is an error.
 //
 // Bound: one read of the row at the path's end (of p, and of q where a child was refused there), since probabilities
 // of drafted tokens alone decide all else; for few requests, the chain of steps.  A cluster of CTAs has a request,
@@ -47,6 +48,7 @@ constexpr int kVCluster = 16;        // CTAs of a request
 constexpr int kTileV = 128;          // tokens of a warp's step: four a lane
 constexpr int kFlight = 5;           // steps whose loads are in flight together
 constexpr double kUnit = 4503599627370496.0;  // 2^52
+constexpr u64 kHeavy = 1ull << 58;  // ... and a capped one stays above this when refused tokens (63 at most) are taken out
 
 enum Step : int { STEP_PASS = 0, STEP_DRAW = 1 };
 
@@ -66,6 +68,7 @@ struct VerifySmem {
   int i, current, length, rounds, step;
   int sole;                // the only token left, or -1: its refusals change nothing (without drafter probabilities)
   bool summed;             // the last pass was over what is left now
+  bool heavy;              // a row that is no distribution
   double left;             // S
 };
 
@@ -94,6 +97,11 @@ __device__ __forceinline__ void residual(const double* inv, int rounds, double (
   }
 }
 
+// At most 2^59 - 1, by the upper half.
+__device__ __forceinline__ u64 capped(u64 v) {
+  const uint32_t hi = min((uint32_t)(v >> 32), 0x07FFFFFFu);
+  return ((u64)hi << 32) | (uint32_t)v;
+}
 __device__ __forceinline__ u64 warp_total(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -163,7 +171,7 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
     s.rounds = 0;
     s.left = 1.0;
     s.sole = -1;
-    s.summed = false;
+    s.summed = s.heavy = false;
     s.path[0] = 0;
   }
   __syncthreads();
@@ -195,6 +203,7 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
           for (int e = 0; e < 4; ++e) sum += whole(r[e]);
         }
       }
+      sum = capped(sum);
     } else {
       for (int v = v0 + lane * 4; v < v1; v += kFlight * kTileV) {
         float4 p[kFlight];
@@ -204,6 +213,7 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
         for (int f = 0; f < kFlight; ++f)
           sum += part(p[f].x) + part(p[f].y) + part(p[f].z) + part(p[f].w);
       }
+      sum = capped(sum);
       if (!a.draft && lane < rounds) {  // refused tokens' shares are taken out again
         for (int k = lane; k < rounds; k += 32)
           if (s.refused[k] >= v0 && s.refused[k] < v1) sum -= part(prow[s.refused[k]]);
@@ -211,12 +221,12 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
     }
     sum = warp_total(sum);
     __syncthreads();
-    if (lane == 0) s.warp_sum[warp] = sum;
+    if (lane == 0) s.warp_sum[warp] = capped(sum);
     __syncthreads();
     if (tid == 0) {
       u64 all = 0;
       for (int w = 0; w < kVW; ++w) all += s.warp_sum[w];
-      s.total[phase] = all;
+      s.total[phase] = capped(all);
     }
     cl.sync();
     u64 all = 0;
@@ -290,6 +300,7 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
     if (tid == 0) {
       ++s.i;
       s.summed = all > 0;
+      if (all >= kHeavy) s.heavy = true;  // looked at in the end: a branch here took 38 -> 41 us (32 trees, most refused)
       if (all > 0) {
         ++s.rounds;
         s.left = (double)all * (1.0 / kUnit);
@@ -306,14 +317,17 @@ __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ 
     all += t;
   }
   asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // the others' sums have been read
+  const bool heavy = s.heavy || all >= kHeavy;  // no distribution: as without nodes
   if (rank == 0) {
-    if (tid < a.width) a.path[(int64_t)b * a.width + tid] = tid < s.length ? s.path[tid] : -1;
+    const int length = heavy ? 0 : s.length;
+    if (tid < a.width) a.path[(int64_t)b * a.width + tid] = tid < length ? s.path[tid] : -1;
     if (tid == 0) {
-      a.accepted[b] = s.length;
-      if (all == 0) a.next[b] = -1;
+      a.accepted[b] = length;
+      if (heavy) record_error(a.err, ERR_PROBS);
+      if (heavy || all == 0) a.next[b] = -1;
     }
   }
-  if (all > 0) {
+  if (all > 0 && !heavy) {
     const float given = a.draw_uniforms[b];
     const double u = given > 0.f ? (double)given : 0.0;  // NaN and negative numbers draw the first token
     const u64 reach = __double2ull_rz(__dmul_rn(u, __ull2double_rn(all)));

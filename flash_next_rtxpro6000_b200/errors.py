@@ -4,8 +4,8 @@ Every wait inside the kernels is bounded: a wait that runs out of time records a
 code in its workspace's ``error_flag`` (the first code of a call wins), the kernel leaves
 its loop and the launch completes, so the CUDA context stays usable, but that call's
 outputs are wrong.  The verify-step operators record in the same way what only the device
-can see of their arguments: positions, cache slots, lengths, pages and parents out of
-bounds (codes 12 to 16), which are not followed.  The launch itself reports success; the
+can see of their arguments: positions, cache slots, lengths, pages, parents, tokens, scales
+and sums of probabilities out of bounds (codes 12 to 19), which are not followed.  The launch itself reports success; the
 flag is how the host learns of either.  Nothing on the device clears a flag.
 
 ``check_device_errors`` reads every flag this process has created (the scratch slots,

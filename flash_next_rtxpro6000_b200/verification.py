@@ -52,8 +52,8 @@ def verify_tokens(
 
     A request without nodes accepts 0 and gives -1; one whose row at the path's end is zeros (nothing of 2^-52
     or more) gives -1.  Parents that are not earlier nodes (those nodes are never asked), tokens outside the
-    vocabulary (refused) and lengths outside the bounds (as without nodes) are reported by
-    ``check_device_errors``."""
+    vocabulary (refused), lengths outside the bounds and rows that are no distributions but sum to 64 or more (both
+    as without nodes) are reported by ``check_device_errors``."""
     return _lib.ops().verify_tokens(target_probs, draft_probs, tokens, parents, node_offsets, node_uniforms,
                                     draw_uniforms, max_nodes, _flag(target_probs), PDL if pdl is None else pdl)
 

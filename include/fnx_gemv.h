@@ -97,6 +97,7 @@ typedef void* fnx_stream_t;
 #define FNX_DEVERR_TREE 16         /* a parent that is not an earlier node            */
 #define FNX_DEVERR_TOKEN 17        /* a drafted token outside the vocabulary          */
 #define FNX_DEVERR_SCALE 18        /* a cache scale that no append writes             */
+#define FNX_DEVERR_PROBS 19        /* a row of probabilities that sums to 64 or more  */
 
 /* Split-K and argmax scratch of the dense GEMVs.  Counters and keys must be zero when
  * first used; every launch leaves them zero again (self-resetting, graph-replay safe).
@@ -615,7 +616,8 @@ int fnx_tree_attention8(const void* q, int64_t q_sn, int64_t q_sh, const void* k
  *  2^21 wide at most.
  * A parent that is not an earlier node records FNX_DEVERR_TREE (such nodes are not asked; -1 is no
  * error), a token outside the vocabulary FNX_DEVERR_TOKEN (refused), lengths outside the bounds
- * FNX_DEVERR_LENGTHS (as without nodes).
+ * FNX_DEVERR_LENGTHS (as without nodes), a row, or what a refusal leaves of it, that sums to 64 or
+ * more FNX_DEVERR_PROBS (as without nodes; rows that the path does not sum are not looked at).
  */
 int fnx_verify_tokens(const float* target, int64_t ldt, const float* draft, int64_t ldd,
                       const int64_t* tokens, const int32_t* parents, const int32_t* node_offsets,

@@ -174,3 +174,55 @@ def test_residuals_keep_the_bits_that_choices_need():
     wrong = [b for b in range(B) if path[b] != want[b]]
     assert not wrong, (len(wrong), wrong[:5], [path[b] for b in wrong[:5]])
     _fx().check_device_errors()
+
+
+def test_rows_of_ones_up_to_63():
+    """Elements are clamped to [0, 1], rows are not: a row of 63 ones is drawn from in equal shares."""
+    V, w = 4000, np.array([0.0, 0.25, 0.3, 1 - 2.0**-24], np.float32)
+    p = np.zeros((4, V), np.float32)
+    p[:, 1 : 63 * 63 : 63] = 1.0
+    at = [1 + 63 * min(int(Fraction(float(x)) * 63), 62) for x in w]
+    assert _call(p, None, [0] * 4, [-1] * 4, range(5), [0.0] * 4, w, 1) == [[[0]] * 4, [1] * 4, at]
+    _fx().check_device_errors()
+
+
+@pytest.mark.parametrize("V", [64, 4095, 4096, 4099, 30000, 2**21])
+def test_rows_of_ones_are_no_distributions(V):
+    """What sums to 64 or more is told, whatever 64 bits hold, and such a request is as one without nodes; others are not
+    affected."""
+    fx = _fx()
+
+    def told(*args):
+        out = _call(*args)
+        with pytest.raises(fx.DeviceWaitError, match="PROBS") as e:
+            fx.check_device_errors()
+        assert "wait" not in str(e.value)
+        return out
+
+    p = np.ones((3, V), np.float32)
+    p[1] = 0.0
+    p[1, V - 1] = 0.75
+    out = told(p, None, [0] * 3, [-1] * 3, range(4), [0.0] * 3, [0.5] * 3, 2)
+    assert out == [[[-1, -1], [0, -1], [-1, -1]], [0, 1, 0], [-1, V - 1, -1]]
+    # the row of the path's end, and what refusals leave: with and without drafter probabilities
+    p = np.ones((4, V), np.float32)
+    p[2:] = 0.0
+    p[0, 5] = 0.5
+    p[2:, 7] = 1.0
+    q = np.zeros((4, V), np.float32)
+    q[:, 5] = 1.0
+    for draft in (None, q):
+        args = (p, draft, [0, 5, 0, 5], [-1, 0, -1, 0], [0, 2, 4], [0.0, 0.75, 0.0, 0.75], [0.5, 0.5], 2)
+        if V > 64:
+            assert told(*args) == [[[-1, -1], [0, -1]], [0, 1], [-1, 7]]
+        else:  # 63 are left: the 32nd of them is token 32, behind token 5
+            assert _call(*args) == [[[0, -1], [0, -1]], [1, 1], [32, 7]]
+    # a refusal's sum is told although the path goes on from there
+    if V > 64:
+        p = np.ones((3, V), np.float32)
+        p[0, 5] = 0.5
+        p[2] = 0.0
+        p[2, 7] = 1.0
+        q[:, 9] = 0.25
+        out = told(p[:3], q[:3], [0, 5, 9], [-1, 0, 0], [0, 3], [0.0, 0.75, 0.0], [0.5], 3)
+        assert out == [[[-1, -1, -1]], [0], [-1]]
