@@ -50,6 +50,10 @@ namespace {
 // Lambdas are inlined by force.  Where the compiler left one out (the third kernel of a unit, say), all that it captures went
 // to local memory: 16 rows of 151,936 logits without top-k took 77 us instead of 56.
 #define FNX_INLINE __attribute__((always_inline))
+// The steps' lambdas, unless the unit leaves them to the compiler (sample.cu).
+#ifndef FNX_INLINE_STEP
+#define FNX_INLINE_STEP FNX_INLINE
+#endif
 
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
@@ -676,11 +680,11 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   const double u = uniform > 0.0f ? (double)uniform : 0.0;  // NaN and negative numbers draw the most likely token
 
   // A found token goes to the CTA's own finds, and these to the first CTA's list in one piece.
-  auto find = [&](u64 key) FNX_INLINE {
+  auto find = [&](u64 key) FNX_INLINE_STEP {
     const uint32_t at = next_shared(finds0);
     if (at < (uint32_t)kCap) s.mine_found[at] = key;
   };
-  auto send = [&]() FNX_INLINE {
+  auto send = [&]() FNX_INLINE_STEP {
     __syncthreads();
     const uint32_t m = s.finds;
     if (tid == 0) s.place = atomicAdd(&first.listed, m);
@@ -716,7 +720,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
         Ranked r;
         if (few) r = rank_list(s, sc, held, by_share);
         else by_share = measure(s, sc, st, held);
-        auto ask = [&](int what, u64 value, double share) FNX_INLINE {
+        auto ask = [&](int what, u64 value, double share) FNX_INLINE_STEP {
           return few ? answer(s, r, held, 0, 0, what, value, share) : answer(s, sc, st, held, 0, 0, what, value, share);
         };
         // the list holds at least top_k tokens, or all there are
@@ -863,7 +867,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     __syncthreads();
   }
   // The interval in which the value is reached; each question has a place of its own for the answer.
-  auto bin_of = [&](int place, int want, u64 value, double share) FNX_INLINE {
+  auto bin_of = [&](int place, int want, u64 value, double share) FNX_INLINE_STEP {
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
       if (reached(want, own_count[q + 1], own_sum[q + 1], value, share) &&
@@ -893,7 +897,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   };
 
   // Sends them to its list.
-  auto gather = [&](const Control& c) FNX_INLINE {
+  auto gather = [&](const Control& c) FNX_INLINE_STEP {
     asked(c, [&](u64 key, float) FNX_INLINE { find(key); });
     send();
     cl.sync();
@@ -903,7 +907,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
   // first CTA.
   u64 klo = 0ull, khi = 0ull;
   int shift = 0;
-  auto split = [&](const Control& c) FNX_INLINE {
+  auto split = [&](const Control& c) FNX_INLINE_STEP {
     klo = ~0ull, khi = 0ull;
     asked(c, [&](u64 key, float) FNX_INLINE {
       klo = key < klo ? key : klo;
@@ -972,7 +976,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
       cl.sync();
     }
   } else {
-    auto tell = [&](const Control& c) FNX_INLINE {
+    auto tell = [&](const Control& c) FNX_INLINE_STEP {
       __syncthreads();
       if (tid == 0) {
         s.ctl = c;
@@ -981,7 +985,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
       cl.sync();
     };
     // The token of interval b at which the value is reached; the list is loaded.
-    auto query = [&](int b, int want, u64 value, double share) FNX_INLINE -> Found {
+    auto query = [&](int b, int want, u64 value, double share) FNX_INLINE_STEP -> Found {
       c = Control{OP_GATHER, b, b, 0, -1, 0ull, ~0ull};
       u64 base_count = s.count[b], base_sum = s.sum[b];
       for (;;) {
@@ -1025,7 +1029,7 @@ __global__ void __launch_bounds__(kST, kMany ? 2 : 1) sample_kernel(const __grid
     u64 unused;
     if (few) r = rank_list(s, sc, held, unused);
     int measured = -1;
-    auto from_list = [&](int b, int what, u64 value, double share) FNX_INLINE {
+    auto from_list = [&](int b, int what, u64 value, double share) FNX_INLINE_STEP {
       if (few) {  // weight ahead of the list's tokens: that of an interval after the others is not in it
         u64 base = s.sum[c.bin_lo];
         if (b > c.bin_hi) base += s.sum[b] - s.sum[c.bin_hi + 1];
