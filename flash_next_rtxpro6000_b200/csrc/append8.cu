@@ -22,22 +22,8 @@ namespace {
 
 constexpr int kAT = 256;  // threads
 
-template <typename T> __device__ __forceinline__ float2 two(uint32_t w);
-template <> __device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-template <> __device__ __forceinline__ float2 two<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
 __device__ __forceinline__ float one(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float one(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ uint32_t round_two(float a, float b);
-template <> __device__ __forceinline__ uint32_t round_two<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-template <> __device__ __forceinline__ uint32_t round_two<__half>(float a, float b) {
-  const __half2 p = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
 
 // 16 elements of a head: two runs of eight, which hold whole pairs where the sizes allow 16-byte vectors.
 struct Unit {
@@ -76,7 +62,7 @@ template <typename T>
 __device__ __forceinline__ void values(const Append8Args& a, const Raw& r, const float* row, int u, bool turned, float (&x)[16]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float2 y = two<T>(r.w[i]);
+    const float2 y = two_floats<T>(r.w[i]);
     x[2 * i] = y.x, x[2 * i + 1] = y.y;
   }
   if (!turned) return;
@@ -155,7 +141,7 @@ __device__ __forceinline__ void queries(const Append8Args& a, int cta) {
       if (!live) continue;
       uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = round_two<T>(x[2 * i], x[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) w[i] = round_pair<T>(x[2 * i], x[2 * i + 1]);
       if (kVec) {
         *reinterpret_cast<uint4*>(dst + un.o0) = make_uint4(w[0], w[1], w[2], w[3]);
         *reinterpret_cast<uint4*>(dst + un.o1) = make_uint4(w[4], w[5], w[6], w[7]);

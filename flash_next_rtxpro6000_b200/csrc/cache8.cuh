@@ -32,6 +32,22 @@ __device__ __forceinline__ float power_above(float s) {
   return __uint_as_float((bits + 0x007FFFFFu) & 0xFF800000u);
 }
 
+// Two 16-bit elements as floats, and two floats rounded to 16 bits.
+template <typename T> __device__ __forceinline__ float2 two_floats(uint32_t w);
+template <> __device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <> __device__ __forceinline__ float2 two_floats<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+template <typename T> __device__ __forceinline__ uint32_t round_pair(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t round_pair<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t round_pair<__half>(float lo, float hi) {
+  const __half2 p = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
 // Two values rounded to e4m3 (to the nearest, ties to even; NaN stays NaN), the first in the low byte.
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
   uint16_t r;

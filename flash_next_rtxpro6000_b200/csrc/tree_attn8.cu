@@ -19,9 +19,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -137,7 +134,7 @@ __global__ void __launch_bounds__(32 * MT * WK * TG, 1) tree_attn8_kernel(const 
       const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(rq.n0 + node) * a.q_sn + (int64_t)h * a.q_sh;
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        x[i] = r < live ? query_two<T>(*reinterpret_cast<const uint32_t*>(q + i * 64 + lane * 2)) : make_float2(0.f, 0.f);
+        x[i] = r < live ? two_floats<T>(*reinterpret_cast<const uint32_t*>(q + i * 64 + lane * 2)) : make_float2(0.f, 0.f);
         const float m = fmaxf(fabsf(x[i].x), fabsf(x[i].y));
         amax = fmaxf(amax, m);
       }

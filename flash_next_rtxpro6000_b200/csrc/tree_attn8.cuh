@@ -69,6 +69,11 @@ __device__ __forceinline__ float4 group_scales(const Attn8Args& a, const Place8&
   return group_factors(a, p.ks < 0 ? make_float2(1.f, 1.f) : make_float2(a.k_scale[p.ks], a.v_scale[p.vs]));
 }
 
+// 16 bytes into shared memory, zeros where they are not there.
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 // Whether one of the four bytes is a NaN.
 __device__ __forceinline__ bool has_nan(uint32_t w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0u; }
 
@@ -76,23 +81,6 @@ __device__ __forceinline__ float e4m3_value(uint8_t v) {
   uint32_t lo, hi;
   deq_fp8_word(v, lo, hi);
   return __half2float(*reinterpret_cast<const __half*>(&lo));
-}
-
-// Two query elements as floats.
-template <typename T> __device__ __forceinline__ float2 query_two(uint32_t w);
-template <> __device__ __forceinline__ float2 query_two<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-template <> __device__ __forceinline__ float2 query_two<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
-
-template <typename T> __device__ __forceinline__ uint32_t round_pair(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t round_pair<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-template <> __device__ __forceinline__ uint32_t round_pair<__half>(float lo, float hi) {
-  const __half2 p = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&p);
 }
 
 // Exponent of the power of two that a row with this largest magnitude takes; 0 where it is not finite.

@@ -80,10 +80,6 @@ template <int RT> __device__ __forceinline__ void take_registers8() {
   else asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
 }
 
-__device__ __forceinline__ void cp16_or_zero(void* to, const void* from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-
 // Two fp32 operations an instruction, and the largest of three.
 __device__ __forceinline__ unsigned long long two(float lo, float hi) {
   unsigned long long r;
@@ -133,10 +129,9 @@ __device__ __forceinline__ void load8(const Attn8Args& a, typename Tc8<D, RT, kA
   using Cfg = Tc8<D, RT, kAlt>;
   constexpr int P = Cfg::kAhead;
   const int N = kValues ? Cfg::kV : Cfg::kK;
-  constexpr int kGroups = 1;  // of 16 keys, a warp
   constexpr int kLanesRow = D / 16;         // lanes of a row: 16 elements each
   constexpr int kRowsPer = 32 / kLanesRow;  // rows of one instruction
-  constexpr int J = 16 / kRowsPer;          // instructions of a group
+  constexpr int J = 16 / kRowsPer;          // instructions of a warp's 16 keys of a tile
   const int lane = threadIdx.x & 31, col = lane % kLanesRow;
   const uint8_t* from = reinterpret_cast<const uint8_t*>(kValues ? a.v_cache : a.k_cache) + col * 16;
   uint8_t* ring = kValues ? s.v[0] : s.k[0];
@@ -148,39 +143,30 @@ __device__ __forceinline__ void load8(const Attn8Args& a, typename Tc8<D, RT, kA
   const int page_step = kTile / a.page_size, in_step = kTile % a.page_size;
   const int block_shift = 31 - __clz(a.block);
   int t = 0, t1 = 0, left = 0, queued = 0;  // tile of the segment, its end, keys from the warp's first on; tiles found
-  int at_page[kGroups], at_in[kGroups];
+  int at_page = 0, at_in = 0;
   const int* table = nullptr;
-  struct Spot {  // the warp's keys of a tile: one page and one block hold a group
-    int page[kGroups], in[kGroups], head, live;
+  struct Spot {  // the warp's keys of a tile, a group: one page and one block hold them
+    int page, in, head, live;
   };
   auto find = [&]() {
-    Spot p;
-    p.head = p.live = 0;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) p.page[g] = p.in[g] = 0;
+    Spot p{0, 0, 0, 0};
     if (t == t1) {
       if (!sg.next()) return p;
       t = sg.t0;
       t1 = sg.t1;
       table = a.page_table + (int64_t)sg.b * a.table_ld;
-      const int pos = t * kTile + pw * kGroups * kGroup;
+      const int pos = t * kTile + pw * kGroup;
       left = sg.rq.ctx + sg.rq.nodes - pos;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        at_page[g] = (pos + g * kGroup) / a.page_size;
-        at_in[g] = pos + g * kGroup - at_page[g] * a.page_size;
-      }
+      at_page = pos / a.page_size;
+      at_in = pos - at_page * a.page_size;
     }
     p.head = sg.head;
     p.live = left;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      if (left > g * kGroup) p.page[g] = __ldg(table + at_page[g]);
-      p.in[g] = at_in[g];
-      at_page[g] += page_step;
-      at_in[g] += in_step;
-      if (at_in[g] >= a.page_size) at_in[g] -= a.page_size, ++at_page[g];
-    }
+    if (left > 0) p.page = __ldg(table + at_page);
+    p.in = at_in;
+    at_page += page_step;
+    at_in += in_step;
+    if (at_in >= a.page_size) at_in -= a.page_size, ++at_page;
     left -= kTile;
     ++t;
     ++queued;
@@ -190,30 +176,26 @@ __device__ __forceinline__ void load8(const Attn8Args& a, typename Tc8<D, RT, kA
   const int64_t* st = kValues ? a.vc_st : a.kc_st;
   const int64_t step = st[1] * kRowsPer;
   from += st[1] * row;
-  uint4* raw = s.raw[kValues][0] + pw * kGroups * J * 32 + lane;  // the lane's own places, J of a group
+  uint4* raw = s.raw[kValues][0] + pw * J * 32 + lane;  // the lane's own J places
   constexpr int kTileRaw = kTile * D / 16;
   auto issue = [&](int slot, const Spot& p) {
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      int live = p.live - g * kGroup;
-      if (live > 0 && (p.page[g] < 0 || p.page[g] >= a.num_pages)) {
-        if (lane == 0) record_error(a.err, ERR_PAGE);
-        live = 0;
-      }
-      const uint8_t* at = from + (int64_t)p.page[g] * st[0] + (int64_t)p.in[g] * st[1] + (int64_t)p.head * st[2];
-#pragma unroll
-      for (int j = 0; j < J; ++j, at += step) {
-        const bool there = j * kRowsPer + row < live;
-        cp16_or_zero(raw + slot * kTileRaw + (g * J + j) * 32, there ? at : from, there);
-      }
+    int live = p.live;
+    if (live > 0 && (p.page < 0 || p.page >= a.num_pages)) {
+      if (lane == 0) record_error(a.err, ERR_PAGE);
+      live = 0;
     }
-    if (!kValues && lane < kGroups) {  // a lane a group
-      float2* to = &s.raw_scales[slot][pw * kGroups + lane];
-      const int page = lane ? p.page[kGroups - 1] : p.page[0], in = lane ? p.in[kGroups - 1] : p.in[0];
-      if (p.live > lane * kGroup && page >= 0 && page < a.num_pages) {
-        const int blk = in >> block_shift;
-        cp_async4(&to->x, a.k_scale + (int64_t)page * a.ks_st[0] + (int64_t)blk * a.ks_st[1] + (int64_t)p.head * a.ks_st[2]);
-        cp_async4(&to->y, a.v_scale + (int64_t)page * a.vs_st[0] + (int64_t)blk * a.vs_st[1] + (int64_t)p.head * a.vs_st[2]);
+    const uint8_t* at = from + (int64_t)p.page * st[0] + (int64_t)p.in * st[1] + (int64_t)p.head * st[2];
+#pragma unroll
+    for (int j = 0; j < J; ++j, at += step) {
+      const bool there = j * kRowsPer + row < live;
+      cp16_or_zero(smem_u32(raw + slot * kTileRaw + j * 32), there ? at : from, there);
+    }
+    if (!kValues && lane == 0) {
+      float2* to = &s.raw_scales[slot][pw];
+      if (p.live > 0 && p.page >= 0 && p.page < a.num_pages) {
+        const int blk = p.in >> block_shift;
+        cp_async4(&to->x, a.k_scale + (int64_t)p.page * a.ks_st[0] + (int64_t)blk * a.ks_st[1] + (int64_t)p.head * a.ks_st[2]);
+        cp_async4(&to->y, a.v_scale + (int64_t)p.page * a.vs_st[0] + (int64_t)blk * a.vs_st[1] + (int64_t)p.head * a.vs_st[2]);
       } else {
         *to = make_float2(1.f, 1.f);
       }
@@ -238,27 +220,24 @@ __device__ __forceinline__ void load8(const Attn8Args& a, typename Tc8<D, RT, kA
       break;
     }
     uint8_t* to = ring + slot * Cfg::kChunk + (col >> 2) * kBlockBytes;
+    uint4 x[J];
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      uint4 x[J];
+    for (int j = 0; j < J; ++j) x[j] = raw[stage * kTileRaw + j * 32];
 #pragma unroll
-      for (int j = 0; j < J; ++j) x[j] = raw[stage * kTileRaw + (g * J + j) * 32];
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int r = (pw * kGroups + g) * kGroup + j * kRowsPer + row;
-        uint4 y[2];
-        deq_fp8_word(x[j].x, y[0].x, y[0].y);
-        deq_fp8_word(x[j].y, y[0].z, y[0].w);
-        deq_fp8_word(x[j].z, y[1].x, y[1].y);
-        deq_fp8_word(x[j].w, y[1].z, y[1].w);
-        // lanes of neighbouring 64-element blocks take the two halves in turn: eight lanes, eight places
-        const int odd = (col >> 2) & 1, u = (col & 3) * 2;
-        *reinterpret_cast<uint4*>(to + r * 128 + (((u + odd) ^ (r & 7)) << 4)) = odd ? y[1] : y[0];
-        *reinterpret_cast<uint4*>(to + r * 128 + (((u + 1 - odd) ^ (r & 7)) << 4)) = odd ? y[0] : y[1];
-      }
+    for (int j = 0; j < J; ++j) {
+      const int r = pw * kGroup + j * kRowsPer + row;
+      uint4 y[2];
+      deq_fp8_word(x[j].x, y[0].x, y[0].y);
+      deq_fp8_word(x[j].y, y[0].z, y[0].w);
+      deq_fp8_word(x[j].z, y[1].x, y[1].y);
+      deq_fp8_word(x[j].w, y[1].z, y[1].w);
+      // lanes of neighbouring 64-element blocks take the two halves in turn: eight lanes, eight places
+      const int odd = (col >> 2) & 1, u = (col & 3) * 2;
+      *reinterpret_cast<uint4*>(to + r * 128 + (((u + odd) ^ (r & 7)) << 4)) = odd ? y[1] : y[0];
+      *reinterpret_cast<uint4*>(to + r * 128 + (((u + 1 - odd) ^ (r & 7)) << 4)) = odd ? y[0] : y[1];
     }
-    if (!kValues && lane < kGroups)  // which copied them
-      s.scales[scale_at.at][pw * kGroups + lane] = group_factors(a, s.raw_scales[stage][pw * kGroups + lane]);
+    if (!kValues && lane == 0)  // which copied them
+      s.scales[scale_at.at][pw] = group_factors(a, s.raw_scales[stage][pw]);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(full[slot]));
@@ -450,7 +429,8 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
         auto eight = [&](int k, int c) {
           return from[k] ? *reinterpret_cast<const uint4*>(from[k] + c * 64) : make_uint4(0u, 0u, 0u, 0u);
         };
-        constexpr int kHold = D / 64 < 2 ? 1 : 2;  // 128 elements of a row at a time
+        constexpr int kHold = 2;  // times 64 elements of a row at a time
+        static_assert(!Cfg::kQInTmem || D / 64 % kHold == 0, "whole steps");
         uint4 held[kHold][8];
 #pragma unroll 1
         for (int c0 = 0; c0 < D / 64; c0 += kHold) {
@@ -465,7 +445,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
               const uint32_t w[4] = {held[c][k].x, held[c][k].y, held[c][k].z, held[c][k].w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float2 y = query_two<T>(w[e]);
+                const float2 y = two_floats<T>(w[e]);
                 top[k] = max_three(top[k], fabsf(y.x), fabsf(y.y));
               }
             }
@@ -489,8 +469,8 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
             uint32_t z[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float2 v = query_two<T>(w[e]);
-              z[e] = round_pair<H>(v.x * top[k], v.y * top[k]);
+              const float2 v = two_floats<T>(w[e]);
+              z[e] = pack2<H>(v.x * top[k], v.y * top[k]);
             }
             *reinterpret_cast<uint4*>(to + y * 128 + (((lane & 7) ^ (y & 7)) << 4)) = make_uint4(z[0], z[1], z[2], z[3]);
           }
@@ -519,7 +499,7 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float2 y = query_two<T>(w[e]);
+              const float2 y = two_floats<T>(w[e]);
               amax = fmaxf(amax, fmaxf(fabsf(y.x), fabsf(y.y)));
             }
           }
@@ -532,8 +512,8 @@ __global__ void __launch_bounds__((4 * RT + 12) * 32, 1) tree_attn8_tc_kernel(co
           const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 z = query_two<T>(w[e]);
-            y[e] = round_pair<H>(z.x * up, z.y * up);
+            const float2 z = two_floats<T>(w[e]);
+            y[e] = pack2<H>(z.x * up, z.y * up);
           }
         };
         if (!(kAlt && rt == 1)) {  // the other set stores them
