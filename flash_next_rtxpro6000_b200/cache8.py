@@ -52,7 +52,10 @@ def rotary_append8(
     context_lens[b] + index.  A block that gets tokens takes the smallest power of two as its scale by which
     its new elements divided fit into e4m3 (at most 448), at least 2^-40, and at least its old scale where
     tokens of the context stay in it; these take the new scale too.  What lies in a block behind the context
-    when the call begins does not count.  Infinite elements and NaN are stored as NaN and do not count.
+    when the call begins does not count.  So drafts that are refused later leave nothing behind but their scale in
+    the block that they shared with the context: its tokens keep what they lost to it (elements below 2^-6 of the
+    scale are rounded to multiples of 2^-9 of it), and the block's next tokens take at least that scale.  Infinite
+    elements and NaN are stored as NaN and do not count.
 
     Rows of no request are rotated and not stored.  Positions outside the table, lengths that contradict
     each other or the page table, and pages outside the cache are reported by ``check_device_errors``;
@@ -84,8 +87,10 @@ def tree_attention8(
     values e4m3 with the scales of their blocks.
 
     Scales outside [2^-40, 2^120] or NaN, which ``rotary_append8`` does not write, are reported by
-    ``check_device_errors`` and count as 2^-40; others need not be powers of two.  Weights are rounded to
-    fp16 for the second product, whatever q's type."""
+    ``check_device_errors`` and count as 2^-40; others need not be powers of two.  The scales of the values that a
+    row sees should lie within a factor of 2^60 of each other.  Weights are rounded to fp16 for the second product,
+    whatever q's type.  The cache takes half of a 16-bit one's memory; the time is about the same, since the chain of
+    a tile's scores and weights bounds both."""
     flag, partials, _ = _scratch(q)
     return _lib.ops().tree_attention8(q, k_cache, v_cache, k_scale, v_scale, page_table, context_lens, node_offsets,
                                       tree_mask, max_nodes, max_context, scale, out, lse, partials, flag,

@@ -78,7 +78,8 @@ def compact_nodes(
     bf16 or fp16, or float8_e4m3fn with k_scale and v_scale ([layers,] pages, page_size / block,
     kv_heads) as of ``rotary_append8``.  There a block's scale becomes the largest of those of the tokens that
     come to it and, where tokens of the context stay in it, its own; elements whose scale changes are rounded
-    again (exact for powers of two, but for elements 2^14 below their block's largest).
+    again (exact for powers of two, but for elements 2^14 below their block's largest).  It does not fall again: tokens
+    keep the scale that refused drafts brought to their block (``rotary_append8``).
 
     Paths that do not rise or reach past the pages, and pages outside the cache, are reported by
     ``check_device_errors``; such a request is left as it was.  No page may be moved in for two requests."""

@@ -565,7 +565,8 @@ int fnx_token_probs(const void* logits, int64_t ldl, int dtype, int M, int V,
  * node_offsets[b + 1] - 1, any number) stored at places context_lens[b] + index of its pages.  A
  * block that gets tokens has the scale s' = the smallest power of two, 2^-40 at least, by which the
  * largest finite magnitude of its new elements divided is at most 448, and not below the block's old
- * scale where tokens of the context stay in it, which take the new scale too.  Elements are rounded
+ * scale where tokens of the context stay in it, which take the new scale too and keep it, also where
+ * the new tokens are drafts that are refused later.  Elements are rounded
  * to the nearest, infinite ones and NaN to NaN.  Rows of no request are rotated and not stored.
  * Lengths that contradict each other or the table record FNX_DEVERR_LENGTHS, pages outside the cache
  * FNX_DEVERR_PAGE: nothing is stored there.  No block may belong to two requests of a call.  At most
