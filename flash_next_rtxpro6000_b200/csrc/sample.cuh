@@ -26,11 +26,11 @@
 //     both values' intervals are sent at once.  An interval with more tokens than the list holds
 //     (many ties, or one token far from the others) is split again by order key and token index
 //     until it fits.
-// Measured (B200): one row of 151,936 bf16 logits 10 us with a top-k of 50, 22 to 37 without top-k (of some
-// 57,000 cycles the histogram's pass takes 15,000 to 19,000, its exponentials and shared-memory adds in
-// equal parts, the gathering 9,000, the exchanges about 1,500 each); 16 such rows in fp32 19 and 42 to 50 us; 128
-// rows of 248,320 52 and 142 to 158 us (175 to 234 with a division and a 64-bit shift a logit in place of quotient()
-// and add_share()).  Two other ways were measured: a list of the likely tokens, made while all weights are added up, in
+// Measured (B200): one row of 151,936 bf16 logits 10 us with a top-k of 50, 21 to 25 without filters or with top-p or
+// min-p, 36 where top-p's interval holds more tokens than the list, 37 with a top-k of 5,000 (of some 57,000 cycles the
+// histogram's pass takes 15,000 to 19,000, its exponentials and shared-memory adds in equal parts, the gathering 9,000, the
+// exchanges about 1,500 each); 16 such rows in fp32 19, 41 to 44 and 62 us; 128 rows of 248,320 51 and 144 to 151 us (175 to
+// 234 with a division and a 64-bit shift a logit in place of quotient() and add_share()).  Two other ways were measured: a list of the likely tokens, made while all weights are added up, in
 // place of the histogram (31 and 92 us where it decides, 65 and 240 where it does not and the histogram follows), and a
 // histogram of counts, then exact sums around the interval that it points at (44 to 52, 128 to 240 us).  The form for
 // many rows has 64 registers a thread and spills some 500 bytes of them.
@@ -1078,10 +1078,12 @@ namespace {
 template <bool kAll>
 int launch_rows(SampleArgs a, cudaStream_t stream) {
   const int size = a.type == LOGITS_F32 ? 4 : 2;
-  // Rows for which clusters of 8 would not all run at once share the SMs two CTAs each, in clusters
-  // of 4: 16 rows of 151,936 fp32 logits take 30 us in clusters of 8 and 50 in clusters of 4, 128
-  // rows of 248,320 take 227 and 137.  (A CTA of a cluster of 4 may hold too many logits for its
-  // histogram's sums above 2^20.)
+  // Rows for which clusters of 8 would not all run at once share the SMs two CTAs each, in clusters of 4.  Measured, in
+  // clusters of 8 and of 4: sampling 14 fp32 rows of 151,936 without filters 24 and 36 us, 19 rows 44 and 36, 128 rows of
+  // 248,320 with all kinds of filters 205 and 100; token_probs with top-p, 14 rows 29 and 41, 19 rows 52 and 41, the 128 rows
+  // 248 and 150.  From 15 to 18 rows some clusters of 8 wait for others: rows of one kind would be faster in clusters
+  // of 4 (16 rows 41 and 34), rows of several kinds, whose short ones end early, are not (24 and 35; token_probs 32 and 44).
+  // (A CTA of a cluster of 4 may hold too many logits for its histogram's sums above 2^20.)
   const bool many = (int64_t)a.M * 8 > num_sms() && a.V <= 1 << 20;
   const int C = many ? 4 : 8;
   const void* k = kAll ? (many ? probs_fn_many(a.type) : probs_fn_one(a.type)) : many ? sample_fn_many(a.type) : sample_fn_one(a.type);

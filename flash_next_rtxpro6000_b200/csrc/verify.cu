@@ -27,8 +27,9 @@
 // each a slice of the rows.  Every CTA walks the tree by itself, so the cluster only exchanges sums: one pass over
 // the slice for each refusal by q, whose sums also serve the final draw.  The token is found from the sums of CTAs,
 // then of warps, then by one more read of the 1/(16 x 8) of the row that holds it.
-// Measured (B200): a chain of 6 nodes, vocabulary of 151,936, 8.5 us; 32 trees of 16 nodes 19.5 us, which is up to four
-// passes over the 1.2 MB of one request's two rows, on 16 of the 148 SMs (in clusters of 8 25 us, with 512 threads 26).
+// Measured (B200): a chain of 6 nodes, vocabulary of 151,936, 8.4 us; 32 trees of 16 nodes 19.9 us, which is up to four
+// passes over the 1.2 MB of one request's two rows, on 16 of the 148 SMs (in clusters of 8 25 us, with 512 threads 26,
+// both with r in 32 bits, which took 8.5 and 19.5).
 #include <cooperative_groups.h>
 
 #include "fnx_common.cuh"
