@@ -123,7 +123,7 @@ __device__ __forceinline__ float4 four(const float* row, int v, int end) {
 
 }  // namespace
 
-// Four blocks an SM, at 64 registers and some 40 bytes of spills: 32 clusters of 16 run at once then (without drafter
+// Four blocks an SM, at 64 registers and some 70 bytes of spills: 32 clusters of 16 run at once then (without drafter
 // probabilities 16.0 us against 17.5 with three, with them 37.8 against 37.4 where most children are refused).
 template <bool kVec>
 __global__ void __launch_bounds__(kVT, 4) verify_kernel(const __grid_constant__ VerifyArgs a) {

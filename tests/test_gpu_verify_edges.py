@@ -226,3 +226,17 @@ def test_rows_of_ones_are_no_distributions(V):
         q[:, 9] = 0.25
         out = told(p[:3], q[:3], [0, 5, 9], [-1, 0, 0], [0, 3], [0.0, 0.75, 0.0], [0.5], 3)
         assert out == [[[-1, -1, -1]], [0], [-1]]
+
+
+@pytest.mark.parametrize("drafts", [True, False])
+@pytest.mark.parametrize("chain", [True, False])
+@pytest.mark.parametrize("counts,V", [([6], 151936), ([5, 1, 0, 16, 2], 4096), ([64], 3001), ([9] * 20, 517), ([33, 64, 12], 250)])
+def test_walks_in_64_bits_at_a_border_of_2_to_the_minus_28(monkeypatch, counts, V, chain, drafts):
+    """Residuals are rounded at 2^-53, and sums lose V 2^-52 < 2^-34 of 1; over an S of 2^-4 at least, a few refusals one
+    after the other stay below 2^-28 of what is compared and drawn from."""
+    from tests import test_gpu_verification as other
+
+    monkeypatch.setattr(other, "NEAR_CHOICE", 2.0**-28)
+    for seed in range(4):
+        other.Drafts(counts, V, seed=100 * seed + V, drafts=drafts, chain=chain, noise=2.0).check()
+    _fx().check_device_errors()
